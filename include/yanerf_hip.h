@@ -15,13 +15,15 @@
  *   - Return 0 on success; non-zero on a bad argument or launch failure, with a message available from
  *     yanerf_last_error() (thread-local).
  *   - Floating point tensors are fp32, row-major and contiguous with the reference's shapes, so torch
- *     tensors pass through without copies. Index tensors are int64.
+ *     tensors pass through without copies. Index tensors are int64. (The learned-code entry points take
+ *     their element and index types as arguments.)
  *   - Empty bundles (zero rays / points / elements) are valid, as empty tensors are in the reference: the call
  *     returns 0 before touching its per-ray buffers, which may then be NULL (torch gives an empty CUDA tensor a
  *     NULL data pointer). yanerf_mlp_backward with zero points writes all-zero parameter gradients (nn.Linear's
  *     gradient over an empty batch); yanerf_scatter_rays with zero rays writes the background image.
  *   - Randomness: a counter-based Philox4x32-10 stream keyed by (seed, offset); every random draw can
- *     instead be INJECTED by passing the uniforms/normals the reference consumed (test mode).
+ *     instead be INJECTED by passing the uniforms/normals the reference consumed (test mode). Dropout
+ *     masks, which the reference has not, are a stated function of (seed, offset) instead.
  */
 #ifndef YANERF_HIP_H
 #define YANERF_HIP_H
@@ -47,7 +49,7 @@ extern "C" {
 const char* yanerf_last_error(void);
 int yanerf_version(void);
 /* First 16 hex digits of the SHA-256 of the sources this library was compiled from (render.hip, mlp.hip,
-   common.hpp, this header, the Makefile, in that order): the Python binding refuses a library whose id does not
+   codes.hip, common.hpp, this header, the Makefile, in that order): the Python binding refuses a library whose id does not
    match the sources beside it (a stale prebuilt .so). Not a reference entry point. */
 const char* yanerf_build_id(void);
 
@@ -254,6 +256,44 @@ int yanerf_adam_table(float* params, float* grads, float* exp_avg, float* exp_av
  * rng_base pointers of yanerf_raygen / yanerf_refine / yanerf_raymarch_opts) += rng_delta, state[1] (the Adam table
  * index) += 1. One thread, stream-ordered. */
 int yanerf_step_advance(uint64_t* state, uint64_t rng_delta, void* stream);
+
+/* ------------------------------------------------------------------------------------------------
+ * Learned codes (not reference entry points: the reference takes its conditional MLP's global_codes, nerf_mlp.py:158-163,
+ * from the caller). Embedding lookup with scaling and dropout, its gradient, and dropout.
+ *   Types: YANERF_TYPE_*; ids are int32 or int64 (id_bytes 4 or 8), contiguous.
+ *   Dropout with probability p: element e (row-major index into the output) is kept where word e % 4 of
+ *   Philox4x32-10(key = seed, counter = (e / 4, offset + *rng_base)) >= T = round(p * 2^32), and is then multiplied by
+ *   1 / (1 - p); it is 0 otherwise, whatever the input holds (T = 2^32, so p = 1: all 0). The mask is never stored: the
+ *   backward evaluates it anew from the same (seed, offset).
+ *   rng_base: NULL, or 1 device u64 added to `offset` (a graph-captured step advances it on the device).
+ *   rng_used: NULL, or 1 device u64 that receives offset + *rng_base, for a backward that runs after the base moved on
+ *     (pass it as that call's rng_base with offset 0). Not written where a call has no elements.
+ *   Sums and products are fp32, each output is rounded once. N, V < 2^31; N * D, V * D <= 2^38.
+ * ---------------------------------------------------------------------------------------------- */
+#define YANERF_TYPE_F32 0
+#define YANERF_TYPE_BF16 1
+#define YANERF_TYPE_F16 2
+
+/* y[e] = keep(e) x[e] / (1 - p) for n contiguous elements; also the gradient, with the output's gradient as x. y may
+ * be x. */
+int yanerf_dropout(const void* x, int type, int64_t n, double p, uint64_t seed, uint64_t offset,
+                   const uint64_t* rng_base, uint64_t* rng_used, void* y, void* stream);
+/* out[n][d] = scale / (1 - p) * table[ids[n]][d] * keep(n D + d), n < N, d < D; row v of the table starts at element
+ * v * table_stride. An id outside [0, V) gives a zero row and sets *oob = 1 (a device int, may be NULL; never cleared
+ * here): the caller decides when to read it back. */
+int yanerf_embedding_forward(const void* table, int table_type, int64_t table_stride, const void* ids, int id_bytes,
+                             int64_t N, int64_t V, int64_t D, double scale, double p, uint64_t seed, uint64_t offset,
+                             const uint64_t* rng_base, uint64_t* rng_used, void* out, int out_type, int* oob,
+                             void* stream);
+/* Bytes of yanerf_embedding_backward's workspace (its contents need not be set), -1 for sizes out of range. */
+int64_t yanerf_embedding_bwd_workspace_bytes(int64_t N, int64_t V, int64_t D);
+/* grad_table[v][d] = scale / (1 - p) * sum over n with ids[n] = v of keep(n D + d) g[n][d]: every row is written, rows
+ * that no id names and row padding_idx (-1: none) with zeros. Ids outside [0, V) take no part. The order of each sum
+ * depends on the ids alone (no float atomics). */
+int yanerf_embedding_backward(const void* g, int g_type, const void* ids, int id_bytes, int64_t N, int64_t V,
+                              int64_t D, int64_t padding_idx, double scale, double p, uint64_t seed, uint64_t offset,
+                              const uint64_t* rng_base, void* grad_table, int table_type, void* workspace,
+                              void* stream);
 
 #ifdef __cplusplus
 }

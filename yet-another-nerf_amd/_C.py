@@ -14,7 +14,7 @@ from pathlib import Path
 PKG = Path(__file__).resolve().parent
 LIB_PATH = Path(os.environ.get("YANERF_HIP_LIB", PKG / "libyanerf_hip.so"))
 # the files the library's build id hashes, in the Makefile's order (csrc/Makefile: SRC_SHA)
-SOURCES = [PKG / "csrc" / f for f in ("render.hip", "mlp.hip", "common.hpp")] + [
+SOURCES = [PKG / "csrc" / f for f in ("render.hip", "mlp.hip", "codes.hip", "common.hpp")] + [
     PKG.parent / "include" / "yanerf_hip.h", PKG / "csrc" / "Makefile"]
 
 
@@ -30,6 +30,8 @@ PREC_BF16 = 1
 PREC_F32X3 = 2  # fp32 as three bf16 terms, six bf16 MFMAs per product (include/yanerf_hip.h)
 PREC_BF16S = 3  # bf16 with bf16 storage throughout (no fp8 sections; include/yanerf_hip.h)
 
+TYPE_F32, TYPE_BF16, TYPE_F16 = 0, 1, 2  # element types of the learned-code entry points
+
 # every symbol include/yanerf_hip.h declares (checked by tests/test_capi.py)
 EXPORTS = (
     "yanerf_last_error", "yanerf_version", "yanerf_build_id", "yanerf_raygen", "yanerf_mlp_num_params",
@@ -39,7 +41,8 @@ EXPORTS = (
     "yanerf_mlp_backward", "yanerf_mlp_backward_phase", "yanerf_composite_forward", "yanerf_composite_backward",
     "yanerf_composite_train", "yanerf_sample_pdf",
     "yanerf_refine", "yanerf_rgb_loss", "yanerf_adam", "yanerf_adam_scalars", "yanerf_adam_table", "yanerf_step_advance",
-    "yanerf_scatter_rays",
+    "yanerf_scatter_rays", "yanerf_dropout", "yanerf_embedding_forward", "yanerf_embedding_bwd_workspace_bytes",
+    "yanerf_embedding_backward",
 )
 
 
@@ -110,6 +113,12 @@ def lib():
         "yanerf_adam_scalars": (c_int, [c_double, c_double, c_double, i64, POINTER(c_float)]),
         "yanerf_adam_table": (c_int, [P, P, P, P, i64, P, P, c_double, c_double, c_double, c_double, i64, P]),
         "yanerf_step_advance": (c_int, [P, c_uint64, P]),
+        "yanerf_dropout": (c_int, [P, c_int, i64, c_double, c_uint64, c_uint64, P, P, P, P]),
+        "yanerf_embedding_forward": (c_int, [P, c_int, i64, P, c_int, i64, i64, i64, c_double, c_double, c_uint64,
+                                             c_uint64, P, P, P, c_int, P, P]),
+        "yanerf_embedding_bwd_workspace_bytes": (i64, [i64, i64, i64]),
+        "yanerf_embedding_backward": (c_int, [P, c_int, P, c_int, i64, i64, i64, i64, c_double, c_double, c_uint64,
+                                              c_uint64, P, P, c_int, P, P]),
     }
     for name, (res, args) in sig.items():
         fn = getattr(L, name)

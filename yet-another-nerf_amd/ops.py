@@ -6,7 +6,8 @@ ROCm device tensors and raises otherwise: there is no CPU/torch fallback for the
 from __future__ import annotations
 
 import ctypes
-from contextlib import contextmanager
+import math
+from contextlib import contextmanager, nullcontext
 from dataclasses import dataclass
 from typing import List, Optional, Sequence, Tuple
 
@@ -475,3 +476,195 @@ def adam_step(params: torch.Tensor, grads: torch.Tensor, exp_avg: torch.Tensor, 
     _C.check(_C.lib().yanerf_adam(_p(params), _p(grads), _p(exp_avg), _p(exp_avg_sq), params.numel(), float(lr),
                                   float(betas[0]), float(betas[1]), float(eps), float(weight_decay), int(step),
                                   _stream()), "yanerf_adam")
+
+
+# ----------------------------------------------------------------------------------------- learned codes
+_TYPES = {torch.float32: _C.TYPE_F32, torch.bfloat16: _C.TYPE_BF16, torch.float16: _C.TYPE_F16}
+_U64 = 0xFFFFFFFFFFFFFFFF
+
+
+def _code_type(what: str, dtype: torch.dtype) -> int:
+    if dtype not in _TYPES:
+        raise TypeError(f"{what}: element type {dtype} is not supported (float32, bfloat16, float16)")
+    return _TYPES[dtype]
+
+
+def _probability(what: str, p) -> float:
+    p = float(p)
+    if not 0.0 <= p <= 1.0:
+        raise ValueError(f"{what}: dropout probability {p} is not in [0, 1]")
+    return p
+
+
+def _on(dev: torch.device):
+    """The launch context of `dev`: kernels of a tensor on another device than the current one run on that device."""
+    return nullcontext() if dev.index == torch.cuda.current_device() else torch.cuda.device(dev)
+
+
+def _mask_rng(what: str, p: float, rng, rng_base: Optional[torch.Tensor], dev: torch.device, n: int):
+    """(seed, offset) of a dropout mask over n elements; (0, 0) where none is drawn (p 0)."""
+    if rng_base is not None:
+        _dev(rng_base)
+        if rng_base.numel() != 1 or rng_base.dtype not in (torch.int64, torch.uint64) or rng_base.device != dev:
+            raise ValueError(f"{what}: rng_base must be one int64 / uint64 element on {dev}")
+    if p == 0.0:
+        return 0, 0
+    if rng is None:
+        return RNG.next(n)
+    seed, off = rng
+    return int(seed) & _U64, int(off) & _U64
+
+
+class _MaskState:
+    """What a backward needs to draw a forward's mask again: (seed, offset) by value, or, with an rng_base (whose value
+    may have moved on by then), the offset that the forward's kernel used, kept on the device."""
+
+    def __init__(self, p: float, seed: int, offset: int, rng_base: Optional[torch.Tensor], keep: bool):
+        self.p, self.seed, self.offset = p, seed, offset
+        self.base = rng_base if p > 0.0 else None
+        self.used = torch.empty(1, dtype=torch.int64, device=rng_base.device) if keep and self.base is not None else None
+
+    def forward_args(self):
+        return self.p, self.seed, self.offset, _p(self.base), _p(self.used)
+
+    def backward_args(self):
+        return (self.p, self.seed, self.offset, None) if self.used is None else (self.p, self.seed, 0, _p(self.used))
+
+
+class _DropoutFn(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, p, seed, offset, rng_base):
+        ctx.mask = _MaskState(p, seed, offset, rng_base, ctx.needs_input_grad[0])
+        x = x.contiguous()
+        y = torch.empty_like(x)
+        with _on(x.device):
+            _C.check(_C.lib().yanerf_dropout(_p(x), _TYPES[x.dtype], x.numel(), *ctx.mask.forward_args(), _p(y),
+                                             _stream()), "yanerf_dropout")
+        return y
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, g):
+        g = g.contiguous()
+        out = torch.empty_like(g)
+        with _on(g.device):
+            _C.check(_C.lib().yanerf_dropout(_p(g), _TYPES[g.dtype], g.numel(), *ctx.mask.backward_args(), None, _p(out),
+                                             _stream()), "yanerf_dropout")
+        return out, None, None, None, None
+
+
+def dropout(x: torch.Tensor, p: float, *, rng: Optional[Tuple[int, int]] = None,
+            rng_base: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """Zero each element of x (float32, bfloat16 or float16, any shape) with probability p and multiply the others by
+    1 / (1 - p). The mask is a function of a Philox counter (include/yanerf_hip.h): it is never stored, and the backward
+    draws it again. A dropped element is 0 even where x is infinite or NaN.
+
+    rng: the (seed, offset) of the mask; the default takes the next of the module stream, which follows
+    torch.manual_seed. rng_base: one int64 element on x's device that is added to offset when the kernel runs (a captured
+    step advances it, so each replay draws another mask; the backward uses the forward's, also if the base has moved)."""
+    _dev(x)
+    _code_type("dropout", x.dtype)
+    p = _probability("dropout", p)
+    seed, off = _mask_rng("dropout", p, rng, rng_base, x.device, x.numel())
+    return _DropoutFn.apply(x, p, seed, off, rng_base)
+
+
+_ID_FLAGS: dict = {}  # device -> sticky int32 flag of ids outside their table (set by the lookup's kernel, cleared here)
+
+
+def _id_flag(dev) -> Optional[torch.Tensor]:
+    f = _ID_FLAGS.get(dev)
+    if f is None and not torch.cuda.is_current_stream_capturing():  # a capture's memory is the graph's own
+        f = _ID_FLAGS[dev] = torch.zeros(1, dtype=torch.int32, device=dev)
+    return f
+
+
+def check_embedding_ids(dev) -> None:
+    """Raise if any lookup on `dev` since the last check met an id outside its table (one host read-back for any number
+    of lookups; skipped while a stream is being captured into a graph)."""
+    dev = torch.device(dev)
+    f = _ID_FLAGS.get(dev if dev.index is not None else torch.device(dev.type, torch.cuda.current_device()))
+    if f is None or torch.cuda.is_current_stream_capturing():
+        return
+    if int(f.item()):
+        f.zero_()
+        raise IndexError("embedding: an id lies outside its table")
+
+
+class _EmbeddingFn(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, table, ids, scale, padding_idx, p, seed, offset, rng_base, out_dtype):
+        V, D = table.shape
+        ctx.mask = _MaskState(p, seed, offset, rng_base, ctx.needs_input_grad[0])
+        ctx.dims = (V, D, table.dtype, scale, padding_idx)
+        if D > 1 and table.stride(1) != 1:
+            table = table.contiguous()
+        ids = ids.contiguous()
+        out = torch.empty(*ids.shape, D, dtype=out_dtype, device=table.device)
+        with _on(table.device):
+            _C.check(_C.lib().yanerf_embedding_forward(
+                _p(table), _TYPES[table.dtype], table.stride(0), _p(ids), ids.element_size(), ids.numel(), V, D, scale,
+                *ctx.mask.forward_args(), _p(out), _TYPES[out_dtype], _p(_id_flag(table.device)), _stream()),
+                "yanerf_embedding_forward")
+        if ctx.needs_input_grad[0]:
+            ctx.save_for_backward(ids)
+        return out
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, g):
+        V, D, dtype, scale, pad = ctx.dims
+        (ids,) = ctx.saved_tensors
+        N = ids.numel()
+        g = g.contiguous()
+        grad = torch.empty(V, D, dtype=dtype, device=g.device)
+        with _on(g.device):
+            nb = _C.lib().yanerf_embedding_bwd_workspace_bytes(N, V, D)
+            ws = torch.empty(max(nb, 1), dtype=torch.uint8, device=g.device)
+            _C.check(_C.lib().yanerf_embedding_backward(
+                _p(g), _TYPES[g.dtype], _p(ids), ids.element_size(), N, V, D, pad, scale, *ctx.mask.backward_args(),
+                _p(grad), _TYPES[dtype], _p(ws), _stream()), "yanerf_embedding_backward")
+        return grad, None, None, None, None, None, None, None, None
+
+
+def embedding(table: torch.Tensor, ids: torch.Tensor, *, scale: float = 1.0, padding_idx: Optional[int] = None,
+              dropout: float = 0.0, out_dtype: Optional[torch.dtype] = None, rng: Optional[Tuple[int, int]] = None,
+              rng_base: Optional[torch.Tensor] = None, check: bool = True) -> torch.Tensor:
+    """scale * table[ids], rows of `table` [V, D] (float32, bfloat16 or float16; rows may be strided) by integer `ids`
+    (int32 or int64, any shape), as [*ids.shape, D] of `out_dtype` (default: the table's). With dropout > 0 the result is
+    dropped out in the same kernel: the mask of `dropout()` over the result, with the same `rng` / `rng_base`.
+
+    The gradient of the table sums the rows' gradients in fp32 in an order fixed by the ids (sorted, no float atomics:
+    the same bits on every run) and is dense: zeros for rows that no id names and for row `padding_idx` (which may count
+    from the end, as in torch.nn.Embedding).
+
+    An id outside [0, V) gives a zero row and sets a flag that `check_embedding_ids` reads back and raises on: here when
+    `check` (a host synchronisation; a loop over ids that it made itself passes check=False), never inside a graph
+    capture."""
+    _dev(table, ids)
+    if table.dim() != 2:
+        raise ValueError(f"embedding: the table must be [V, D], got {tuple(table.shape)}")
+    out_dtype = table.dtype if out_dtype is None else out_dtype
+    _code_type("embedding", table.dtype)
+    _code_type("embedding", out_dtype)
+    if ids.dtype not in (torch.int32, torch.int64):
+        raise TypeError(f"embedding: ids must be int32 or int64, got {ids.dtype}")
+    if ids.device != table.device:
+        raise RuntimeError(f"embedding: ids on {ids.device}, table on {table.device}")
+    V, D = table.shape
+    if V == 0 and ids.numel():
+        raise IndexError("embedding: ids into an empty table")
+    pad = -1
+    if padding_idx is not None:
+        if not -V <= padding_idx < V:
+            raise ValueError(f"embedding: padding_idx {padding_idx} is outside a table of {V} rows")
+        pad = int(padding_idx) % V
+    scale = float(scale)
+    if not math.isfinite(scale):
+        raise ValueError("embedding: scale is not finite")
+    p = _probability("embedding", dropout)
+    seed, off = _mask_rng("embedding", p, rng, rng_base, table.device, ids.numel() * D)
+    out = _EmbeddingFn.apply(table, ids, scale, pad, p, seed, off, rng_base, out_dtype)
+    if check:
+        check_embedding_ids(table.device)
+    return out
