@@ -64,7 +64,7 @@ def bwd(**kw):
 @pytest.mark.parametrize("call", [fwd, bwd])
 @pytest.mark.parametrize("kw,msg", [
     (dict(tt=7), "type"), (dict(ib=2), "ids of 2"), (dict(N=-1), "negative"), (dict(V=-1), "negative"),
-    (dict(D=-1), "negative"), (dict(N=1 << 31), "2^31"), (dict(V=1 << 31), "2^31"), (dict(N=1 << 30, D=1 << 9), "2^38"),
+    (dict(D=-1), "negative"), (dict(N=1 << 31), "2^31"), (dict(V=1 << 31), "2^31"), (dict(N=1 << 30, D=1 << 9), "2^38"), (dict(D=(1 << 24) + 1), "2^24"),
     (dict(V=1 << 30, D=1 << 9), "2^38"), (dict(scale=float("inf")), "scale"), (dict(scale=float("nan")), "scale"),
     (dict(p=1.01), "probability"), (dict(p=float("nan")), "probability"), (dict(ids=None), "null")])
 def test_embedding_c_refusals(call, kw, msg):

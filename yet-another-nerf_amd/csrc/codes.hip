@@ -12,6 +12,7 @@
 // The gradient sorts the positions by id with a stable sort, so the terms of a row are added in an order that only the
 // ids fix: no float atomics, the same bits on every run.
 #include <cmath>
+#include <type_traits>
 
 #include "common.hpp"
 
@@ -29,6 +30,13 @@ inline void with_type(int t, F&& f) {
   if (t == kF32) f(float{});
   else if (t == kBf16) f(__bf16{});
   else f(_Float16{});
+}
+
+// f(I{}) with I the index type of `bytes`
+template <typename F>
+inline void with_index(int bytes, F&& f) {
+  if (bytes == 8) f(int64_t{});
+  else f(int32_t{});
 }
 
 // workgroups for `work` of them, bounded so that a launch stays under 2^32 threads (the kernels stride over the rest)
@@ -65,29 +73,225 @@ __device__ __forceinline__ bool keep_at(const Mask& m, uint64_t off, uint64_t e)
   return w >= m.threshold;
 }
 
+// keep of the elements 4 q .. 4 q + 3
+struct Keep4 {
+  bool k[4];
+};
+__device__ __forceinline__ Keep4 keep_group(const Mask& m, uint64_t off, uint64_t q) {
+  if (m.mode != 1) {
+    const bool k = m.mode == 0;
+    return {{k, k, k, k}};
+  }
+  const u4 r = philox(m.seed, off, q);
+  return {{r.x >= m.threshold, r.y >= m.threshold, r.z >= m.threshold, r.w >= m.threshold}};
+}
+
+// ------------------------------------------------------------------------------------------ vectors
+template <int BYTES>
+struct RawOf;
+template <>
+struct RawOf<4> {
+  typedef uint32_t type;
+};
+template <>
+struct RawOf<8> {
+  typedef uint32_t type __attribute__((ext_vector_type(2)));
+};
+template <>
+struct RawOf<16> {
+  typedef uint32_t type __attribute__((ext_vector_type(4)));
+};
+
+// VEC elements at p as floats: one load of up to 16 bytes where ALIGNED, else VEC loads
+template <typename T, int VEC, bool ALIGNED, bool NT>
+__device__ __forceinline__ void load_vec(const T* p, float (&v)[VEC]) {
+  if constexpr (ALIGNED) {
+    typedef typename RawOf<VEC * sizeof(T)>::type R;
+    struct A {
+      T t[VEC];
+    };
+    const R r = NT ? __builtin_nontemporal_load((const R*)p) : *(const R*)p;
+    const A a = __builtin_bit_cast(A, r);
+#pragma unroll
+    for (int k = 0; k < VEC; ++k) v[k] = (float)a.t[k];
+  } else {
+#pragma unroll
+    for (int k = 0; k < VEC; ++k) v[k] = (float)p[k];
+  }
+}
+template <typename T, int VEC, bool ALIGNED, bool NT>
+__device__ __forceinline__ void store_vec(T* p, const float (&v)[VEC]) {
+  if constexpr (ALIGNED && VEC * sizeof(T) == 32) {
+    const float lo[4] = {v[0], v[1], v[2], v[3]}, hi[4] = {v[4], v[5], v[6], v[7]};
+    store_vec<T, 4, true, NT>(p, lo);
+    store_vec<T, 4, true, NT>(p + 4, hi);
+  } else if constexpr (ALIGNED) {
+    typedef typename RawOf<VEC * sizeof(T)>::type R;
+    struct A {
+      T t[VEC];
+    };
+    A a;
+#pragma unroll
+    for (int k = 0; k < VEC; ++k) a.t[k] = (T)v[k];
+    const R r = __builtin_bit_cast(R, a);
+    if (NT) __builtin_nontemporal_store(r, (R*)p);
+    else *(R*)p = r;
+  } else {
+#pragma unroll
+    for (int k = 0; k < VEC; ++k) p[k] = (T)v[k];
+  }
+}
+
+// unsigned division by a number fixed for a launch, for dividends below 2^31: n / d = (n * mul) >> shift
+struct Div {
+  uint32_t d, mul;
+  int shift;
+};
+inline Div make_div(int64_t d) {
+  int s = 0;
+  while ((1ll << s) < d) ++s;
+  return {(uint32_t)d, (uint32_t)((1ull << (31 + s)) / (uint64_t)d + 1), 31 + s};
+}
+__device__ __forceinline__ uint32_t div_by(uint32_t n, const Div& d) {
+  return (uint32_t)(((uint64_t)n * d.mul) >> d.shift);
+}
+
+inline bool aligned(const void* p, int64_t bytes) { return ((uintptr_t)p & (uint64_t)(bytes - 1)) == 0; }
+
 // ------------------------------------------------------------------------------------------ dropout
-template <typename T>
-__global__ void dropout_kernel(const T* x, T* y, int64_t n, Mask m, float f, uint64_t* used) {
+// Bound by the bytes of x and y: 16 bytes a lane each way, and one Philox call for every 4 elements hides behind them.
+template <typename T, bool ALIGNED, bool NT>
+__global__ __launch_bounds__(256) void dropout_kernel(const T* x, T* y, int64_t n, Mask m, float f, uint64_t* used) {
+  constexpr int VEC = 16 / sizeof(T);
   const uint64_t off = mask_offset(m);
-  int64_t e = (int64_t)blockIdx.x * blockDim.x + threadIdx.x;
-  if (e == 0 && used) *used = off;
-  for (; e < n; e += (int64_t)gridDim.x * blockDim.x)
-    y[e] = keep_at(m, off, (uint64_t)e) ? (T)((float)x[e] * f) : (T)0.0f;
+  const int64_t first = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  if (first == 0 && used) *used = off;
+  for (int64_t i = first; i * VEC < n; i += (int64_t)gridDim.x * 256) {
+    const int64_t e = i * VEC;
+    float v[VEC];
+    const bool whole = e + VEC <= n;
+    if (whole) {
+      load_vec<T, VEC, ALIGNED, NT>(x + e, v);
+    } else {
+#pragma unroll
+      for (int k = 0; k < VEC; ++k) v[k] = e + k < n ? (float)x[e + k] : 0.0f;
+    }
+#pragma unroll
+    for (int q = 0; q < VEC / 4; ++q) {
+      const Keep4 keep = keep_group(m, off, (uint64_t)(e >> 2) + q);
+#pragma unroll
+      for (int k = 0; k < 4; ++k) v[4 * q + k] = keep.k[k] ? v[4 * q + k] * f : 0.0f;
+    }
+    if (whole) {
+      store_vec<T, VEC, ALIGNED, NT>(y + e, v);
+    } else {
+#pragma unroll
+      for (int k = 0; k < VEC; ++k)
+        if (e + k < n) y[e + k] = (T)v[k];
+    }
+  }
 }
 
 // ------------------------------------------------------------------------------------------ lookup
-template <typename TT, typename OT, typename IT>
-__global__ void embedding_kernel(const TT* table, int64_t stride, const IT* ids, int64_t N, int64_t V, int64_t D,
-                                 OT* out, Mask m, float f, uint64_t* used, int* oob) {
+// A workgroup takes `rows` consecutive ids. Rows of whole vectors: lane t of the tile's rows * D / VEC vectors copies one,
+// kUnroll of them in flight. The ids and hot rows come from L1 / L2, so the output's bytes bound it.
+constexpr int kUnroll = 4;
+
+template <typename TT, typename OT, typename IT, int VEC, bool NT>
+__global__ __launch_bounds__(256) void embedding_rows_of_vectors_kernel(const TT* table, int64_t stride, const IT* ids,
+                                                                        int64_t N, int64_t V, Div dv, int rows, OT* out,
+                                                                        Mask m, float f, uint64_t* used, int* oob) {
   const uint64_t off = mask_offset(m);
-  int64_t e = (int64_t)blockIdx.x * blockDim.x + threadIdx.x;
-  if (e == 0 && used) *used = off;
-  for (; e < N * D; e += (int64_t)gridDim.x * blockDim.x) {
-    const int64_t n = e / D, d = e - n * D;
-    const int64_t id = (int64_t)ids[n];
-    const bool bad = id < 0 || id >= V;
-    if (bad && oob) *oob = 1;
-    out[e] = (!bad && keep_at(m, off, (uint64_t)e)) ? (OT)((float)table[id * stride + d] * f) : (OT)0.0f;
+  if (blockIdx.x == 0 && threadIdx.x == 0 && used) *used = off;
+  for (int64_t n0 = (int64_t)blockIdx.x * rows; n0 < N; n0 += (int64_t)gridDim.x * rows) {
+    const uint32_t total = (uint32_t)(N - n0 < rows ? N - n0 : rows) * dv.d;
+    for (uint32_t t0 = threadIdx.x; t0 < total; t0 += 256 * kUnroll) {
+      float v[kUnroll][VEC];
+      int64_t id[kUnroll];
+      uint32_t col[kUnroll];
+#pragma unroll
+      for (int u = 0; u < kUnroll; ++u) {
+        const uint32_t t = t0 + u * 256;
+        if (t < total) {
+          const uint32_t r = div_by(t, dv);
+          col[u] = t - r * dv.d;
+          id[u] = (int64_t)ids[n0 + r];
+        }
+      }
+#pragma unroll
+      for (int u = 0; u < kUnroll; ++u) {
+        if (t0 + u * 256 < total) {
+          if (id[u] >= 0 && id[u] < V) {
+            load_vec<TT, VEC, true, false>(table + id[u] * stride + (int64_t)col[u] * VEC, v[u]);
+#pragma unroll
+            for (int k = 0; k < VEC; ++k) v[u][k] *= f;
+          } else {
+            if (oob) *oob = 1;
+#pragma unroll
+            for (int k = 0; k < VEC; ++k) v[u][k] = 0.0f;
+          }
+        }
+      }
+#pragma unroll
+      for (int u = 0; u < kUnroll; ++u) {
+        const uint32_t t = t0 + u * 256;
+        if (t < total) {
+          const int64_t i = n0 * dv.d + t;  // the vector's index in the output
+          if (m.mode != 0) {
+#pragma unroll
+            for (int q = 0; q < VEC / 4; ++q) {
+              const Keep4 keep = keep_group(m, off, (uint64_t)i * (VEC / 4) + q);
+#pragma unroll
+              for (int k = 0; k < 4; ++k) v[u][4 * q + k] = keep.k[k] ? v[u][4 * q + k] : 0.0f;
+            }
+          }
+          store_vec<OT, VEC, true, NT>(out + i * VEC, v[u]);
+        }
+      }
+    }
+  }
+}
+
+// Any other row length, stride or alignment: a lane takes 4 consecutive elements of the output, wherever rows begin, so
+// that one Philox call still serves 4 of them and stores stay wide. `rows` is a multiple of 4.
+template <typename TT, typename OT, typename IT, bool ALIGNED>
+__global__ __launch_bounds__(256) void embedding_any_rows_kernel(const TT* table, int64_t stride, const IT* ids,
+                                                                 int64_t N, int64_t V, Div dd, int rows, OT* out, Mask m,
+                                                                 float f, uint64_t* used, int* oob) {
+  const uint64_t off = mask_offset(m);
+  if (blockIdx.x == 0 && threadIdx.x == 0 && used) *used = off;
+  for (int64_t n0 = (int64_t)blockIdx.x * rows; n0 < N; n0 += (int64_t)gridDim.x * rows) {
+    const uint32_t total = (uint32_t)(N - n0 < rows ? N - n0 : rows) * dd.d;
+    for (uint32_t t = threadIdx.x * 4; t < total; t += 256 * 4) {
+      uint32_t r = div_by(t, dd), c = t - r * dd.d;
+      float v[4];
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        v[k] = 0.0f;
+        if (t + k < total) {
+          const int64_t id = (int64_t)ids[n0 + r];
+          if (id >= 0 && id < V) v[k] = (float)table[id * stride + c] * f;
+          else if (oob) *oob = 1;
+        }
+        if (++c == dd.d) {
+          c = 0;
+          ++r;
+        }
+      }
+      const int64_t e = n0 * dd.d + t;
+      if (m.mode != 0) {
+        const Keep4 keep = keep_group(m, off, (uint64_t)e >> 2);
+#pragma unroll
+        for (int k = 0; k < 4; ++k) v[k] = keep.k[k] ? v[k] : 0.0f;
+      }
+      if (t + 4 <= total) {
+        store_vec<OT, 4, ALIGNED, false>(out + e, v);
+      } else {
+#pragma unroll
+        for (int k = 0; k < 4; ++k)
+          if (t + k < total) out[e + k] = (OT)v[k];
+      }
+    }
   }
 }
 
@@ -132,9 +336,33 @@ struct KeyFromPairs {
   __device__ __forceinline__ uint32_t pos(int64_t i) const { return poss[i]; }
 };
 
+// the gradient's zeros, written beside the sort's first launch: rows that no id names keep them
+struct Fill {
+  char* p;
+  int64_t bytes;
+  int wide;  // p is 16-byte aligned
+};
+__device__ __forceinline__ void fill_zeros(const Fill& z, int64_t worker, int64_t workers) {
+  typedef uint32_t v4 __attribute__((ext_vector_type(4)));
+  int64_t done = 0;
+  if (z.wide) {
+    for (int64_t i = worker; i < z.bytes / 16; i += workers) ((v4*)z.p)[i] = v4{0, 0, 0, 0};
+    done = z.bytes / 16 * 16;
+  }
+  for (int64_t i = done / 2 + worker; i < z.bytes / 2; i += workers) ((uint16_t*)z.p)[i] = 0;
+}
+
+__global__ __launch_bounds__(256) void fill_kernel(Fill z) {
+  fill_zeros(z, (int64_t)blockIdx.x * 256 + threadIdx.x, (int64_t)gridDim.x * 256);
+}
+
 template <typename Src>
 __global__ __launch_bounds__(kSortThreads) void sort_count_kernel(Src src, int64_t N, int shift, int width,
-                                                                  uint32_t* counts, int64_t blocks) {
+                                                                  uint32_t* counts, int64_t blocks, Fill z) {
+  if (blockIdx.x >= blocks) {
+    fill_zeros(z, (blockIdx.x - blocks) * kSortThreads + threadIdx.x, (int64_t)(gridDim.x - blocks) * kSortThreads);
+    return;
+  }
   __shared__ uint32_t hist[kBins];
   hist[threadIdx.x] = 0;
   __syncthreads();
@@ -240,9 +468,263 @@ __global__ __launch_bounds__(kSortThreads) void sort_scatter_kernel(Src src, int
   }
 }
 
+// The same sort for N up to 1024 * ITEMS in one workgroup: keys and positions stay in registers and pass through LDS
+// between the digits, while the other workgroups of the launch write the gradient's zeros.
+constexpr int kSmallThreads = 1024, kSmallWaves = kSmallThreads / 64;
+
+template <typename IT, int ITEMS>
+__global__ __launch_bounds__(kSmallThreads) void small_sort_kernel(KeyFromIds<IT> src, int N, int passes, int width,
+                                                                   uint32_t* keys_out, uint32_t* pos_out, Fill z) {
+  if (blockIdx.x > 0) {
+    fill_zeros(z, (int64_t)(blockIdx.x - 1) * kSmallThreads + threadIdx.x, (int64_t)(gridDim.x - 1) * kSmallThreads);
+    return;
+  }
+  constexpr int CAP = kSmallThreads * ITEMS;
+  __shared__ uint32_t skey[CAP];
+  __shared__ uint16_t spos[CAP];
+  __shared__ volatile uint32_t cnt[kSmallWaves][kBins];
+  __shared__ uint32_t scan[kBins];
+  const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63;
+  const uint32_t mask = (1u << width) - 1;
+  const int base = wave * (64 * ITEMS) + lane;
+  uint32_t key[ITEMS], rank[ITEMS];
+  uint16_t pos[ITEMS];
+#pragma unroll
+  for (int j = 0; j < ITEMS; ++j) {
+    const int i = base + j * 64;
+    key[j] = i < N ? src.key(i) : 0u;
+    pos[j] = (uint16_t)i;
+  }
+  for (int pass = 0; pass < passes; ++pass) {
+    const int shift = pass * width;
+    for (int k = tid; k < kSmallWaves * kBins; k += kSmallThreads) (&cnt[0][0])[k] = 0;
+    __syncthreads();
+#pragma unroll
+    for (int j = 0; j < ITEMS; ++j) {
+      const bool valid = base + j * 64 < N;
+      const uint32_t dig = (key[j] >> shift) & mask;
+      const uint64_t peers = wave_match(dig, width, valid);
+      const uint32_t below = __popcll(peers & ((1ull << lane) - 1));
+      const uint32_t before = cnt[wave][dig];
+      rank[j] = before + below;
+      __builtin_amdgcn_wave_barrier();
+      if (valid && below == 0) cnt[wave][dig] = before + __popcll(peers);
+      __builtin_amdgcn_wave_barrier();
+    }
+    __syncthreads();
+    uint32_t total = 0;
+    if (tid < kBins) {
+      for (int w = 0; w < kSmallWaves; ++w) total += cnt[w][tid];
+      scan[tid] = total;
+    }
+    __syncthreads();
+    for (int o = 1; o < kBins; o <<= 1) {
+      uint32_t t = 0;
+      if (tid < kBins && tid >= o) t = scan[tid - o];
+      __syncthreads();
+      if (tid < kBins) scan[tid] += t;
+      __syncthreads();
+    }
+    if (tid < kBins) {
+      uint32_t at = scan[tid] - total;
+      for (int w = 0; w < kSmallWaves; ++w) {
+        const uint32_t c = cnt[w][tid];
+        cnt[w][tid] = at;
+        at += c;
+      }
+    }
+    __syncthreads();
+#pragma unroll
+    for (int j = 0; j < ITEMS; ++j) {
+      if (base + j * 64 < N) {
+        const uint32_t to = cnt[wave][(key[j] >> shift) & mask] + rank[j];
+        skey[to] = key[j];
+        spos[to] = pos[j];
+      }
+    }
+    __syncthreads();
+#pragma unroll
+    for (int j = 0; j < ITEMS; ++j) {
+      if (base + j * 64 < N) {
+        key[j] = skey[base + j * 64];
+        pos[j] = spos[base + j * 64];
+      }
+    }
+  }
+#pragma unroll
+  for (int j = 0; j < ITEMS; ++j) {
+    if (base + j * 64 < N) {
+      keys_out[base + j * 64] = key[j];
+      pos_out[base + j * 64] = pos[j];
+    }
+  }
+}
+
 // ------------------------------------------------------------------------------------------ gradient
-__device__ __forceinline__ int64_t lower_bound(const uint32_t* keys, int64_t N, uint32_t v) {
-  int64_t lo = 0, hi = N;
+// A run is the sorted positions of one row. The positions are cut into equal pieces whatever the runs' lengths are, so
+// that a row named by most ids costs no more than many rows named once: a group of lanes (one vector of columns a lane)
+// adds a piece, writes the rows whose runs lie inside it, and leaves the sums of the runs that its ends cut. The workgroup
+// joins those of its groups in LDS, run_join_kernel those that cross workgroups. Pieces depend on N alone, so the order of
+// every sum does.
+struct RunPlan {
+  int vec;         // elements a lane
+  int lg;          // log2 of the lanes a group
+  int64_t chunks;  // column chunks of (1 << lg) * vec
+  int piece;       // positions a group, a multiple of 4
+  int64_t span, blocks;  // positions a workgroup, workgroups
+};
+
+inline RunPlan run_plan(int64_t N, int64_t D, int vec) {
+  RunPlan r;
+  r.vec = vec;
+  const int64_t dv = (D + vec - 1) / vec;
+  r.lg = 0;
+  while (r.lg < 6 && (1ll << r.lg) < dv) ++r.lg;
+  r.chunks = (dv + (1 << r.lg) - 1) >> r.lg;
+  const int64_t groups = 256 >> r.lg;
+  // enough workgroups for the chip, else longer pieces: fewer runs are cut
+  const int64_t want = 2048 / r.chunks > 0 ? 2048 / r.chunks : 1;
+  int64_t t = (N + groups * want - 1) / (groups * want);
+  t = t < 8 ? 8 : t > 64 ? 64 : t;
+  while ((N + groups * t - 1) / (groups * t) * r.chunks > (1 << 22)) t *= 2;
+  r.piece = (int)((t + 3) / 4 * 4);
+  r.span = groups * r.piece;
+  r.blocks = (N + r.span - 1) / r.span;
+  return r;
+}
+
+template <typename GT, int VEC>
+__device__ __forceinline__ void masked_term(const GT* g, int64_t D, uint32_t pos, int64_t d, const Mask& m, uint64_t off,
+                                            float (&v)[VEC]) {
+  const int64_t e = (int64_t)pos * D + d;
+  load_vec<GT, VEC, (VEC > 1), false>(g + e, v);
+  if (m.mode == 0) return;
+  if constexpr (VEC == 1) {
+    if (!keep_at(m, off, (uint64_t)e)) v[0] = 0.0f;
+  } else {
+#pragma unroll
+    for (int q = 0; q < VEC / 4; ++q) {
+      const Keep4 keep = keep_group(m, off, (uint64_t)(e >> 2) + q);
+#pragma unroll
+      for (int k = 0; k < 4; ++k) v[4 * q + k] = keep.k[k] ? v[4 * q + k] : 0.0f;
+    }
+  }
+}
+
+template <typename TT, int VEC, bool ALIGNED>
+__device__ __forceinline__ void write_row(TT* grad, int64_t D, uint32_t row, int64_t d, float f, const float (&acc)[VEC]) {
+  float v[VEC];
+#pragma unroll
+  for (int k = 0; k < VEC; ++k) v[k] = acc[k] * f;
+  store_vec<TT, VEC, ALIGNED, false>(grad + (int64_t)row * D + d, v);
+}
+
+enum { kHead = 1, kThrough = 2, kTail = 4 };
+
+template <typename GT, typename TT, int VEC, bool ALIGNED>
+__global__ __launch_bounds__(256) void run_sum_kernel(const GT* g, const uint32_t* keys, const uint32_t* pos, int64_t N,
+                                                      uint32_t V, int64_t D, RunPlan r, Mask m, float f, TT* grad,
+                                                      float* heads, float* tails) {
+  __shared__ float head[256 * VEC], tail[256 * VEC];
+  __shared__ uint8_t flags[256];
+  const uint64_t off = mask_offset(m);
+  const int groups = 256 >> r.lg, group = threadIdx.x >> r.lg, sub = threadIdx.x & ((1 << r.lg) - 1);
+  const int64_t block = blockIdx.x % (uint32_t)r.blocks, chunk = blockIdx.x / (uint32_t)r.blocks;
+  const int64_t d = ((chunk << r.lg) + sub) * VEC;
+  const bool col = d < D;
+  const int64_t base = block * r.span;
+  const int64_t a = base + (int64_t)group * r.piece;
+  const int64_t b = a + r.piece < N ? a + r.piece : N;
+  float acc[VEC];
+#pragma unroll
+  for (int k = 0; k < VEC; ++k) acc[k] = 0.0f;
+  int flag = 0;
+  uint32_t cur = V;
+  if (a < N) {
+    cur = keys[a];
+    bool cut = a > 0 && keys[a - 1] == cur;  // the run began in an earlier piece
+    for (int64_t i = a; i < b; i += 4) {
+      uint32_t kk[4], pp[4];
+#pragma unroll
+      for (int u = 0; u < 4; ++u) {
+        kk[u] = i + u < b ? keys[i + u] : V;
+        pp[u] = i + u < b ? pos[i + u] : 0u;
+      }
+      float v[4][VEC];
+#pragma unroll
+      for (int u = 0; u < 4; ++u) {
+        if (kk[u] != V && col) {
+          masked_term<GT, VEC>(g, D, pp[u], d, m, off, v[u]);
+        } else {
+#pragma unroll
+          for (int k = 0; k < VEC; ++k) v[u][k] = 0.0f;
+        }
+      }
+#pragma unroll
+      for (int u = 0; u < 4; ++u) {
+        if (i + u < b) {
+          if (kk[u] != cur) {
+            if (cut) {
+#pragma unroll
+              for (int k = 0; k < VEC; ++k) head[threadIdx.x * VEC + k] = acc[k];
+              flag |= kHead;
+            } else if (col) {
+              write_row<TT, VEC, ALIGNED>(grad, D, cur, d, f, acc);
+            }
+            cut = false;
+            cur = kk[u];
+#pragma unroll
+            for (int k = 0; k < VEC; ++k) acc[k] = 0.0f;
+          }
+#pragma unroll
+          for (int k = 0; k < VEC; ++k) acc[k] += v[u][k];
+        }
+      }
+    }
+    const bool goes_on = b < N && keys[b] == cur;
+    if (cur != V) {
+      if (cut) {
+#pragma unroll
+        for (int k = 0; k < VEC; ++k) head[threadIdx.x * VEC + k] = acc[k];
+        flag |= goes_on ? kHead | kThrough : kHead;
+      } else if (goes_on) {
+#pragma unroll
+        for (int k = 0; k < VEC; ++k) tail[threadIdx.x * VEC + k] = acc[k];
+        flag |= kTail;
+      } else if (col) {
+        write_row<TT, VEC, ALIGNED>(grad, D, cur, d, f, acc);
+      }
+    }
+  }
+  if (sub == 0) flags[group] = (uint8_t)flag;
+  __syncthreads();
+  const bool from_before = group == 0 && (flag & kHead);
+  if (!from_before && !(flag & kTail)) return;
+  // two runs may leave a group 0: the one that came in (its sum goes to `heads`) and the one it starts
+  for (int which = from_before ? 0 : 1; which < 2; ++which) {
+    if (which == 1 && !(flag & kTail)) break;
+    float s[VEC];
+#pragma unroll
+    for (int k = 0; k < VEC; ++k) s[k] = (which ? tail : head)[threadIdx.x * VEC + k];
+    bool open = which == 1 || (flag & kThrough);
+    for (int h = group + 1; h < groups && open; ++h) {
+#pragma unroll
+      for (int k = 0; k < VEC; ++k) s[k] += head[(threadIdx.x + ((h - group) << r.lg)) * VEC + k];
+      open = flags[h] & kThrough;
+    }
+    if (!col) continue;
+    if (which == 0 || open) {
+      float* to = (which ? tails : heads) + block * D + d;
+#pragma unroll
+      for (int k = 0; k < VEC; ++k) to[k] = s[k];
+    } else {
+      write_row<TT, VEC, ALIGNED>(grad, D, cur, d, f, s);
+    }
+  }
+}
+
+// first position of [lo, hi) whose key is not below v
+__device__ __forceinline__ int64_t lower_bound(const uint32_t* keys, int64_t lo, int64_t hi, uint32_t v) {
   while (lo < hi) {
     const int64_t mid = (lo + hi) >> 1;
     if (keys[mid] < v) lo = mid + 1;
@@ -251,32 +733,55 @@ __device__ __forceinline__ int64_t lower_bound(const uint32_t* keys, int64_t N, 
   return lo;
 }
 
-// one wave a row of the table: its terms in the order of their positions
-template <typename GT, typename TT>
-__global__ __launch_bounds__(256) void embedding_rows_kernel(const GT* g, const uint32_t* keys, const uint32_t* pos,
-                                                             int64_t N, int64_t V, int64_t D, Mask m, float f,
-                                                             TT* grad) {
-  const int lane = threadIdx.x & 63;
-  const uint64_t off = mask_offset(m);
-  for (int64_t v = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6); v < V; v += (int64_t)gridDim.x * 4) {
-    const int64_t a = lower_bound(keys, N, (uint32_t)v), b = lower_bound(keys, N, (uint32_t)v + 1);
-    for (int64_t d = lane; d < D; d += 64) {
-      float s = 0.0f;
-      for (int64_t i = a; i < b; ++i) {
-        const int64_t e = (int64_t)pos[i] * D + d;
-        if (keep_at(m, off, (uint64_t)e)) s += (float)g[e];
-      }
-      grad[v * D + d] = (TT)(s * f);
+// the run that workgroup b of run_sum_kernel started and did not end: its tail and the heads of the workgroups after it
+template <typename TT, int VEC, bool ALIGNED>
+__global__ __launch_bounds__(256) void run_join_kernel(const uint32_t* keys, int64_t N, uint32_t V, int64_t D, RunPlan r,
+                                                       float f, TT* grad, const float* heads, const float* tails) {
+  const int64_t b = blockIdx.x % (uint32_t)r.blocks, next = (b + 1) * r.span;
+  if (next >= N) return;
+  const uint32_t key = keys[next - 1];
+  if (key == V || keys[next] != key) return;
+  if (b > 0 && keys[b * r.span] == key && keys[b * r.span - 1] == key) return;  // it began earlier
+  int64_t end = (b + 2) * r.span < N ? (b + 2) * r.span : N;
+  if (keys[end - 1] == key) end = lower_bound(keys, end, N, key + 1);
+  else end = next + 1;  // ends inside the next workgroup
+  const int64_t last = (end - 1) / r.span;
+  __shared__ float part[256 * VEC];
+  const int groups = 256 >> r.lg, group = threadIdx.x >> r.lg, sub = threadIdx.x & ((1 << r.lg) - 1);
+  const int64_t d = (((int64_t)(blockIdx.x / (uint32_t)r.blocks) << r.lg) + sub) * VEC;
+  const bool col = d < D;
+  float s[VEC];
+#pragma unroll
+  for (int k = 0; k < VEC; ++k) s[k] = 0.0f;
+  if (col) {
+#pragma unroll 4
+    for (int64_t h = b + 1 + group; h <= last; h += groups) {
+#pragma unroll
+      for (int k = 0; k < VEC; ++k) s[k] += heads[h * D + d + k];
     }
   }
+#pragma unroll
+  for (int k = 0; k < VEC; ++k) part[threadIdx.x * VEC + k] = s[k];
+  __syncthreads();
+  if (group != 0 || !col) return;
+#pragma unroll
+  for (int k = 0; k < VEC; ++k) s[k] = tails[b * D + d + k];
+  const int64_t used = last - b < groups ? last - b : groups;
+  for (int q = 0; q < used; ++q) {
+#pragma unroll
+    for (int k = 0; k < VEC; ++k) s[k] += part[(threadIdx.x + (q << r.lg)) * VEC + k];
+  }
+  write_row<TT, VEC, ALIGNED>(grad, D, key, d, f, s);
 }
 
 // ------------------------------------------------------------------------------------------ workspace
+constexpr int64_t kSmallSort = 16 * kSmallThreads;
+
 struct GradWs {
-  int64_t counts, totals, keys[2], pos[2], bytes;
+  int64_t counts, totals, keys[2], pos[2], heads, tails, bytes;
 };
 
-inline GradWs grad_ws(int64_t N, int64_t V) {
+inline GradWs grad_ws(int64_t N, int64_t V, int64_t D) {
   const SortPlan s = sort_plan(N, V);
   GradWs w;
   int64_t at = 0;
@@ -285,37 +790,80 @@ inline GradWs grad_ws(int64_t N, int64_t V) {
     at += (bytes + 255) / 256 * 256;
     return r;
   };
-  w.counts = take(kBins * s.blocks * 4);
-  w.totals = take(kBins * 4);
+  const bool small = N <= kSmallSort;
+  w.counts = take(small ? 0 : kBins * s.blocks * 4);
+  w.totals = take(small ? 0 : kBins * 4);
   for (int i = 0; i < 2; ++i) {
-    w.keys[i] = take(N * 4);
-    w.pos[i] = take(N * 4);
+    w.keys[i] = take(small && i ? 0 : N * 4);
+    w.pos[i] = take(small && i ? 0 : N * 4);
   }
+  int64_t blocks = 0;  // of whichever vector the pointers' alignment allows
+  for (int vec : {1, 4, 8}) {
+    const int64_t b = run_plan(N, D, vec).blocks;
+    blocks = b > blocks ? b : blocks;
+  }
+  w.heads = take(blocks * D * 4);
+  w.tails = take(blocks * D * 4);
   w.bytes = at;
   return w;
 }
 
 template <typename Src>
-inline void sort_pass(Src src, int64_t N, int pass, const SortPlan& s, char* ws, const GradWs& w, hipStream_t st) {
+inline void sort_pass(Src src, int64_t N, int pass, const SortPlan& s, char* ws, const GradWs& w, const Fill& z,
+                      hipStream_t st) {
   uint32_t* counts = (uint32_t*)(ws + w.counts);
   uint32_t* totals = (uint32_t*)(ws + w.totals);
   const int shift = pass * s.width;
-  hipLaunchKernelGGL(sort_count_kernel<Src>, dim3((unsigned)s.blocks), dim3(kSortThreads), 0, st, src, N, shift,
-                     s.width, counts, s.blocks);
+  int64_t fill = z.bytes / (kSortThreads * 16 * 4);
+  fill = z.bytes == 0 ? 0 : fill < 1 ? 1 : fill > 2048 ? 2048 : fill;
+  hipLaunchKernelGGL(sort_count_kernel<Src>, dim3((unsigned)(s.blocks + fill)), dim3(kSortThreads), 0, st, src, N, shift,
+                     s.width, counts, s.blocks, z);
   hipLaunchKernelGGL(sort_scan_kernel, dim3(1u << s.width), dim3(256), 0, st, counts, s.blocks, totals);
   hipLaunchKernelGGL(sort_scatter_kernel<Src>, dim3((unsigned)s.blocks), dim3(kSortThreads), 0, st, src, N, shift,
                      s.width, counts, s.blocks, totals, (uint32_t*)(ws + w.keys[pass & 1]),
                      (uint32_t*)(ws + w.pos[pass & 1]));
 }
 
+// sorts the ids and clears the gradient; which of the two buffers holds the pairs
+template <typename IT>
+inline int sort_ids(const IT* ids, int64_t N, int64_t V, int64_t pad, char* ws, const GradWs& w, const Fill& z,
+                    hipStream_t st) {
+  const SortPlan s = sort_plan(N, V);
+  const KeyFromIds<IT> src{ids, V, pad};
+  if (N <= kSmallSort) {
+    int64_t fill = z.bytes / (kSmallThreads * 16 * 2);
+    fill = fill < 1 ? 1 : fill > 1024 ? 1024 : fill;
+    auto* k = N <= 4 * kSmallThreads ? small_sort_kernel<IT, 4> : small_sort_kernel<IT, 16>;
+    hipLaunchKernelGGL(k, dim3((unsigned)(1 + fill)), dim3(kSmallThreads), 0, st, src, (int)N, s.passes, s.width,
+                       (uint32_t*)(ws + w.keys[0]), (uint32_t*)(ws + w.pos[0]), z);
+    return 0;
+  }
+  for (int pass = 0; pass < s.passes; ++pass) {
+    const int from = (pass - 1) & 1;
+    if (pass == 0) sort_pass(src, N, pass, s, ws, w, z, st);
+    else sort_pass(KeyFromPairs{(const uint32_t*)(ws + w.keys[from]), (const uint32_t*)(ws + w.pos[from])}, N, pass, s, ws,
+                   w, Fill{nullptr, 0, 0}, st);
+  }
+  return (s.passes - 1) & 1;
+}
+
 // sizes that the kernels' 32-bit positions and keys, and the grids, hold
 inline int embedding_sizes_ok(const char* what, int64_t N, int64_t V, int64_t D) {
   YN_CHECK(N >= 0 && V >= 0 && D >= 0, "%s: negative size", what);
   YN_CHECK(N < (1ll << 31) && V < (1ll << 31), "%s: N=%lld or V=%lld is 2^31 or more", what, (long long)N, (long long)V);
-  YN_CHECK(D <= (1ll << 31) && (D == 0 || (N <= (1ll << 38) / D && V <= (1ll << 38) / D)),
-           "%s: more than 2^38 elements", what);
+  YN_CHECK(D <= (1ll << 24), "%s: D=%lld is more than 2^24", what, (long long)D);
+  YN_CHECK(D == 0 || (N <= (1ll << 38) / D && V <= (1ll << 38) / D), "%s: more than 2^38 elements", what);
   return 0;
 }
+// rows a workgroup takes, so that it has about `work` units of `per_row` each (fewer where N of them leave CUs idle)
+inline int tile_rows(int64_t N, int64_t per_row, int64_t work, int64_t multiple) {
+  const int64_t spread = (N * per_row + 1023) / 1024;  // 4 workgroups a CU
+  const int64_t w = spread < work ? (spread > 256 ? spread : 256) : work;
+  const int64_t r = (w / per_row + multiple - 1) / multiple * multiple;
+  return (int)(r < multiple ? multiple : r);
+}
+// outputs that leave no cache lines worth keeping (the Infinity Cache holds 256 MB) are stored non-temporally
+inline bool streams_past_cache(int64_t bytes) { return bytes >= (64ll << 20); }
 inline int mask_args_ok(const char* what, double p) {
   YN_CHECK(p >= 0.0 && p <= 1.0, "%s: p=%g is not a probability", what, p);
   return 0;
@@ -336,10 +884,13 @@ int yanerf_dropout(const void* x, int type, int64_t n, double p, uint64_t seed, 
   YN_CHECK(x && y, "dropout: null pointer");
   const Mask m = make_mask(p, seed, offset, rng_base);
   const float f = (float)mask_scale(p, m);
+  const bool al = aligned(x, 16) && aligned(y, 16), nt = streams_past_cache(n * type_bytes(type));
   with_type(type, [&](auto t) {
     using T = decltype(t);
-    hipLaunchKernelGGL(dropout_kernel<T>, grid_for((n + 255) / 256), dim3(256), 0, as_stream(stream),
-                       (const T*)x, (T*)y, n, m, f, rng_used);
+    constexpr int VEC = 16 / sizeof(T);
+    const dim3 grid = grid_for((n + 256 * VEC - 1) / (256 * VEC));
+    auto* k = !al ? dropout_kernel<T, false, false> : nt ? dropout_kernel<T, true, true> : dropout_kernel<T, true, false>;
+    hipLaunchKernelGGL(k, grid, dim3(256), 0, as_stream(stream), (const T*)x, (T*)y, n, m, f, rng_used);
   });
   YN_LAUNCH_CHECK("dropout");
   return 0;
@@ -359,17 +910,36 @@ int yanerf_embedding_forward(const void* table, int table_type, int64_t table_st
   YN_CHECK(table_stride >= 0, "embedding: negative table stride");
   const Mask m = make_mask(p, seed, offset, rng_base);
   const float f = (float)(scale * mask_scale(p, m));
+  const int64_t wide = 16 / (type_bytes(table_type) > type_bytes(out_type) ? type_bytes(table_type) : type_bytes(out_type));
+  auto fits = [&](int64_t vec) {
+    return D % vec == 0 && table_stride % vec == 0 && aligned(table, vec * type_bytes(table_type)) &&
+           aligned(out, vec * type_bytes(out_type));
+  };
+  const int64_t vec = fits(wide) ? wide : fits(4) ? 4 : 0;
+  const bool nt = streams_past_cache(N * D * type_bytes(out_type));
   with_type(table_type, [&](auto tt) {
     with_type(out_type, [&](auto ot) {
       using TT = decltype(tt);
       using OT = decltype(ot);
-      const dim3 grid = grid_for((N * D + 255) / 256);
-      if (id_bytes == 8)
-        hipLaunchKernelGGL((embedding_kernel<TT, OT, int64_t>), grid, dim3(256), 0, as_stream(stream),
-                           (const TT*)table, table_stride, (const int64_t*)ids, N, V, D, (OT*)out, m, f, rng_used, oob);
-      else
-        hipLaunchKernelGGL((embedding_kernel<TT, OT, int32_t>), grid, dim3(256), 0, as_stream(stream),
-                           (const TT*)table, table_stride, (const int32_t*)ids, N, V, D, (OT*)out, m, f, rng_used, oob);
+      with_index(id_bytes, [&](auto it) {
+        using IT = decltype(it);
+        if (vec) {
+          constexpr int W = 16 / (sizeof(TT) > sizeof(OT) ? sizeof(TT) : sizeof(OT));
+          const int rows = tile_rows(N, D / vec, 256 * kUnroll, 1);
+          auto* k = vec == 4 ? (nt ? embedding_rows_of_vectors_kernel<TT, OT, IT, 4, true>
+                                   : embedding_rows_of_vectors_kernel<TT, OT, IT, 4, false>)
+                             : (nt ? embedding_rows_of_vectors_kernel<TT, OT, IT, W, true>
+                                   : embedding_rows_of_vectors_kernel<TT, OT, IT, W, false>);
+          hipLaunchKernelGGL(k, grid_for((N + rows - 1) / rows), dim3(256), 0, as_stream(stream), (const TT*)table,
+                             table_stride, (const IT*)ids, N, V, make_div(D / vec), rows, (OT*)out, m, f, rng_used, oob);
+        } else {
+          const int rows = tile_rows(N, D, 256 * 4 * kUnroll, 4);
+          auto* k = aligned(out, 4 * sizeof(OT)) ? embedding_any_rows_kernel<TT, OT, IT, true>
+                                                 : embedding_any_rows_kernel<TT, OT, IT, false>;
+          hipLaunchKernelGGL(k, grid_for((N + rows - 1) / rows), dim3(256), 0, as_stream(stream), (const TT*)table,
+                             table_stride, (const IT*)ids, N, V, make_div(D), rows, (OT*)out, m, f, rng_used, oob);
+        }
+      });
     });
   });
   YN_LAUNCH_CHECK("embedding");
@@ -378,7 +948,7 @@ int yanerf_embedding_forward(const void* table, int table_type, int64_t table_st
 
 int64_t yanerf_embedding_bwd_workspace_bytes(int64_t N, int64_t V, int64_t D) {
   if (embedding_sizes_ok("embedding_bwd_workspace", N, V, D)) return -1;
-  return N == 0 || V == 0 || D == 0 ? 0 : grad_ws(N, V).bytes;
+  return N == 0 || V == 0 || D == 0 ? 0 : grad_ws(N, V, D).bytes;
 }
 
 int yanerf_embedding_backward(const void* g, int g_type, const void* ids, int id_bytes, int64_t N, int64_t V,
@@ -399,26 +969,41 @@ int yanerf_embedding_backward(const void* g, int g_type, const void* ids, int id
   const float f = (float)(scale * mask_scale(p, m));
   hipStream_t st = as_stream(stream);
   char* ws = (char*)workspace;
-  const GradWs w = grad_ws(N, V);
-  const SortPlan s = sort_plan(N, V);
-  if (N > 0)
-    for (int pass = 0; pass < s.passes; ++pass) {
-      if (pass > 0)
-        sort_pass(KeyFromPairs{(const uint32_t*)(ws + w.keys[(pass - 1) & 1]),
-                               (const uint32_t*)(ws + w.pos[(pass - 1) & 1])}, N, pass, s, ws, w, st);
-      else if (id_bytes == 8)
-        sort_pass(KeyFromIds<int64_t>{(const int64_t*)ids, V, padding_idx}, N, pass, s, ws, w, st);
-      else
-        sort_pass(KeyFromIds<int32_t>{(const int32_t*)ids, V, padding_idx}, N, pass, s, ws, w, st);
-    }
-  const int last = (s.passes - 1) & 1;
+  const Fill z{(char*)grad_table, V * D * type_bytes(table_type), aligned(grad_table, 16)};
+  if (N == 0) {
+    hipLaunchKernelGGL(fill_kernel, grid_for((z.bytes + 4095) / 4096), dim3(256), 0, st, z);
+    YN_LAUNCH_CHECK("embedding_backward");
+    return 0;
+  }
+  const GradWs w = grad_ws(N, V, D);
+  int at = 0;
+  with_index(id_bytes, [&](auto it) { at = sort_ids((const decltype(it)*)ids, N, V, padding_idx, ws, w, z, st); });
+  const uint32_t* keys = (const uint32_t*)(ws + w.keys[at]);
+  const uint32_t* pos = (const uint32_t*)(ws + w.pos[at]);
+  float *heads = (float*)(ws + w.heads), *tails = (float*)(ws + w.tails);
+  const int gb = (int)type_bytes(g_type);
+  const int vec = D % (16 / gb) == 0 && aligned(g, 16) ? 16 / gb : D % 4 == 0 && aligned(g, 4 * gb) ? 4 : 1;
+  const bool al = vec > 1 && aligned(grad_table, vec * type_bytes(table_type) < 16 ? vec * type_bytes(table_type) : 16);
+  const RunPlan r = run_plan(N, D, vec);
+  const dim3 grid((unsigned)(r.blocks * r.chunks));
   with_type(g_type, [&](auto gt) {
     with_type(table_type, [&](auto tt) {
       using GT = decltype(gt);
       using TT = decltype(tt);
-      hipLaunchKernelGGL((embedding_rows_kernel<GT, TT>), grid_for((V + 3) / 4), dim3(256), 0, st,
-                         (const GT*)g, (const uint32_t*)(ws + w.keys[last]), (const uint32_t*)(ws + w.pos[last]), N, V,
-                         D, m, f, (TT*)grad_table);
+      auto go = [&](auto vc, auto ac) {
+        constexpr int VEC = decltype(vc)::value;
+        constexpr bool AL = decltype(ac)::value;
+        hipLaunchKernelGGL((run_sum_kernel<GT, TT, VEC, AL>), grid, dim3(256), 0, st, (const GT*)g, keys, pos, N,
+                           (uint32_t)V, D, r, m, f, (TT*)grad_table, heads, tails);
+        if (r.blocks > 1)
+          hipLaunchKernelGGL((run_join_kernel<TT, VEC, AL>), grid, dim3(256), 0, st, keys, N, (uint32_t)V, D, r, f,
+                             (TT*)grad_table, heads, tails);
+      };
+      using std::integral_constant;
+      if (vec == 1) go(integral_constant<int, 1>{}, std::false_type{});
+      else if (vec == 4) al ? go(integral_constant<int, 4>{}, std::true_type{}) : go(integral_constant<int, 4>{}, std::false_type{});
+      else if constexpr (sizeof(GT) == 2)
+        al ? go(integral_constant<int, 8>{}, std::true_type{}) : go(integral_constant<int, 8>{}, std::false_type{});
     });
   });
   YN_LAUNCH_CHECK("embedding_backward");

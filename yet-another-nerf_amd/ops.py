@@ -496,9 +496,16 @@ def _probability(what: str, p) -> float:
     return p
 
 
-def _on(dev: torch.device):
-    """The launch context of `dev`: kernels of a tensor on another device than the current one run on that device."""
-    return nullcontext() if dev.index == torch.cuda.current_device() else torch.cuda.device(dev)
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)  # of a device, without a Stream object (3-14 us)
+
+
+def _launch(dev: int, entry, *args) -> None:
+    """entry(*args, stream) on device `dev` and its current stream, whichever device is current."""
+    here = torch.cuda.current_device()
+    with nullcontext() if dev == here else torch.cuda.device(dev):
+        stream = _raw_stream(dev) if _raw_stream is not None else torch.cuda.current_stream(dev).cuda_stream
+        if entry(*args, stream):
+            _C.check(1, entry.__name__)
 
 
 def _mask_rng(what: str, p: float, rng, rng_base: Optional[torch.Tensor], dev: torch.device, n: int):
@@ -515,31 +522,26 @@ def _mask_rng(what: str, p: float, rng, rng_base: Optional[torch.Tensor], dev: t
     return int(seed) & _U64, int(off) & _U64
 
 
-class _MaskState:
-    """What a backward needs to draw a forward's mask again: (seed, offset) by value, or, with an rng_base (whose value
-    may have moved on by then), the offset that the forward's kernel used, kept on the device."""
-
-    def __init__(self, p: float, seed: int, offset: int, rng_base: Optional[torch.Tensor], keep: bool):
-        self.p, self.seed, self.offset = p, seed, offset
-        self.base = rng_base if p > 0.0 else None
-        self.used = torch.empty(1, dtype=torch.int64, device=rng_base.device) if keep and self.base is not None else None
-
-    def forward_args(self):
-        return self.p, self.seed, self.offset, _p(self.base), _p(self.used)
-
-    def backward_args(self):
-        return (self.p, self.seed, self.offset, None) if self.used is None else (self.p, self.seed, 0, _p(self.used))
+def _mask_args(ctx, p: float, seed: int, offset: int, rng_base: Optional[torch.Tensor], keep: bool):
+    """The mask arguments of a forward's entry point; ctx.mask gets its backward's. With an rng_base, whose value may have
+    moved on by then, the backward adds the offset that the forward's kernel left in `used`."""
+    if rng_base is None or p == 0.0:
+        ctx.mask = (p, seed, offset, None)
+        return p, seed, offset, None, None
+    if not keep:
+        return p, seed, offset, rng_base.data_ptr(), None
+    ctx.used = torch.empty(1, dtype=torch.int64, device=rng_base.device)
+    ctx.mask = (p, seed, 0, ctx.used.data_ptr())
+    return p, seed, offset, rng_base.data_ptr(), ctx.used.data_ptr()
 
 
 class _DropoutFn(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, p, seed, offset, rng_base):
-        ctx.mask = _MaskState(p, seed, offset, rng_base, ctx.needs_input_grad[0])
         x = x.contiguous()
         y = torch.empty_like(x)
-        with _on(x.device):
-            _C.check(_C.lib().yanerf_dropout(_p(x), _TYPES[x.dtype], x.numel(), *ctx.mask.forward_args(), _p(y),
-                                             _stream()), "yanerf_dropout")
+        _launch(x.get_device(), _C.lib().yanerf_dropout, x.data_ptr(), _TYPES[x.dtype], x.numel(),
+                *_mask_args(ctx, p, seed, offset, rng_base, ctx.needs_input_grad[0]), y.data_ptr())
         return y
 
     @staticmethod
@@ -547,9 +549,8 @@ class _DropoutFn(torch.autograd.Function):
     def backward(ctx, g):
         g = g.contiguous()
         out = torch.empty_like(g)
-        with _on(g.device):
-            _C.check(_C.lib().yanerf_dropout(_p(g), _TYPES[g.dtype], g.numel(), *ctx.mask.backward_args(), None, _p(out),
-                                             _stream()), "yanerf_dropout")
+        _launch(g.get_device(), _C.lib().yanerf_dropout, g.data_ptr(), _TYPES[g.dtype], g.numel(), *ctx.mask, None,
+                out.data_ptr())
         return out, None, None, None, None
 
 
@@ -595,18 +596,18 @@ class _EmbeddingFn(torch.autograd.Function):
     @staticmethod
     def forward(ctx, table, ids, scale, padding_idx, p, seed, offset, rng_base, out_dtype):
         V, D = table.shape
-        ctx.mask = _MaskState(p, seed, offset, rng_base, ctx.needs_input_grad[0])
-        ctx.dims = (V, D, table.dtype, scale, padding_idx)
         if D > 1 and table.stride(1) != 1:
             table = table.contiguous()
         ids = ids.contiguous()
         out = torch.empty(*ids.shape, D, dtype=out_dtype, device=table.device)
-        with _on(table.device):
-            _C.check(_C.lib().yanerf_embedding_forward(
-                _p(table), _TYPES[table.dtype], table.stride(0), _p(ids), ids.element_size(), ids.numel(), V, D, scale,
-                *ctx.mask.forward_args(), _p(out), _TYPES[out_dtype], _p(_id_flag(table.device)), _stream()),
-                "yanerf_embedding_forward")
-        if ctx.needs_input_grad[0]:
+        keep = ctx.needs_input_grad[0]
+        flag = _id_flag(table.device)
+        _launch(table.get_device(), _C.lib().yanerf_embedding_forward, table.data_ptr(), _TYPES[table.dtype],
+                table.stride(0), ids.data_ptr(), ids.element_size(), ids.numel(), V, D, scale,
+                *_mask_args(ctx, p, seed, offset, rng_base, keep), out.data_ptr(), _TYPES[out_dtype],
+                None if flag is None else flag.data_ptr())
+        if keep:
+            ctx.dims = (V, D, table.dtype, scale, padding_idx)
             ctx.save_for_backward(ids)
         return out
 
@@ -618,12 +619,10 @@ class _EmbeddingFn(torch.autograd.Function):
         N = ids.numel()
         g = g.contiguous()
         grad = torch.empty(V, D, dtype=dtype, device=g.device)
-        with _on(g.device):
-            nb = _C.lib().yanerf_embedding_bwd_workspace_bytes(N, V, D)
-            ws = torch.empty(max(nb, 1), dtype=torch.uint8, device=g.device)
-            _C.check(_C.lib().yanerf_embedding_backward(
-                _p(g), _TYPES[g.dtype], _p(ids), ids.element_size(), N, V, D, pad, scale, *ctx.mask.backward_args(),
-                _p(grad), _TYPES[dtype], _p(ws), _stream()), "yanerf_embedding_backward")
+        L = _C.lib()
+        ws = torch.empty(L.yanerf_embedding_bwd_workspace_bytes(N, V, D), dtype=torch.uint8, device=g.device)
+        _launch(g.get_device(), L.yanerf_embedding_backward, g.data_ptr(), _TYPES[g.dtype], ids.data_ptr(),
+                ids.element_size(), N, V, D, pad, scale, *ctx.mask, grad.data_ptr(), _TYPES[dtype], ws.data_ptr())
         return grad, None, None, None, None, None, None, None, None
 
 
