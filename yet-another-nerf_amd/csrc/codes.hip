@@ -90,6 +90,10 @@ __device__ __forceinline__ Keep4 keep_group(const Mask& m, uint64_t off, uint64_
 template <int BYTES>
 struct RawOf;
 template <>
+struct RawOf<2> {
+  typedef uint16_t type;
+};
+template <>
 struct RawOf<4> {
   typedef uint32_t type;
 };
@@ -159,36 +163,36 @@ __device__ __forceinline__ uint32_t div_by(uint32_t n, const Div& d) {
 inline bool aligned(const void* p, int64_t bytes) { return ((uintptr_t)p & (uint64_t)(bytes - 1)) == 0; }
 
 // ------------------------------------------------------------------------------------------ dropout
-// Bound by the bytes of x and y: 16 bytes a lane each way, and one Philox call for every 4 elements hides behind them.
+// Bound by the bytes of x and y: 16 bytes a lane each way, loaded before anything else is looked at, and one Philox call
+// for every 4 elements hides behind them. A lane takes one vector: loops over more of them measured 10 % slower.
 template <typename T, bool ALIGNED, bool NT>
-__global__ __launch_bounds__(256) void dropout_kernel(const T* x, T* y, int64_t n, Mask m, float f, uint64_t* used) {
+__global__ __launch_bounds__(256) void dropout_kernel(const T* x, T* y, int64_t n, int64_t first, Mask m, float f,
+                                                      uint64_t* used) {
   constexpr int VEC = 16 / sizeof(T);
+  const int64_t e = first + ((int64_t)blockIdx.x * 256 + threadIdx.x) * VEC;
+  if (e >= n) return;
+  float v[VEC];
+  const bool whole = e + VEC <= n;
+  if (whole) {
+    load_vec<T, VEC, ALIGNED, NT>(x + e, v);
+  } else {
+#pragma unroll
+    for (int k = 0; k < VEC; ++k) v[k] = e + k < n ? (float)x[e + k] : 0.0f;
+  }
   const uint64_t off = mask_offset(m);
-  const int64_t first = (int64_t)blockIdx.x * 256 + threadIdx.x;
-  if (first == 0 && used) *used = off;
-  for (int64_t i = first; i * VEC < n; i += (int64_t)gridDim.x * 256) {
-    const int64_t e = i * VEC;
-    float v[VEC];
-    const bool whole = e + VEC <= n;
-    if (whole) {
-      load_vec<T, VEC, ALIGNED, NT>(x + e, v);
-    } else {
+  if (e == 0 && used) *used = off;
 #pragma unroll
-      for (int k = 0; k < VEC; ++k) v[k] = e + k < n ? (float)x[e + k] : 0.0f;
-    }
+  for (int q = 0; q < VEC / 4; ++q) {
+    const Keep4 keep = keep_group(m, off, (uint64_t)(e >> 2) + q);
 #pragma unroll
-    for (int q = 0; q < VEC / 4; ++q) {
-      const Keep4 keep = keep_group(m, off, (uint64_t)(e >> 2) + q);
+    for (int k = 0; k < 4; ++k) v[4 * q + k] = keep.k[k] ? v[4 * q + k] * f : 0.0f;
+  }
+  if (whole) {
+    store_vec<T, VEC, ALIGNED, NT>(y + e, v);
+  } else {
 #pragma unroll
-      for (int k = 0; k < 4; ++k) v[4 * q + k] = keep.k[k] ? v[4 * q + k] * f : 0.0f;
-    }
-    if (whole) {
-      store_vec<T, VEC, ALIGNED, NT>(y + e, v);
-    } else {
-#pragma unroll
-      for (int k = 0; k < VEC; ++k)
-        if (e + k < n) y[e + k] = (T)v[k];
-    }
+    for (int k = 0; k < VEC; ++k)
+      if (e + k < n) y[e + k] = (T)v[k];
   }
 }
 
@@ -468,131 +472,66 @@ __global__ __launch_bounds__(kSortThreads) void sort_scatter_kernel(Src src, int
   }
 }
 
-// The same sort for N up to 1024 * ITEMS in one workgroup: keys and positions stay in registers and pass through LDS
-// between the digits, while the other workgroups of the launch write the gradient's zeros.
-constexpr int kSmallThreads = 1024, kSmallWaves = kSmallThreads / 64;
+// Short lists are sorted in one launch: the place of a pair is the number of pairs below it, counted against all of them.
+// A workgroup holds every pair in LDS as (key << 14) | index, so that they all differ; a wave takes kRankItems pairs at a
+// time, and each comparison of one with 64 others is one v_cmp, whose lanes the scalar unit counts. 16384 ids: 2.7e8
+// comparisons, 16 k vector cycles a SIMD. Workgroups beyond the first `blocks` write the gradient's zeros meanwhile.
+constexpr int kIndexBits = 14;
+constexpr int64_t kRankMax = 1 << kIndexBits;
+constexpr int kRankThreads = 1024, kRankItems = 4, kRankTile = kRankThreads / 64 * kRankItems;
 
-template <typename IT, int ITEMS>
-__global__ __launch_bounds__(kSmallThreads) void small_sort_kernel(KeyFromIds<IT> src, int N, int passes, int width,
-                                                                   uint32_t* keys_out, uint32_t* pos_out, Fill z) {
-  if (blockIdx.x > 0) {
-    fill_zeros(z, (int64_t)(blockIdx.x - 1) * kSmallThreads + threadIdx.x, (int64_t)(gridDim.x - 1) * kSmallThreads);
+template <typename IT, typename P>
+__global__ __launch_bounds__(kRankThreads) void rank_sort_kernel(KeyFromIds<IT> src, int N, int blocks, uint32_t* keys_out,
+                                                                 uint32_t* pos_out, Fill z) {
+  if ((int)blockIdx.x >= blocks) {
+    fill_zeros(z, (int64_t)(blockIdx.x - blocks) * kRankThreads + threadIdx.x,
+               (int64_t)(gridDim.x - blocks) * kRankThreads);
     return;
   }
-  constexpr int CAP = kSmallThreads * ITEMS;
-  __shared__ uint32_t skey[CAP];
-  __shared__ uint16_t spos[CAP];
-  __shared__ volatile uint32_t cnt[kSmallWaves][kBins];
-  __shared__ uint32_t scan[kBins];
-  const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63;
-  const uint32_t mask = (1u << width) - 1;
-  const int base = wave * (64 * ITEMS) + lane;
-  uint32_t key[ITEMS], rank[ITEMS];
-  uint16_t pos[ITEMS];
+  extern __shared__ __attribute__((aligned(16))) char rank_lds[];
+  P* pairs = (P*)rank_lds;
+  const int padded = (N + 255) / 256 * 256;
+  for (int i = threadIdx.x; i < padded; i += kRankThreads)
+    pairs[i] = i < N ? ((P)src.key(i) << kIndexBits) | (P)i : ~(P)0;  // no pair is below another than these
+  __syncthreads();
+  const int lane = threadIdx.x & 63;
+  const int first = blockIdx.x * kRankTile + (threadIdx.x >> 6) * kRankItems;
+  P item[kRankItems];
+  int rank[kRankItems];
 #pragma unroll
-  for (int j = 0; j < ITEMS; ++j) {
-    const int i = base + j * 64;
-    key[j] = i < N ? src.key(i) : 0u;
-    pos[j] = (uint16_t)i;
+  for (int t = 0; t < kRankItems; ++t) {
+    const P p = pairs[first + t < padded ? first + t : 0];
+    if constexpr (sizeof(P) == 4) {
+      item[t] = __builtin_amdgcn_readfirstlane(p);
+    } else {
+      item[t] = ((P)(uint32_t)__builtin_amdgcn_readfirstlane((uint32_t)(p >> 32)) << 32) |
+                (uint32_t)__builtin_amdgcn_readfirstlane((uint32_t)p);
+    }
+    rank[t] = 0;
   }
-  for (int pass = 0; pass < passes; ++pass) {
-    const int shift = pass * width;
-    for (int k = tid; k < kSmallWaves * kBins; k += kSmallThreads) (&cnt[0][0])[k] = 0;
-    __syncthreads();
+  for (int i = lane; i < padded; i += 256) {
+    P other[4];
 #pragma unroll
-    for (int j = 0; j < ITEMS; ++j) {
-      const bool valid = base + j * 64 < N;
-      const uint32_t dig = (key[j] >> shift) & mask;
-      const uint64_t peers = wave_match(dig, width, valid);
-      const uint32_t below = __popcll(peers & ((1ull << lane) - 1));
-      const uint32_t before = cnt[wave][dig];
-      rank[j] = before + below;
-      __builtin_amdgcn_wave_barrier();
-      if (valid && below == 0) cnt[wave][dig] = before + __popcll(peers);
-      __builtin_amdgcn_wave_barrier();
-    }
-    __syncthreads();
-    uint32_t total = 0;
-    if (tid < kBins) {
-      for (int w = 0; w < kSmallWaves; ++w) total += cnt[w][tid];
-      scan[tid] = total;
-    }
-    __syncthreads();
-    for (int o = 1; o < kBins; o <<= 1) {
-      uint32_t t = 0;
-      if (tid < kBins && tid >= o) t = scan[tid - o];
-      __syncthreads();
-      if (tid < kBins) scan[tid] += t;
-      __syncthreads();
-    }
-    if (tid < kBins) {
-      uint32_t at = scan[tid] - total;
-      for (int w = 0; w < kSmallWaves; ++w) {
-        const uint32_t c = cnt[w][tid];
-        cnt[w][tid] = at;
-        at += c;
-      }
-    }
-    __syncthreads();
+    for (int u = 0; u < 4; ++u) other[u] = pairs[i + u * 64];
 #pragma unroll
-    for (int j = 0; j < ITEMS; ++j) {
-      if (base + j * 64 < N) {
-        const uint32_t to = cnt[wave][(key[j] >> shift) & mask] + rank[j];
-        skey[to] = key[j];
-        spos[to] = pos[j];
-      }
-    }
-    __syncthreads();
+    for (int u = 0; u < 4; ++u)
 #pragma unroll
-    for (int j = 0; j < ITEMS; ++j) {
-      if (base + j * 64 < N) {
-        key[j] = skey[base + j * 64];
-        pos[j] = spos[base + j * 64];
-      }
-    }
+      for (int t = 0; t < kRankItems; ++t) rank[t] += __popcll(__ballot(other[u] < item[t]));
   }
 #pragma unroll
-  for (int j = 0; j < ITEMS; ++j) {
-    if (base + j * 64 < N) {
-      keys_out[base + j * 64] = key[j];
-      pos_out[base + j * 64] = pos[j];
+  for (int t = 0; t < kRankItems; ++t) {
+    if (lane == t && first + t < N) {
+      keys_out[rank[t]] = (uint32_t)(item[t] >> kIndexBits);
+      pos_out[rank[t]] = first + t;
     }
   }
 }
 
 // ------------------------------------------------------------------------------------------ gradient
-// A run is the sorted positions of one row. The positions are cut into equal pieces whatever the runs' lengths are, so
+// A run is the sorted positions of one row. Sorted positions are cut into equal pieces whatever the runs' lengths are, so
 // that a row named by most ids costs no more than many rows named once: a group of lanes (one vector of columns a lane)
-// adds a piece, writes the rows whose runs lie inside it, and leaves the sums of the runs that its ends cut. The workgroup
-// joins those of its groups in LDS, run_join_kernel those that cross workgroups. Pieces depend on N alone, so the order of
-// every sum does.
-struct RunPlan {
-  int vec;         // elements a lane
-  int lg;          // log2 of the lanes a group
-  int64_t chunks;  // column chunks of (1 << lg) * vec
-  int piece;       // positions a group, a multiple of 4
-  int64_t span, blocks;  // positions a workgroup, workgroups
-};
-
-inline RunPlan run_plan(int64_t N, int64_t D, int vec) {
-  RunPlan r;
-  r.vec = vec;
-  const int64_t dv = (D + vec - 1) / vec;
-  r.lg = 0;
-  while (r.lg < 6 && (1ll << r.lg) < dv) ++r.lg;
-  r.chunks = (dv + (1 << r.lg) - 1) >> r.lg;
-  const int64_t groups = 256 >> r.lg;
-  // enough workgroups for the chip, else longer pieces: fewer runs are cut
-  const int64_t want = 2048 / r.chunks > 0 ? 2048 / r.chunks : 1;
-  int64_t t = (N + groups * want - 1) / (groups * want);
-  t = t < 8 ? 8 : t > 64 ? 64 : t;
-  while ((N + groups * t - 1) / (groups * t) * r.chunks > (1 << 22)) t *= 2;
-  r.piece = (int)((t + 3) / 4 * 4);
-  r.span = groups * r.piece;
-  r.blocks = (N + r.span - 1) / r.span;
-  return r;
-}
-
+// adds a piece, writes the rows whose runs lie inside it, and leaves the sums of the runs that its ends cut, which are then
+// joined in the order of the pieces. Pieces depend on the ids alone, so the order of every sum does.
 template <typename GT, int VEC>
 __device__ __forceinline__ void masked_term(const GT* g, int64_t D, uint32_t pos, int64_t d, const Mask& m, uint64_t off,
                                             float (&v)[VEC]) {
@@ -601,6 +540,10 @@ __device__ __forceinline__ void masked_term(const GT* g, int64_t D, uint32_t pos
   if (m.mode == 0) return;
   if constexpr (VEC == 1) {
     if (!keep_at(m, off, (uint64_t)e)) v[0] = 0.0f;
+  } else if constexpr (VEC == 2) {
+    const Keep4 keep = keep_group(m, off, (uint64_t)(e >> 2));
+    v[0] = ((e & 2) ? keep.k[2] : keep.k[0]) ? v[0] : 0.0f;
+    v[1] = ((e & 2) ? keep.k[3] : keep.k[1]) ? v[1] : 0.0f;
   } else {
 #pragma unroll
     for (int q = 0; q < VEC / 4; ++q) {
@@ -611,49 +554,56 @@ __device__ __forceinline__ void masked_term(const GT* g, int64_t D, uint32_t pos
   }
 }
 
-template <typename TT, int VEC, bool ALIGNED>
-__device__ __forceinline__ void write_row(TT* grad, int64_t D, uint32_t row, int64_t d, float f, const float (&acc)[VEC]) {
+template <typename TT, int VEC>
+__device__ __forceinline__ void write_row(TT* grad, int64_t D, int64_t row, int64_t d, float f, const float (&acc)[VEC]) {
   float v[VEC];
 #pragma unroll
   for (int k = 0; k < VEC; ++k) v[k] = acc[k] * f;
-  store_vec<TT, VEC, ALIGNED, false>(grad + (int64_t)row * D + d, v);
+  store_vec<TT, VEC, (VEC > 1), false>(grad + row * D + d, v);
 }
 
+// What a workgroup's groups leave for each other in LDS: the sum of the run that entered a piece (head) and of the one
+// that leaves it (tail)
 enum { kHead = 1, kThrough = 2, kTail = 4 };
+template <int THREADS, int VEC>
+struct RunEnds {
+  float head[THREADS * VEC], tail[THREADS * VEC];
+  uint8_t flags[THREADS];
+};
 
-template <typename GT, typename TT, int VEC, bool ALIGNED>
-__global__ __launch_bounds__(256) void run_sum_kernel(const GT* g, const uint32_t* keys, const uint32_t* pos, int64_t N,
-                                                      uint32_t V, int64_t D, RunPlan r, Mask m, float f, TT* grad,
-                                                      float* heads, float* tails) {
-  __shared__ float head[256 * VEC], tail[256 * VEC];
-  __shared__ uint8_t flags[256];
-  const uint64_t off = mask_offset(m);
-  const int groups = 256 >> r.lg, group = threadIdx.x >> r.lg, sub = threadIdx.x & ((1 << r.lg) - 1);
-  const int64_t block = blockIdx.x % (uint32_t)r.blocks, chunk = blockIdx.x / (uint32_t)r.blocks;
-  const int64_t d = ((chunk << r.lg) + sub) * VEC;
+// Adds the sorted positions [0, N) of `src` that this workgroup's groups hold: group q the `piece` from base + q * piece.
+// src.key(i) orders the runs, src.pos(i) is the row of g, src.row(key) the row of the table; a key of src.none() takes no
+// part. The runs that enter or leave the workgroup's span go to heads / tails [D], which a workgroup with the whole of
+// [0, N) never writes.
+template <int THREADS, typename GT, typename TT, int VEC, typename Src>
+__device__ __forceinline__ void sum_runs(RunEnds<THREADS, VEC>& ends, const Src& src, int64_t N, int64_t base, int piece,
+                                         int lg, const GT* g, int64_t D, int64_t d, const Mask& m, uint64_t off, float f,
+                                         TT* grad, float* heads, float* tails) {
+  constexpr int U = 8;
+  const int groups = THREADS >> lg, group = threadIdx.x >> lg, sub = threadIdx.x & ((1 << lg) - 1);
   const bool col = d < D;
-  const int64_t base = block * r.span;
-  const int64_t a = base + (int64_t)group * r.piece;
-  const int64_t b = a + r.piece < N ? a + r.piece : N;
+  const int64_t a = base + (int64_t)group * piece;
+  const int64_t b = a + piece < N ? a + piece : N;
+  const uint32_t none = src.none();
   float acc[VEC];
 #pragma unroll
   for (int k = 0; k < VEC; ++k) acc[k] = 0.0f;
   int flag = 0;
-  uint32_t cur = V;
+  uint32_t cur = none;
   if (a < N) {
-    cur = keys[a];
-    bool cut = a > 0 && keys[a - 1] == cur;  // the run began in an earlier piece
-    for (int64_t i = a; i < b; i += 4) {
-      uint32_t kk[4], pp[4];
+    cur = src.key(a);
+    bool cut = a > 0 && src.key(a - 1) == cur;  // the run began in an earlier piece
+    for (int64_t i = a; i < b; i += U) {
+      uint32_t kk[U], pp[U];
 #pragma unroll
-      for (int u = 0; u < 4; ++u) {
-        kk[u] = i + u < b ? keys[i + u] : V;
-        pp[u] = i + u < b ? pos[i + u] : 0u;
+      for (int u = 0; u < U; ++u) {
+        kk[u] = i + u < b ? src.key(i + u) : none;
+        pp[u] = i + u < b ? src.pos(i + u) : 0u;
       }
-      float v[4][VEC];
+      float v[U][VEC];
 #pragma unroll
-      for (int u = 0; u < 4; ++u) {
-        if (kk[u] != V && col) {
+      for (int u = 0; u < U; ++u) {
+        if (kk[u] != none && col) {
           masked_term<GT, VEC>(g, D, pp[u], d, m, off, v[u]);
         } else {
 #pragma unroll
@@ -661,15 +611,15 @@ __global__ __launch_bounds__(256) void run_sum_kernel(const GT* g, const uint32_
         }
       }
 #pragma unroll
-      for (int u = 0; u < 4; ++u) {
+      for (int u = 0; u < U; ++u) {
         if (i + u < b) {
           if (kk[u] != cur) {
             if (cut) {
 #pragma unroll
-              for (int k = 0; k < VEC; ++k) head[threadIdx.x * VEC + k] = acc[k];
+              for (int k = 0; k < VEC; ++k) ends.head[threadIdx.x * VEC + k] = acc[k];
               flag |= kHead;
             } else if (col) {
-              write_row<TT, VEC, ALIGNED>(grad, D, cur, d, f, acc);
+              write_row<TT, VEC>(grad, D, src.row(cur), d, f, acc);
             }
             cut = false;
             cur = kk[u];
@@ -681,46 +631,251 @@ __global__ __launch_bounds__(256) void run_sum_kernel(const GT* g, const uint32_
         }
       }
     }
-    const bool goes_on = b < N && keys[b] == cur;
-    if (cur != V) {
+    const bool goes_on = b < N && src.key(b) == cur;
+    if (cur != none) {
       if (cut) {
 #pragma unroll
-        for (int k = 0; k < VEC; ++k) head[threadIdx.x * VEC + k] = acc[k];
+        for (int k = 0; k < VEC; ++k) ends.head[threadIdx.x * VEC + k] = acc[k];
         flag |= goes_on ? kHead | kThrough : kHead;
       } else if (goes_on) {
 #pragma unroll
-        for (int k = 0; k < VEC; ++k) tail[threadIdx.x * VEC + k] = acc[k];
+        for (int k = 0; k < VEC; ++k) ends.tail[threadIdx.x * VEC + k] = acc[k];
         flag |= kTail;
       } else if (col) {
-        write_row<TT, VEC, ALIGNED>(grad, D, cur, d, f, acc);
+        write_row<TT, VEC>(grad, D, src.row(cur), d, f, acc);
       }
     }
   }
-  if (sub == 0) flags[group] = (uint8_t)flag;
+  if (sub == 0) ends.flags[group] = (uint8_t)flag;
   __syncthreads();
   const bool from_before = group == 0 && (flag & kHead);
-  if (!from_before && !(flag & kTail)) return;
-  // two runs may leave a group 0: the one that came in (its sum goes to `heads`) and the one it starts
+  // two runs may leave group 0: the one that came in (its sum goes to `heads`) and the one it starts
   for (int which = from_before ? 0 : 1; which < 2; ++which) {
     if (which == 1 && !(flag & kTail)) break;
     float s[VEC];
 #pragma unroll
-    for (int k = 0; k < VEC; ++k) s[k] = (which ? tail : head)[threadIdx.x * VEC + k];
+    for (int k = 0; k < VEC; ++k) s[k] = (which ? ends.tail : ends.head)[threadIdx.x * VEC + k];
     bool open = which == 1 || (flag & kThrough);
     for (int h = group + 1; h < groups && open; ++h) {
 #pragma unroll
-      for (int k = 0; k < VEC; ++k) s[k] += head[(threadIdx.x + ((h - group) << r.lg)) * VEC + k];
-      open = flags[h] & kThrough;
+      for (int k = 0; k < VEC; ++k) s[k] += ends.head[(threadIdx.x + ((h - group) << lg)) * VEC + k];
+      open = ends.flags[h] & kThrough;
     }
     if (!col) continue;
     if (which == 0 || open) {
-      float* to = (which ? tails : heads) + block * D + d;
+      float* to = (which ? tails : heads) + d;
 #pragma unroll
       for (int k = 0; k < VEC; ++k) to[k] = s[k];
     } else {
-      write_row<TT, VEC, ALIGNED>(grad, D, cur, d, f, s);
+      write_row<TT, VEC>(grad, D, src.row(cur), d, f, s);
     }
   }
+}
+
+// ---- short id lists: one launch. Every workgroup owns a set of table rows (and a chunk of their columns): it reads all
+// ids, keeps the positions of its own rows in order, sorts them by row, adds their runs and writes zeros to its other
+// rows. The rows come in groups of 2^lgroup neighbours dealt out to the workgroups in turn, so that the low ids, which
+// word frequencies favour, spread over the chip. What it costs is that each workgroup reads every id (from L2).
+constexpr int kOwnThreads = 512, kOwnWaves = kOwnThreads / 64;
+constexpr int64_t kOwnMax = 4096;  // ids
+
+struct OwnPlan {
+  int lg;           // log2 of the lanes a group
+  int64_t chunks;   // column chunks
+  int lgroup, lown; // log2 of the rows a row group, of the owners of row groups
+  int64_t slots;    // rows an owner has (some beyond the table)
+  int cap;          // list entries, a power of two
+  int64_t lds;      // bytes of list and presence bits
+};
+
+inline OwnPlan own_plan(int64_t N, int64_t V, int64_t D, int vec, int64_t g_bytes, int64_t t_bytes) {
+  OwnPlan o;
+  const int64_t dv = (D + vec - 1) / vec;
+  o.lg = 0;
+  while (o.lg < 4 && (1ll << o.lg) < dv) ++o.lg;  // up to 16 lanes: 256 bytes of a row
+  while (o.lg < 6 && ((dv + (1 << o.lg) - 1) >> o.lg) > 64) ++o.lg;
+  o.chunks = (dv + (1 << o.lg) - 1) >> o.lg;
+  o.lgroup = 0;
+  while (((int64_t)1 << o.lgroup) * D * t_bytes < 128 && ((int64_t)1 << o.lgroup) < V) ++o.lgroup;
+  // owners: one for every 32 KB of zeros or 8 KB of gradient rows, up to 1024 workgroups
+  const int64_t most = 1024 / o.chunks > 1 ? 1024 / o.chunks : 1;
+  int64_t want = V * D * t_bytes / 32768;
+  want = want > N * D * g_bytes / 8192 ? want : N * D * g_bytes / 8192;
+  want = want < most ? want : most;
+  o.lown = 0;
+  while (((int64_t)1 << o.lown) < want && ((int64_t)1 << (o.lown + o.lgroup)) < V) ++o.lown;
+  const int64_t deal = (int64_t)1 << (o.lown + o.lgroup);
+  o.slots = (V + deal - 1) / deal << o.lgroup;
+  o.cap = 1;
+  while (o.cap < N) o.cap *= 2;
+  o.lds = (int64_t)o.cap * 4 + (o.slots + 31) / 32 * 4;
+  return o;
+}
+// the list packs (slot, index) into 32 bits, and list and presence bits share the LDS with RunEnds
+inline bool own_fits(int64_t N, const OwnPlan& o) {
+  return N <= kOwnMax && o.slots < (1ll << (32 - kIndexBits)) && o.lds <= 100 * 1024;
+}
+
+struct OwnList {
+  const uint32_t* list;
+  OwnPlan o;
+  uint32_t owner;
+  __device__ __forceinline__ uint32_t none() const { return 0xffffffffu; }
+  __device__ __forceinline__ uint32_t key(int64_t i) const { return list[i] >> kIndexBits; }
+  __device__ __forceinline__ uint32_t pos(int64_t i) const { return list[i] & ((1u << kIndexBits) - 1); }
+  __device__ __forceinline__ int64_t row(uint32_t slot) const {
+    return (((((int64_t)slot >> o.lgroup) << o.lown) + owner) << o.lgroup) + (slot & ((1u << o.lgroup) - 1));
+  }
+};
+
+template <typename GT, typename TT, int VEC>
+__global__ __launch_bounds__(kOwnThreads) void own_rows_kernel(const GT* g, const void* ids, int id_bytes, int N, int64_t V,
+                                                               int64_t D, int64_t pad, OwnPlan o, Mask m, float f,
+                                                               TT* grad) {
+  extern __shared__ uint32_t shared[];
+  __shared__ RunEnds<kOwnThreads, VEC> ends;
+  __shared__ int wave_count[kOwnWaves], unsorted;
+  uint32_t* list = shared;
+  uint32_t* present = shared + o.cap;
+  const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63;
+  const uint32_t owner = blockIdx.x & ((1u << o.lown) - 1);
+  const int64_t chunk = blockIdx.x >> o.lown;
+  const OwnList src{list, o, owner};
+  const uint32_t in_group = (1u << o.lgroup) - 1;
+  for (int k = tid; k < (o.slots + 31) / 32; k += kOwnThreads) present[k] = 0;
+  if (tid == 0) unsorted = 0;
+
+  // 1. the positions of this owner's rows, in order: count, then place
+  const int span = ((N + kOwnWaves - 1) / kOwnWaves + 63) / 64 * 64;  // a wave's consecutive ids
+  const int first = wave * span, end = first + span < N ? first + span : N;
+  auto slot_of = [&](int i) -> int64_t {  // -1: not this owner's
+    const int64_t id = id_bytes == 8 ? ((const int64_t*)ids)[i] : (int64_t)((const int32_t*)ids)[i];
+    const int64_t grp = id >> o.lgroup;
+    const bool mine = id >= 0 && id < V && id != pad && ((uint32_t)grp & ((1u << o.lown) - 1)) == owner;
+    return mine ? ((grp >> o.lown) << o.lgroup) + (id & in_group) : -1;
+  };
+  constexpr int B = 8;  // ids in flight a lane
+  int count = 0;
+  for (int i0 = first; i0 < end; i0 += 64 * B) {
+    int64_t slot[B];
+#pragma unroll
+    for (int u = 0; u < B; ++u) slot[u] = i0 + u * 64 + lane < end ? slot_of(i0 + u * 64 + lane) : -1;
+#pragma unroll
+    for (int u = 0; u < B; ++u) count += __popcll(__ballot(slot[u] >= 0));
+  }
+  if (lane == 0) wave_count[wave] = count;
+  __syncthreads();
+  int at = 0, M = 0;
+#pragma unroll
+  for (int w = 0; w < kOwnWaves; ++w) {
+    at += w < wave ? wave_count[w] : 0;
+    M += wave_count[w];
+  }
+  if (count) {
+    for (int i0 = first; i0 < end; i0 += 64 * B) {
+      int64_t slot[B];
+#pragma unroll
+      for (int u = 0; u < B; ++u) slot[u] = i0 + u * 64 + lane < end ? slot_of(i0 + u * 64 + lane) : -1;
+#pragma unroll
+      for (int u = 0; u < B; ++u) {
+        const uint64_t mine = __ballot(slot[u] >= 0);
+        if (slot[u] >= 0) {
+          list[at + __popcll(mine & ((1ull << lane) - 1))] =
+              ((uint32_t)slot[u] << kIndexBits) | (uint32_t)(i0 + u * 64 + lane);
+          atomicOr(&present[slot[u] >> 5], 1u << (slot[u] & 31));
+        }
+        at += __popcll(mine);
+      }
+    }
+  }
+  __syncthreads();
+
+  // 2. zeros for the rows that no position names
+  const int64_t d0 = (chunk << o.lg) * VEC;
+  for (int64_t t = tid; t < (o.slots << o.lg); t += kOwnThreads) {
+    const int64_t slot = t >> o.lg, d = d0 + (t & ((1 << o.lg) - 1)) * VEC;
+    const int64_t row = src.row((uint32_t)slot);
+    if (row < V && d < D && !(present[slot >> 5] >> (slot & 31) & 1)) {
+      const float zero[VEC] = {};
+      store_vec<TT, VEC, (VEC > 1), false>(grad + row * D + d, zero);
+    }
+  }
+
+  // 3. sort by (slot, index): the entries differ, so any sort is stable. Often there is nothing to do.
+  for (int i = tid; i + 1 < M; i += kOwnThreads)
+    if (list[i] > list[i + 1]) unsorted = 1;
+  __syncthreads();
+  if (unsorted) {
+    int n = 1;
+    while (n < M) n *= 2;
+    for (int i = M + tid; i < n; i += kOwnThreads) list[i] = 0xffffffffu;
+    __syncthreads();
+    for (int k = 2; k <= n; k *= 2) {
+      for (int j = k / 2; j > 0; j /= 2) {
+        for (int t = tid; t < n / 2; t += kOwnThreads) {
+          const int i = ((t & ~(j - 1)) << 1) | (t & (j - 1));
+          const uint32_t x = list[i], y = list[i + j];
+          if ((x > y) == ((i & k) == 0)) {
+            list[i] = y;
+            list[i + j] = x;
+          }
+        }
+        __syncthreads();
+      }
+    }
+  }
+
+  // 4. the runs
+  const int groups = kOwnThreads >> o.lg;
+  const int64_t d = d0 + (tid & ((1 << o.lg) - 1)) * VEC;
+  const int piece = (M + groups - 1) / groups;
+  sum_runs<kOwnThreads, GT, TT, VEC>(ends, src, M, 0, piece, o.lg, g, D, d, m, mask_offset(m), f, grad, nullptr, nullptr);
+}
+
+// ---- long id lists: the sorted pairs in memory, a workgroup's runs cut by its neighbours' joined in a second launch
+struct RunPlan {
+  int lg;          // log2 of the lanes a group
+  int64_t chunks;  // column chunks of (1 << lg) vectors
+  int piece;       // positions a group
+  int64_t span, blocks;  // positions a workgroup, workgroups
+};
+constexpr int kRunThreads = 256;
+
+inline RunPlan run_plan(int64_t N, int64_t D, int vec) {
+  RunPlan r;
+  const int64_t dv = (D + vec - 1) / vec;
+  r.lg = 0;
+  while (r.lg < 6 && (1ll << r.lg) < dv) ++r.lg;
+  r.chunks = (dv + (1 << r.lg) - 1) >> r.lg;
+  const int64_t groups = kRunThreads >> r.lg;
+  // enough workgroups for the chip, else longer pieces: fewer runs are cut
+  const int64_t want = 2048 / r.chunks > 0 ? 2048 / r.chunks : 1;
+  int64_t t = (N + groups * want - 1) / (groups * want);
+  t = t < 8 ? 8 : t > 64 ? 64 : t;
+  while ((N + groups * t - 1) / (groups * t) * r.chunks > (1 << 22)) t *= 2;
+  r.piece = (int)((t + 7) / 8 * 8);
+  r.span = groups * r.piece;
+  r.blocks = (N + r.span - 1) / r.span;
+  return r;
+}
+
+struct SortedPairs {
+  const uint32_t *keys, *poss;
+  uint32_t V;
+  __device__ __forceinline__ uint32_t none() const { return V; }
+  __device__ __forceinline__ uint32_t key(int64_t i) const { return keys[i]; }
+  __device__ __forceinline__ uint32_t pos(int64_t i) const { return poss[i]; }
+  __device__ __forceinline__ int64_t row(uint32_t key) const { return key; }
+};
+
+template <typename GT, typename TT, int VEC>
+__global__ __launch_bounds__(kRunThreads) void run_sum_kernel(const GT* g, SortedPairs src, int64_t N, int64_t D, RunPlan r,
+                                                              Mask m, float f, TT* grad, float* heads, float* tails) {
+  __shared__ RunEnds<kRunThreads, VEC> ends;
+  const int64_t block = blockIdx.x % (uint32_t)r.blocks, chunk = blockIdx.x / (uint32_t)r.blocks;
+  const int64_t d = ((chunk << r.lg) + (threadIdx.x & ((1 << r.lg) - 1))) * VEC;
+  sum_runs<kRunThreads, GT, TT, VEC>(ends, src, N, block * r.span, r.piece, r.lg, g, D, d, m, mask_offset(m), f, grad,
+                                     heads + block * D, tails + block * D);
 }
 
 // first position of [lo, hi) whose key is not below v
@@ -734,9 +889,10 @@ __device__ __forceinline__ int64_t lower_bound(const uint32_t* keys, int64_t lo,
 }
 
 // the run that workgroup b of run_sum_kernel started and did not end: its tail and the heads of the workgroups after it
-template <typename TT, int VEC, bool ALIGNED>
-__global__ __launch_bounds__(256) void run_join_kernel(const uint32_t* keys, int64_t N, uint32_t V, int64_t D, RunPlan r,
-                                                       float f, TT* grad, const float* heads, const float* tails) {
+template <typename TT, int VEC>
+__global__ __launch_bounds__(kRunThreads) void run_join_kernel(const uint32_t* keys, int64_t N, uint32_t V, int64_t D,
+                                                               RunPlan r, float f, TT* grad, const float* heads,
+                                                               const float* tails) {
   const int64_t b = blockIdx.x % (uint32_t)r.blocks, next = (b + 1) * r.span;
   if (next >= N) return;
   const uint32_t key = keys[next - 1];
@@ -746,8 +902,8 @@ __global__ __launch_bounds__(256) void run_join_kernel(const uint32_t* keys, int
   if (keys[end - 1] == key) end = lower_bound(keys, end, N, key + 1);
   else end = next + 1;  // ends inside the next workgroup
   const int64_t last = (end - 1) / r.span;
-  __shared__ float part[256 * VEC];
-  const int groups = 256 >> r.lg, group = threadIdx.x >> r.lg, sub = threadIdx.x & ((1 << r.lg) - 1);
+  __shared__ float part[kRunThreads * VEC];
+  const int groups = kRunThreads >> r.lg, group = threadIdx.x >> r.lg, sub = threadIdx.x & ((1 << r.lg) - 1);
   const int64_t d = (((int64_t)(blockIdx.x / (uint32_t)r.blocks) << r.lg) + sub) * VEC;
   const bool col = d < D;
   float s[VEC];
@@ -771,12 +927,10 @@ __global__ __launch_bounds__(256) void run_join_kernel(const uint32_t* keys, int
 #pragma unroll
     for (int k = 0; k < VEC; ++k) s[k] += part[(threadIdx.x + (q << r.lg)) * VEC + k];
   }
-  write_row<TT, VEC, ALIGNED>(grad, D, key, d, f, s);
+  write_row<TT, VEC>(grad, D, key, d, f, s);
 }
 
 // ------------------------------------------------------------------------------------------ workspace
-constexpr int64_t kSmallSort = 16 * kSmallThreads;
-
 struct GradWs {
   int64_t counts, totals, keys[2], pos[2], heads, tails, bytes;
 };
@@ -790,15 +944,14 @@ inline GradWs grad_ws(int64_t N, int64_t V, int64_t D) {
     at += (bytes + 255) / 256 * 256;
     return r;
   };
-  const bool small = N <= kSmallSort;
-  w.counts = take(small ? 0 : kBins * s.blocks * 4);
-  w.totals = take(small ? 0 : kBins * 4);
+  w.counts = take(kBins * s.blocks * 4);
+  w.totals = take(kBins * 4);
   for (int i = 0; i < 2; ++i) {
-    w.keys[i] = take(small && i ? 0 : N * 4);
-    w.pos[i] = take(small && i ? 0 : N * 4);
+    w.keys[i] = take(N * 4);
+    w.pos[i] = take(N * 4);
   }
   int64_t blocks = 0;  // of whichever vector the pointers' alignment allows
-  for (int vec : {1, 4, 8}) {
+  for (int vec : {1, 2, 4, 8}) {
     const int64_t b = run_plan(N, D, vec).blocks;
     blocks = b > blocks ? b : blocks;
   }
@@ -830,11 +983,14 @@ inline int sort_ids(const IT* ids, int64_t N, int64_t V, int64_t pad, char* ws, 
                     hipStream_t st) {
   const SortPlan s = sort_plan(N, V);
   const KeyFromIds<IT> src{ids, V, pad};
-  if (N <= kSmallSort) {
-    int64_t fill = z.bytes / (kSmallThreads * 16 * 2);
+  if (N <= kRankMax) {
+    const int blocks = (int)((N + kRankTile - 1) / kRankTile);
+    int64_t fill = z.bytes / (kRankThreads * 16 * 2);
     fill = fill < 1 ? 1 : fill > 1024 ? 1024 : fill;
-    auto* k = N <= 4 * kSmallThreads ? small_sort_kernel<IT, 4> : small_sort_kernel<IT, 16>;
-    hipLaunchKernelGGL(k, dim3((unsigned)(1 + fill)), dim3(kSmallThreads), 0, st, src, (int)N, s.passes, s.width,
+    const bool narrow = V < (1ll << (32 - kIndexBits));  // keys 0 .. V beside the index in 32 bits
+    auto* k = narrow ? rank_sort_kernel<IT, uint32_t> : rank_sort_kernel<IT, uint64_t>;
+    hipLaunchKernelGGL(k, dim3((unsigned)(blocks + fill)), dim3(kRankThreads),
+                       (unsigned)((N + 255) / 256 * 256 * (narrow ? 4 : 8)), st, src, (int)N, blocks,
                        (uint32_t*)(ws + w.keys[0]), (uint32_t*)(ws + w.pos[0]), z);
     return 0;
   }
@@ -888,9 +1044,12 @@ int yanerf_dropout(const void* x, int type, int64_t n, double p, uint64_t seed, 
   with_type(type, [&](auto t) {
     using T = decltype(t);
     constexpr int VEC = 16 / sizeof(T);
-    const dim3 grid = grid_for((n + 256 * VEC - 1) / (256 * VEC));
     auto* k = !al ? dropout_kernel<T, false, false> : nt ? dropout_kernel<T, true, true> : dropout_kernel<T, true, false>;
-    hipLaunchKernelGGL(k, grid, dim3(256), 0, as_stream(stream), (const T*)x, (T*)y, n, m, f, rng_used);
+    for (int64_t first = 0; first < n; first += 1ll << 32) {  // a launch holds fewer than 2^32 lanes
+      const int64_t part = n - first < 1ll << 32 ? n - first : 1ll << 32;
+      hipLaunchKernelGGL(k, dim3((unsigned)((part + 256 * VEC - 1) / (256 * VEC))), dim3(256), 0, as_stream(stream),
+                         (const T*)x, (T*)y, first + part, first, m, f, rng_used);
+    }
   });
   YN_LAUNCH_CHECK("dropout");
   return 0;
@@ -975,35 +1134,41 @@ int yanerf_embedding_backward(const void* g, int g_type, const void* ids, int id
     YN_LAUNCH_CHECK("embedding_backward");
     return 0;
   }
-  const GradWs w = grad_ws(N, V, D);
-  int at = 0;
-  with_index(id_bytes, [&](auto it) { at = sort_ids((const decltype(it)*)ids, N, V, padding_idx, ws, w, z, st); });
-  const uint32_t* keys = (const uint32_t*)(ws + w.keys[at]);
-  const uint32_t* pos = (const uint32_t*)(ws + w.pos[at]);
-  float *heads = (float*)(ws + w.heads), *tails = (float*)(ws + w.tails);
-  const int gb = (int)type_bytes(g_type);
-  const int vec = D % (16 / gb) == 0 && aligned(g, 16) ? 16 / gb : D % 4 == 0 && aligned(g, 4 * gb) ? 4 : 1;
-  const bool al = vec > 1 && aligned(grad_table, vec * type_bytes(table_type) < 16 ? vec * type_bytes(table_type) : 16);
-  const RunPlan r = run_plan(N, D, vec);
-  const dim3 grid((unsigned)(r.blocks * r.chunks));
+  // elements a lane: rows of g and of the gradient start at multiples of it, and loads are of up to 16 bytes
+  const int64_t gb = type_bytes(g_type), tb = type_bytes(table_type);
+  int vec = (int)(16 / gb);
+  while (vec > 1 && (D % vec || !aligned(g, vec * gb) || !aligned(grad_table, vec * tb < 16 ? vec * tb : 16))) vec /= 2;
+  auto launch = [&](auto gt, auto tt, auto vc) {
+    using GT = decltype(gt);
+    using TT = decltype(tt);
+    constexpr int VEC = decltype(vc)::value;
+    const OwnPlan o = own_plan(N < kOwnMax ? N : kOwnMax, V, D, VEC, gb, tb);
+    if (own_fits(N, o)) {
+      hipLaunchKernelGGL((own_rows_kernel<GT, TT, VEC>), dim3((unsigned)(o.chunks << o.lown)), dim3(kOwnThreads),
+                         (unsigned)o.lds, st, (const GT*)g, ids, id_bytes, (int)N, V, D, padding_idx, o, m, f,
+                         (TT*)grad_table);
+      return;
+    }
+    const GradWs w = grad_ws(N, V, D);
+    const RunPlan r = run_plan(N, D, VEC);
+    int at = 0;
+    with_index(id_bytes, [&](auto it) { at = sort_ids((const decltype(it)*)ids, N, V, padding_idx, ws, w, z, st); });
+    const SortedPairs src{(const uint32_t*)(ws + w.keys[at]), (const uint32_t*)(ws + w.pos[at]), (uint32_t)V};
+    float *heads = (float*)(ws + w.heads), *tails = (float*)(ws + w.tails);
+    const dim3 grid((unsigned)(r.blocks * r.chunks));
+    hipLaunchKernelGGL((run_sum_kernel<GT, TT, VEC>), grid, dim3(kRunThreads), 0, st, (const GT*)g, src, N, D, r, m, f,
+                       (TT*)grad_table, heads, tails);
+    if (r.blocks > 1)
+      hipLaunchKernelGGL((run_join_kernel<TT, VEC>), grid, dim3(kRunThreads), 0, st, src.keys, N, (uint32_t)V, D, r, f,
+                         (TT*)grad_table, heads, tails);
+  };
   with_type(g_type, [&](auto gt) {
     with_type(table_type, [&](auto tt) {
-      using GT = decltype(gt);
-      using TT = decltype(tt);
-      auto go = [&](auto vc, auto ac) {
-        constexpr int VEC = decltype(vc)::value;
-        constexpr bool AL = decltype(ac)::value;
-        hipLaunchKernelGGL((run_sum_kernel<GT, TT, VEC, AL>), grid, dim3(256), 0, st, (const GT*)g, keys, pos, N,
-                           (uint32_t)V, D, r, m, f, (TT*)grad_table, heads, tails);
-        if (r.blocks > 1)
-          hipLaunchKernelGGL((run_join_kernel<TT, VEC, AL>), grid, dim3(256), 0, st, keys, N, (uint32_t)V, D, r, f,
-                             (TT*)grad_table, heads, tails);
-      };
       using std::integral_constant;
-      if (vec == 1) go(integral_constant<int, 1>{}, std::false_type{});
-      else if (vec == 4) al ? go(integral_constant<int, 4>{}, std::true_type{}) : go(integral_constant<int, 4>{}, std::false_type{});
-      else if constexpr (sizeof(GT) == 2)
-        al ? go(integral_constant<int, 8>{}, std::true_type{}) : go(integral_constant<int, 8>{}, std::false_type{});
+      if (vec == 1) launch(gt, tt, integral_constant<int, 1>{});
+      else if (vec == 2) launch(gt, tt, integral_constant<int, 2>{});
+      else if (vec == 4) launch(gt, tt, integral_constant<int, 4>{});
+      else if constexpr (sizeof(gt) == 2) launch(gt, tt, integral_constant<int, 8>{});
     });
   });
   YN_LAUNCH_CHECK("embedding_backward");

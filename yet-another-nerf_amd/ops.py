@@ -501,11 +501,22 @@ _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)  # of a devic
 
 def _launch(dev: int, entry, *args) -> None:
     """entry(*args, stream) on device `dev` and its current stream, whichever device is current."""
-    here = torch.cuda.current_device()
-    with nullcontext() if dev == here else torch.cuda.device(dev):
-        stream = _raw_stream(dev) if _raw_stream is not None else torch.cuda.current_stream(dev).cuda_stream
-        if entry(*args, stream):
-            _C.check(1, entry.__name__)
+    if dev != torch.cuda.current_device():
+        with torch.cuda.device(dev):
+            return _launch(dev, entry, *args)
+    if entry(*args, _raw_stream(dev) if _raw_stream is not None else torch.cuda.current_stream(dev).cuda_stream):
+        _C.check(1, entry.__name__)
+
+
+def _once(backward):
+    """once_differentiable for a backward; its wrapper (1.4 us) is entered only where a graph of the backward is asked
+    for (create_graph=True)."""
+    wrapped = torch.autograd.function.once_differentiable(backward)
+
+    def call(ctx, g):
+        return wrapped(ctx, g) if torch.is_grad_enabled() else backward(ctx, g)
+
+    return call
 
 
 def _mask_rng(what: str, p: float, rng, rng_base: Optional[torch.Tensor], dev: torch.device, n: int):
@@ -537,21 +548,21 @@ def _mask_args(ctx, p: float, seed: int, offset: int, rng_base: Optional[torch.T
 
 class _DropoutFn(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, x, p, seed, offset, rng_base):
+    def forward(ctx, x, mask):
         x = x.contiguous()
         y = torch.empty_like(x)
         _launch(x.get_device(), _C.lib().yanerf_dropout, x.data_ptr(), _TYPES[x.dtype], x.numel(),
-                *_mask_args(ctx, p, seed, offset, rng_base, ctx.needs_input_grad[0]), y.data_ptr())
+                *_mask_args(ctx, *mask, ctx.needs_input_grad[0]), y.data_ptr())
         return y
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
+    @_once
     def backward(ctx, g):
         g = g.contiguous()
         out = torch.empty_like(g)
         _launch(g.get_device(), _C.lib().yanerf_dropout, g.data_ptr(), _TYPES[g.dtype], g.numel(), *ctx.mask, None,
                 out.data_ptr())
-        return out, None, None, None, None
+        return out, None
 
 
 def dropout(x: torch.Tensor, p: float, *, rng: Optional[Tuple[int, int]] = None,
@@ -567,7 +578,7 @@ def dropout(x: torch.Tensor, p: float, *, rng: Optional[Tuple[int, int]] = None,
     _code_type("dropout", x.dtype)
     p = _probability("dropout", p)
     seed, off = _mask_rng("dropout", p, rng, rng_base, x.device, x.numel())
-    return _DropoutFn.apply(x, p, seed, off, rng_base)
+    return _DropoutFn.apply(x, (p, seed, off, rng_base))
 
 
 _ID_FLAGS: dict = {}  # device -> sticky int32 flag of ids outside their table (set by the lookup's kernel, cleared here)
@@ -594,7 +605,7 @@ def check_embedding_ids(dev) -> None:
 
 class _EmbeddingFn(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, table, ids, scale, padding_idx, p, seed, offset, rng_base, out_dtype):
+    def forward(ctx, table, ids, scale, padding_idx, mask, out_dtype):
         V, D = table.shape
         if D > 1 and table.stride(1) != 1:
             table = table.contiguous()
@@ -604,7 +615,7 @@ class _EmbeddingFn(torch.autograd.Function):
         flag = _id_flag(table.device)
         _launch(table.get_device(), _C.lib().yanerf_embedding_forward, table.data_ptr(), _TYPES[table.dtype],
                 table.stride(0), ids.data_ptr(), ids.element_size(), ids.numel(), V, D, scale,
-                *_mask_args(ctx, p, seed, offset, rng_base, keep), out.data_ptr(), _TYPES[out_dtype],
+                *_mask_args(ctx, *mask, keep), out.data_ptr(), _TYPES[out_dtype],
                 None if flag is None else flag.data_ptr())
         if keep:
             ctx.dims = (V, D, table.dtype, scale, padding_idx)
@@ -612,7 +623,7 @@ class _EmbeddingFn(torch.autograd.Function):
         return out
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
+    @_once
     def backward(ctx, g):
         V, D, dtype, scale, pad = ctx.dims
         (ids,) = ctx.saved_tensors
@@ -623,7 +634,7 @@ class _EmbeddingFn(torch.autograd.Function):
         ws = torch.empty(L.yanerf_embedding_bwd_workspace_bytes(N, V, D), dtype=torch.uint8, device=g.device)
         _launch(g.get_device(), L.yanerf_embedding_backward, g.data_ptr(), _TYPES[g.dtype], ids.data_ptr(),
                 ids.element_size(), N, V, D, pad, scale, *ctx.mask, grad.data_ptr(), _TYPES[dtype], ws.data_ptr())
-        return grad, None, None, None, None, None, None, None, None
+        return grad, None, None, None, None, None
 
 
 def embedding(table: torch.Tensor, ids: torch.Tensor, *, scale: float = 1.0, padding_idx: Optional[int] = None,
@@ -663,7 +674,7 @@ def embedding(table: torch.Tensor, ids: torch.Tensor, *, scale: float = 1.0, pad
         raise ValueError("embedding: scale is not finite")
     p = _probability("embedding", dropout)
     seed, off = _mask_rng("embedding", p, rng, rng_base, table.device, ids.numel() * D)
-    out = _EmbeddingFn.apply(table, ids, scale, pad, p, seed, off, rng_base, out_dtype)
+    out = _EmbeddingFn.apply(table, ids, scale, pad, (p, seed, off, rng_base), out_dtype)
     if check:
         check_embedding_ids(table.device)
     return out
