@@ -66,13 +66,6 @@ inline double mask_scale(double p, const Mask& m) { return m.mode == 2 ? 0.0 : 1
 
 __device__ __forceinline__ uint64_t mask_offset(const Mask& m) { return m.offset + (m.base ? *m.base : 0ull); }
 
-__device__ __forceinline__ bool keep_at(const Mask& m, uint64_t off, uint64_t e) {
-  if (m.mode != 1) return m.mode == 0;
-  const u4 r = philox(m.seed, off, e >> 2);
-  const uint32_t w = (e & 2) ? ((e & 1) ? r.w : r.z) : ((e & 1) ? r.y : r.x);
-  return w >= m.threshold;
-}
-
 // keep of the elements 4 q .. 4 q + 3
 struct Keep4 {
   bool k[4];
@@ -84,6 +77,27 @@ __device__ __forceinline__ Keep4 keep_group(const Mask& m, uint64_t off, uint64_
   }
   const u4 r = philox(m.seed, off, q);
   return {{r.x >= m.threshold, r.y >= m.threshold, r.z >= m.threshold, r.w >= m.threshold}};
+}
+
+// zeros where the VEC elements from e, a multiple of VEC, are dropped
+template <int VEC>
+__device__ __forceinline__ void apply_keep(const Mask& m, uint64_t off, int64_t e, float (&v)[VEC]) {
+  if constexpr (VEC >= 4) {
+#pragma unroll
+    for (int q = 0; q < VEC / 4; ++q) {
+      const Keep4 keep = keep_group(m, off, (uint64_t)(e >> 2) + q);
+#pragma unroll
+      for (int k = 0; k < 4; ++k) v[4 * q + k] = keep.k[k] ? v[4 * q + k] : 0.0f;
+    }
+  } else {
+    const Keep4 keep = keep_group(m, off, (uint64_t)(e >> 2));
+#pragma unroll
+    for (int k = 0; k < VEC; ++k) {
+      const bool odd = VEC == 1 && (e & 1);
+      const bool lo = odd ? keep.k[1] : keep.k[k], hi = odd ? keep.k[3] : keep.k[2 + k];
+      v[k] = ((e & 2) ? hi : lo) ? v[k] : 0.0f;
+    }
+  }
 }
 
 // ------------------------------------------------------------------------------------------ vectors
@@ -182,11 +196,8 @@ __global__ __launch_bounds__(256) void dropout_kernel(const T* x, T* y, int64_t 
   const uint64_t off = mask_offset(m);
   if (e == 0 && used) *used = off;
 #pragma unroll
-  for (int q = 0; q < VEC / 4; ++q) {
-    const Keep4 keep = keep_group(m, off, (uint64_t)(e >> 2) + q);
-#pragma unroll
-    for (int k = 0; k < 4; ++k) v[4 * q + k] = keep.k[k] ? v[4 * q + k] * f : 0.0f;
-  }
+  for (int k = 0; k < VEC; ++k) v[k] *= f;
+  if (m.mode != 0) apply_keep<VEC>(m, off, e, v);
   if (whole) {
     store_vec<T, VEC, ALIGNED, NT>(y + e, v);
   } else {
@@ -241,14 +252,7 @@ __global__ __launch_bounds__(256) void embedding_rows_of_vectors_kernel(const TT
         const uint32_t t = t0 + u * 256;
         if (t < total) {
           const int64_t i = n0 * dv.d + t;  // the vector's index in the output
-          if (m.mode != 0) {
-#pragma unroll
-            for (int q = 0; q < VEC / 4; ++q) {
-              const Keep4 keep = keep_group(m, off, (uint64_t)i * (VEC / 4) + q);
-#pragma unroll
-              for (int k = 0; k < 4; ++k) v[u][4 * q + k] = keep.k[k] ? v[u][4 * q + k] : 0.0f;
-            }
-          }
+          if (m.mode != 0) apply_keep<VEC>(m, off, i * VEC, v[u]);
           store_vec<OT, VEC, true, NT>(out + i * VEC, v[u]);
         }
       }
@@ -300,45 +304,29 @@ __global__ __launch_bounds__(256) void embedding_any_rows_kernel(const TT* table
 }
 
 // ------------------------------------------------------------------------------------------ sort
-// Stable least-significant-digit radix sort of (id, position) pairs. Ids that take no part in the gradient (outside
-// the table, the padding row) get the key V, which sorts last. One pass: per-block digit counts, an exclusive scan of
-// each digit's counts over the blocks, and a scatter in which a wave ranks equal digits by ballots, so that equal keys
-// keep their order.
-constexpr int kSortThreads = 256, kSortWaves = kSortThreads / 64, kSortItems = 16;
-constexpr int kSortTile = kSortThreads * kSortItems;
-constexpr int kBins = 256;
-
-struct SortPlan {
-  int passes, width;
-  int64_t blocks;
+// Stable sorts of (id, position) pairs by id. Ids that take no part in the gradient (outside the table, the padding row)
+// get the key V, which sorts last.
+struct Pair {
+  uint32_t key, pos;
 };
 
-inline SortPlan sort_plan(int64_t N, int64_t V) {
-  int bits = 1;
-  while (bits < 32 && (V >> bits)) ++bits;  // keys 0 .. V
-  SortPlan s;
-  s.passes = (bits + 7) / 8;
-  s.width = (bits + s.passes - 1) / s.passes;
-  s.blocks = (N + kSortTile - 1) / kSortTile;
-  return s;
-}
-
-// first pass: keys come from the ids, positions are the indices themselves
+// where keys come from: the ids (positions are the indices themselves), or pairs
 template <typename IT>
 struct KeyFromIds {
   const IT* ids;
   int64_t V, pad;
-  __device__ __forceinline__ uint32_t key(int64_t i) const {
+  __device__ __forceinline__ Pair at(int64_t i) const {
     const int64_t id = (int64_t)ids[i];
-    return (uint32_t)((id < 0 || id >= V || id == pad) ? V : id);
+    return {(uint32_t)((id < 0 || id >= V || id == pad) ? V : id), (uint32_t)i};
   }
-  __device__ __forceinline__ uint32_t pos(int64_t i) const { return (uint32_t)i; }
 };
 struct KeyFromPairs {
-  const uint32_t *keys, *poss;
-  __device__ __forceinline__ uint32_t key(int64_t i) const { return keys[i]; }
-  __device__ __forceinline__ uint32_t pos(int64_t i) const { return poss[i]; }
+  const Pair* pairs;
+  __device__ __forceinline__ Pair at(int64_t i) const {
+    return __builtin_bit_cast(Pair, *(const uint64_t*)(pairs + i));
+  }
 };
+__device__ __forceinline__ void store_pair(Pair* to, Pair p) { *(uint64_t*)to = __builtin_bit_cast(uint64_t, p); }
 
 // the gradient's zeros, written beside the sort's first launch: rows that no id names keep them
 struct Fill {
@@ -355,95 +343,165 @@ __device__ __forceinline__ void fill_zeros(const Fill& z, int64_t worker, int64_
   }
   for (int64_t i = done / 2 + worker; i < z.bytes / 2; i += workers) ((uint16_t*)z.p)[i] = 0;
 }
-
 __global__ __launch_bounds__(256) void fill_kernel(Fill z) {
   fill_zeros(z, (int64_t)blockIdx.x * 256 + threadIdx.x, (int64_t)gridDim.x * 256);
 }
 
-template <typename Src>
-__global__ __launch_bounds__(kSortThreads) void sort_count_kernel(Src src, int64_t N, int shift, int width,
-                                                                  uint32_t* counts, int64_t blocks, Fill z) {
-  if (blockIdx.x >= blocks) {
-    fill_zeros(z, (blockIdx.x - blocks) * kSortThreads + threadIdx.x, (int64_t)(gridDim.x - blocks) * kSortThreads);
-    return;
-  }
-  __shared__ uint32_t hist[kBins];
-  hist[threadIdx.x] = 0;
-  __syncthreads();
-  const uint32_t mask = (1u << width) - 1;
-  const int64_t base = (int64_t)blockIdx.x * kSortTile;
-  for (int j = 0; j < kSortItems; ++j) {
-    const int64_t i = base + j * kSortThreads + threadIdx.x;
-    if (i < N) atomicAdd(&hist[(src.key(i) >> shift) & mask], 1u);
-  }
-  __syncthreads();
-  if (threadIdx.x <= mask) counts[threadIdx.x * blocks + blockIdx.x] = hist[threadIdx.x];
+// Long lists: least-significant-digit radix sort, digits of up to 10 bits. A pass counts the digits of each tile, scans each
+// digit's counts over the tiles, and scatters: a wave ranks equal digits by ballots, so that equal keys keep their order,
+// and a tile's pairs are first put in order in LDS, so that they leave as runs and not one by one. With no more than
+// kFewTiles tiles the scatter reads the counts of all of them itself and the scan's launch is left out.
+constexpr int kSortThreads = 256, kSortWaves = kSortThreads / 64;
+constexpr int64_t kFewTiles = 64;
+
+struct SortPlan {
+  int passes, width, bins, items;
+  int64_t tiles;
+};
+
+inline SortPlan sort_plan(int64_t N, int64_t V) {
+  int bits = 1;
+  while (bits < 32 && (V >> bits)) ++bits;  // keys 0 .. V
+  SortPlan s;
+  s.passes = (bits + 9) / 10;
+  s.width = (bits + s.passes - 1) / s.passes;
+  s.bins = s.width <= 8 ? 256 : 1024;
+  s.items = N <= kFewTiles * kSortThreads * 8 ? 8 : 16;
+  s.tiles = (N + kSortThreads * s.items - 1) / (kSortThreads * s.items);
+  return s;
 }
 
-// exclusive scan of counts[digit][0 .. blocks) in place, one workgroup a digit; its sum into totals[digit]
-__global__ __launch_bounds__(256) void sort_scan_kernel(uint32_t* counts, int64_t blocks, uint32_t* totals) {
-  __shared__ uint32_t part[256];
-  uint32_t* c = counts + (int64_t)blockIdx.x * blocks;
+template <typename Src, int BINS, int ITEMS>
+__global__ __launch_bounds__(kSortThreads) void sort_count_kernel(Src src, int64_t N, int shift, int width,
+                                                                  uint32_t* counts, int64_t tiles, Fill z) {
+  if (blockIdx.x >= tiles) {
+    fill_zeros(z, (blockIdx.x - tiles) * kSortThreads + threadIdx.x, (int64_t)(gridDim.x - tiles) * kSortThreads);
+    return;
+  }
+  __shared__ uint32_t hist[BINS];
+  for (int k = threadIdx.x; k < BINS; k += kSortThreads) hist[k] = 0;
+  __syncthreads();
+  const uint32_t mask = (1u << width) - 1;
+  const int64_t base = (int64_t)blockIdx.x * (kSortThreads * ITEMS) + threadIdx.x;
+  uint32_t key[ITEMS];
+#pragma unroll
+  for (int j = 0; j < ITEMS; ++j) key[j] = base + j * kSortThreads < N ? src.at(base + j * kSortThreads).key : 0u;
+#pragma unroll
+  for (int j = 0; j < ITEMS; ++j)
+    if (base + j * kSortThreads < N) atomicAdd(&hist[(key[j] >> shift) & mask], 1u);
+  __syncthreads();
+  for (int k = threadIdx.x; k <= (int)mask; k += kSortThreads) counts[k * tiles + blockIdx.x] = hist[k];
+}
+
+// sum of v over the lanes before this one, of the whole workgroup's in `total`; part has a slot a wave
+template <int WAVES>
+__device__ __forceinline__ uint32_t block_exclusive_scan(uint32_t v, uint32_t* part, uint32_t& total) {
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  uint32_t inc = v;
+#pragma unroll
+  for (int o = 1; o < 64; o <<= 1) {
+    const uint32_t t = __shfl_up(inc, o, 64);
+    if (lane >= o) inc += t;
+  }
+  __syncthreads();  // part may still be read from an earlier call
+  if (lane == 63) part[wave] = inc;
+  __syncthreads();
+  uint32_t before = 0;
+  total = 0;
+#pragma unroll
+  for (int w = 0; w < WAVES; ++w) {
+    before += w < wave ? part[w] : 0u;
+    total += part[w];
+  }
+  return before + inc - v;
+}
+
+// exclusive scan of counts[digit][0 .. tiles) in place, one workgroup a digit; its sum into totals[digit]
+__global__ __launch_bounds__(256) void sort_scan_kernel(uint32_t* counts, int64_t tiles, uint32_t* totals) {
+  __shared__ uint32_t part[4];
+  uint32_t* c = counts + (int64_t)blockIdx.x * tiles;
   uint32_t run = 0;
-  for (int64_t b0 = 0; b0 < blocks; b0 += 256) {
-    const int64_t b = b0 + threadIdx.x;
-    const uint32_t v = b < blocks ? c[b] : 0u;
-    part[threadIdx.x] = v;
-    __syncthreads();
-    for (int o = 1; o < 256; o <<= 1) {
-      const uint32_t t = threadIdx.x >= (unsigned)o ? part[threadIdx.x - o] : 0u;
-      __syncthreads();
-      part[threadIdx.x] += t;
-      __syncthreads();
+  for (int64_t b0 = 0; b0 < tiles; b0 += 1024) {
+    const int64_t b = b0 + threadIdx.x * 4;
+    uint32_t v[4], sum = 0, total;
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      v[k] = b + k < tiles ? c[b + k] : 0u;
+      sum += v[k];
     }
-    if (b < blocks) c[b] = run + part[threadIdx.x] - v;
-    run += part[255];
-    __syncthreads();
+    uint32_t at = run + block_exclusive_scan<4>(sum, part, total);
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      if (b + k < tiles) c[b + k] = at;
+      at += v[k];
+    }
+    run += total;
   }
   if (threadIdx.x == 0) totals[blockIdx.x] = run;
 }
 
 // lanes of this wave whose digit equals this lane's
-__device__ __forceinline__ uint64_t wave_match(uint32_t digit, int width, bool valid) {
-  uint64_t peers = __ballot(valid);
-  for (int b = 0; b < width; ++b) {
+template <int BITS>
+__device__ __forceinline__ uint64_t wave_match(uint32_t digit, bool valid) {
+  const uint64_t all = __ballot(valid);
+  uint32_t lo = (uint32_t)all, hi = (uint32_t)(all >> 32);
+#pragma unroll
+  for (int b = 0; b < BITS; ++b) {
     const uint64_t bal = __ballot((digit >> b) & 1);
-    peers &= ((digit >> b) & 1) ? bal : ~bal;
+    const uint32_t same = (digit >> b) & 1 ? 0u : ~0u;
+    lo &= (uint32_t)bal ^ same;
+    hi &= (uint32_t)(bal >> 32) ^ same;
   }
-  return peers;
+  return ((uint64_t)hi << 32) | lo;
 }
 
-template <typename Src>
+template <typename Src, int BINS, int ITEMS>
 __global__ __launch_bounds__(kSortThreads) void sort_scatter_kernel(Src src, int64_t N, int shift, int width,
-                                                                    const uint32_t* counts, int64_t blocks,
-                                                                    const uint32_t* totals, uint32_t* keys_out,
-                                                                    uint32_t* pos_out) {
-  __shared__ volatile uint32_t cnt[kSortWaves][kBins];  // a wave's count of each digit so far, then its first slot
-  __shared__ uint32_t scan[kBins];
-  const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
+                                                                    const uint32_t* counts, int64_t tiles,
+                                                                    const uint32_t* totals, Pair* out) {
+  constexpr int PER = BINS / kSortThreads, TILE = kSortThreads * ITEMS, BITS = BINS == 256 ? 8 : 10;
+  __shared__ volatile uint32_t cnt[kSortWaves][BINS];  // a wave's count of each digit so far, then its first slot
+  __shared__ uint32_t delta[BINS];                     // place in the output less place in the tile
+  __shared__ uint64_t sorted[TILE];
+  __shared__ uint32_t part[kSortWaves];
+  const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63;
   const uint32_t mask = (1u << width) - 1;
-  for (int w = 0; w < kSortWaves; ++w) cnt[w][threadIdx.x] = 0;
-  const uint32_t total = threadIdx.x <= mask ? totals[threadIdx.x] : 0u;
-  scan[threadIdx.x] = total;
+  for (int k = tid; k < kSortWaves * BINS; k += kSortThreads) (&cnt[0][0])[k] = 0;
+  const int64_t base = (int64_t)blockIdx.x * TILE;
+  const int64_t mine = base + wave * (64 * ITEMS) + lane;
+  Pair p[ITEMS];
+#pragma unroll
+  for (int j = 0; j < ITEMS; ++j) p[j] = mine + j * 64 < N ? src.at(mine + j * 64) : Pair{0, 0};
+  // where this tile's digits go: the digit's own place, after the same digit of the tiles before
+  uint32_t place[PER], sum = 0, all;
+#pragma unroll
+  for (int k = 0; k < PER; ++k) {
+    const uint32_t dig = tid * PER + k;
+    uint32_t before = 0, total = 0;
+    if (dig <= mask) {
+      const uint32_t* c = counts + (int64_t)dig * tiles;
+      if (totals) {
+        before = c[blockIdx.x];
+        total = totals[dig];
+      } else {
+        for (int64_t t = 0; t < tiles; ++t) {
+          const uint32_t v = c[t];
+          before += t < blockIdx.x ? v : 0u;
+          total += v;
+        }
+      }
+    }
+    place[k] = sum + before;
+    sum += total;
+  }
+  const uint32_t digit_base = block_exclusive_scan<kSortWaves>(sum, part, all);
   __syncthreads();
-  for (int o = 1; o < kBins; o <<= 1) {
-    const uint32_t t = threadIdx.x >= (unsigned)o ? scan[threadIdx.x - o] : 0u;
-    __syncthreads();
-    scan[threadIdx.x] += t;
-    __syncthreads();
-  }
-  const int64_t base = (int64_t)blockIdx.x * kSortTile + wave * (64 * kSortItems);
-  uint32_t key[kSortItems], rank[kSortItems];
+  uint32_t rank[ITEMS];
 #pragma unroll
-  for (int j = 0; j < kSortItems; ++j) {
-    const int64_t i = base + j * 64 + lane;
-    key[j] = i < N ? src.key(i) : 0u;
-  }
-#pragma unroll
-  for (int j = 0; j < kSortItems; ++j) {
-    const bool valid = base + j * 64 + lane < N;
-    const uint32_t dig = (key[j] >> shift) & mask;
-    const uint64_t peers = wave_match(dig, width, valid);
+  for (int j = 0; j < ITEMS; ++j) {
+    const bool valid = mine + j * 64 < N;
+    const uint32_t dig = (p[j].key >> shift) & mask;
+    const uint64_t peers = wave_match<BITS>(dig, valid);
     const uint32_t below = __popcll(peers & ((1ull << lane) - 1));
     const uint32_t before = cnt[wave][dig];
     rank[j] = before + below;
@@ -452,22 +510,40 @@ __global__ __launch_bounds__(kSortThreads) void sort_scatter_kernel(Src src, int
     __builtin_amdgcn_wave_barrier();
   }
   __syncthreads();
-  if (threadIdx.x <= mask) {
-    uint32_t at = scan[threadIdx.x] - total + counts[threadIdx.x * blocks + blockIdx.x];
+  sum = 0;
+  uint32_t here[PER];
+#pragma unroll
+  for (int k = 0; k < PER; ++k) {
+    here[k] = sum;
+#pragma unroll
+    for (int w = 0; w < kSortWaves; ++w) sum += cnt[w][tid * PER + k];
+  }
+  const uint32_t first = block_exclusive_scan<kSortWaves>(sum, part, all);
+#pragma unroll
+  for (int k = 0; k < PER; ++k) {
+    const int dig = tid * PER + k;
+    uint32_t at = first + here[k];
+    delta[dig] = digit_base + place[k] - at;
+#pragma unroll
     for (int w = 0; w < kSortWaves; ++w) {
-      const uint32_t c = cnt[w][threadIdx.x];
-      cnt[w][threadIdx.x] = at;
+      const uint32_t c = cnt[w][dig];
+      cnt[w][dig] = at;
       at += c;
     }
   }
   __syncthreads();
 #pragma unroll
-  for (int j = 0; j < kSortItems; ++j) {
-    const int64_t i = base + j * 64 + lane;
-    if (i < N) {
-      const uint32_t to = cnt[wave][(key[j] >> shift) & mask] + rank[j];
-      keys_out[to] = key[j];
-      pos_out[to] = src.pos(i);
+  for (int j = 0; j < ITEMS; ++j)
+    if (mine + j * 64 < N)
+      sorted[cnt[wave][(p[j].key >> shift) & mask] + rank[j]] = __builtin_bit_cast(uint64_t, p[j]);
+  __syncthreads();
+  const uint32_t held = (uint32_t)(N - base < TILE ? N - base : TILE);
+#pragma unroll
+  for (int j = 0; j < ITEMS; ++j) {
+    const uint32_t i = tid + j * kSortThreads;
+    if (i < held) {
+      const Pair q = __builtin_bit_cast(Pair, sorted[i]);
+      store_pair(out + (delta[(q.key >> shift) & mask] + i), q);
     }
   }
 }
@@ -481,8 +557,8 @@ constexpr int64_t kRankMax = 1 << kIndexBits;
 constexpr int kRankThreads = 1024, kRankItems = 4, kRankTile = kRankThreads / 64 * kRankItems;
 
 template <typename IT, typename P>
-__global__ __launch_bounds__(kRankThreads) void rank_sort_kernel(KeyFromIds<IT> src, int N, int blocks, uint32_t* keys_out,
-                                                                 uint32_t* pos_out, Fill z) {
+__global__ __launch_bounds__(kRankThreads) void rank_sort_kernel(KeyFromIds<IT> src, int N, int blocks, Pair* out,
+                                                                 Fill z) {
   if ((int)blockIdx.x >= blocks) {
     fill_zeros(z, (int64_t)(blockIdx.x - blocks) * kRankThreads + threadIdx.x,
                (int64_t)(gridDim.x - blocks) * kRankThreads);
@@ -492,7 +568,7 @@ __global__ __launch_bounds__(kRankThreads) void rank_sort_kernel(KeyFromIds<IT> 
   P* pairs = (P*)rank_lds;
   const int padded = (N + 255) / 256 * 256;
   for (int i = threadIdx.x; i < padded; i += kRankThreads)
-    pairs[i] = i < N ? ((P)src.key(i) << kIndexBits) | (P)i : ~(P)0;  // no pair is below another than these
+    pairs[i] = i < N ? ((P)src.at(i).key << kIndexBits) | (P)i : ~(P)0;  // no pair is below another than these
   __syncthreads();
   const int lane = threadIdx.x & 63;
   const int first = blockIdx.x * kRankTile + (threadIdx.x >> 6) * kRankItems;
@@ -520,10 +596,7 @@ __global__ __launch_bounds__(kRankThreads) void rank_sort_kernel(KeyFromIds<IT> 
   }
 #pragma unroll
   for (int t = 0; t < kRankItems; ++t) {
-    if (lane == t && first + t < N) {
-      keys_out[rank[t]] = (uint32_t)(item[t] >> kIndexBits);
-      pos_out[rank[t]] = first + t;
-    }
+    if (lane == t && first + t < N) store_pair(out + rank[t], {(uint32_t)(item[t] >> kIndexBits), (uint32_t)(first + t)});
   }
 }
 
@@ -537,21 +610,7 @@ __device__ __forceinline__ void masked_term(const GT* g, int64_t D, uint32_t pos
                                             float (&v)[VEC]) {
   const int64_t e = (int64_t)pos * D + d;
   load_vec<GT, VEC, (VEC > 1), false>(g + e, v);
-  if (m.mode == 0) return;
-  if constexpr (VEC == 1) {
-    if (!keep_at(m, off, (uint64_t)e)) v[0] = 0.0f;
-  } else if constexpr (VEC == 2) {
-    const Keep4 keep = keep_group(m, off, (uint64_t)(e >> 2));
-    v[0] = ((e & 2) ? keep.k[2] : keep.k[0]) ? v[0] : 0.0f;
-    v[1] = ((e & 2) ? keep.k[3] : keep.k[1]) ? v[1] : 0.0f;
-  } else {
-#pragma unroll
-    for (int q = 0; q < VEC / 4; ++q) {
-      const Keep4 keep = keep_group(m, off, (uint64_t)(e >> 2) + q);
-#pragma unroll
-      for (int k = 0; k < 4; ++k) v[4 * q + k] = keep.k[k] ? v[4 * q + k] : 0.0f;
-    }
-  }
+  if (m.mode != 0) apply_keep<VEC>(m, off, e, v);
 }
 
 template <typename TT, int VEC>
@@ -572,8 +631,8 @@ struct RunEnds {
 };
 
 // Adds the sorted positions [0, N) of `src` that this workgroup's groups hold: group q the `piece` from base + q * piece.
-// src.key(i) orders the runs, src.pos(i) is the row of g, src.row(key) the row of the table; a key of src.none() takes no
-// part. The runs that enter or leave the workgroup's span go to heads / tails [D], which a workgroup with the whole of
+// src.pair(i) holds the key that orders the runs and the row of g, src.row(key) is the row of the table; a key of
+// src.none() takes no part. The runs that enter or leave the workgroup's span go to heads / tails [D], which a workgroup with the whole of
 // [0, N) never writes.
 template <int THREADS, typename GT, typename TT, int VEC, typename Src>
 __device__ __forceinline__ void sum_runs(RunEnds<THREADS, VEC>& ends, const Src& src, int64_t N, int64_t base, int piece,
@@ -594,17 +653,14 @@ __device__ __forceinline__ void sum_runs(RunEnds<THREADS, VEC>& ends, const Src&
     cur = src.key(a);
     bool cut = a > 0 && src.key(a - 1) == cur;  // the run began in an earlier piece
     for (int64_t i = a; i < b; i += U) {
-      uint32_t kk[U], pp[U];
+      Pair q[U];
 #pragma unroll
-      for (int u = 0; u < U; ++u) {
-        kk[u] = i + u < b ? src.key(i + u) : none;
-        pp[u] = i + u < b ? src.pos(i + u) : 0u;
-      }
+      for (int u = 0; u < U; ++u) q[u] = i + u < b ? src.pair(i + u) : Pair{none, 0u};
       float v[U][VEC];
 #pragma unroll
       for (int u = 0; u < U; ++u) {
-        if (kk[u] != none && col) {
-          masked_term<GT, VEC>(g, D, pp[u], d, m, off, v[u]);
+        if (q[u].key != none && col) {
+          masked_term<GT, VEC>(g, D, q[u].pos, d, m, off, v[u]);
         } else {
 #pragma unroll
           for (int k = 0; k < VEC; ++k) v[u][k] = 0.0f;
@@ -613,7 +669,7 @@ __device__ __forceinline__ void sum_runs(RunEnds<THREADS, VEC>& ends, const Src&
 #pragma unroll
       for (int u = 0; u < U; ++u) {
         if (i + u < b) {
-          if (kk[u] != cur) {
+          if (q[u].key != cur) {
             if (cut) {
 #pragma unroll
               for (int k = 0; k < VEC; ++k) ends.head[threadIdx.x * VEC + k] = acc[k];
@@ -622,7 +678,7 @@ __device__ __forceinline__ void sum_runs(RunEnds<THREADS, VEC>& ends, const Src&
               write_row<TT, VEC>(grad, D, src.row(cur), d, f, acc);
             }
             cut = false;
-            cur = kk[u];
+            cur = q[u].key;
 #pragma unroll
             for (int k = 0; k < VEC; ++k) acc[k] = 0.0f;
           }
@@ -722,7 +778,10 @@ struct OwnList {
   uint32_t owner;
   __device__ __forceinline__ uint32_t none() const { return 0xffffffffu; }
   __device__ __forceinline__ uint32_t key(int64_t i) const { return list[i] >> kIndexBits; }
-  __device__ __forceinline__ uint32_t pos(int64_t i) const { return list[i] & ((1u << kIndexBits) - 1); }
+  __device__ __forceinline__ Pair pair(int64_t i) const {
+    const uint32_t e = list[i];
+    return {e >> kIndexBits, e & ((1u << kIndexBits) - 1)};
+  }
   __device__ __forceinline__ int64_t row(uint32_t slot) const {
     return (((((int64_t)slot >> o.lgroup) << o.lown) + owner) << o.lgroup) + (slot & ((1u << o.lgroup) - 1));
   }
@@ -860,11 +919,11 @@ inline RunPlan run_plan(int64_t N, int64_t D, int vec) {
 }
 
 struct SortedPairs {
-  const uint32_t *keys, *poss;
+  const Pair* pairs;
   uint32_t V;
   __device__ __forceinline__ uint32_t none() const { return V; }
-  __device__ __forceinline__ uint32_t key(int64_t i) const { return keys[i]; }
-  __device__ __forceinline__ uint32_t pos(int64_t i) const { return poss[i]; }
+  __device__ __forceinline__ uint32_t key(int64_t i) const { return pairs[i].key; }
+  __device__ __forceinline__ Pair pair(int64_t i) const { return KeyFromPairs{pairs}.at(i); }
   __device__ __forceinline__ int64_t row(uint32_t key) const { return key; }
 };
 
@@ -879,10 +938,10 @@ __global__ __launch_bounds__(kRunThreads) void run_sum_kernel(const GT* g, Sorte
 }
 
 // first position of [lo, hi) whose key is not below v
-__device__ __forceinline__ int64_t lower_bound(const uint32_t* keys, int64_t lo, int64_t hi, uint32_t v) {
+__device__ __forceinline__ int64_t lower_bound(const Pair* pairs, int64_t lo, int64_t hi, uint32_t v) {
   while (lo < hi) {
     const int64_t mid = (lo + hi) >> 1;
-    if (keys[mid] < v) lo = mid + 1;
+    if (pairs[mid].key < v) lo = mid + 1;
     else hi = mid;
   }
   return lo;
@@ -890,16 +949,16 @@ __device__ __forceinline__ int64_t lower_bound(const uint32_t* keys, int64_t lo,
 
 // the run that workgroup b of run_sum_kernel started and did not end: its tail and the heads of the workgroups after it
 template <typename TT, int VEC>
-__global__ __launch_bounds__(kRunThreads) void run_join_kernel(const uint32_t* keys, int64_t N, uint32_t V, int64_t D,
+__global__ __launch_bounds__(kRunThreads) void run_join_kernel(const Pair* pairs, int64_t N, uint32_t V, int64_t D,
                                                                RunPlan r, float f, TT* grad, const float* heads,
                                                                const float* tails) {
   const int64_t b = blockIdx.x % (uint32_t)r.blocks, next = (b + 1) * r.span;
   if (next >= N) return;
-  const uint32_t key = keys[next - 1];
-  if (key == V || keys[next] != key) return;
-  if (b > 0 && keys[b * r.span] == key && keys[b * r.span - 1] == key) return;  // it began earlier
+  const uint32_t key = pairs[next - 1].key;
+  if (key == V || pairs[next].key != key) return;
+  if (b > 0 && pairs[b * r.span].key == key && pairs[b * r.span - 1].key == key) return;  // it began earlier
   int64_t end = (b + 2) * r.span < N ? (b + 2) * r.span : N;
-  if (keys[end - 1] == key) end = lower_bound(keys, end, N, key + 1);
+  if (pairs[end - 1].key == key) end = lower_bound(pairs, end, N, key + 1);
   else end = next + 1;  // ends inside the next workgroup
   const int64_t last = (end - 1) / r.span;
   __shared__ float part[kRunThreads * VEC];
@@ -932,7 +991,7 @@ __global__ __launch_bounds__(kRunThreads) void run_join_kernel(const uint32_t* k
 
 // ------------------------------------------------------------------------------------------ workspace
 struct GradWs {
-  int64_t counts, totals, keys[2], pos[2], heads, tails, bytes;
+  int64_t counts, totals, pairs[2], heads, tails, bytes;
 };
 
 inline GradWs grad_ws(int64_t N, int64_t V, int64_t D) {
@@ -944,12 +1003,9 @@ inline GradWs grad_ws(int64_t N, int64_t V, int64_t D) {
     at += (bytes + 255) / 256 * 256;
     return r;
   };
-  w.counts = take(kBins * s.blocks * 4);
-  w.totals = take(kBins * 4);
-  for (int i = 0; i < 2; ++i) {
-    w.keys[i] = take(N * 4);
-    w.pos[i] = take(N * 4);
-  }
+  w.counts = take(s.bins * s.tiles * 4);
+  w.totals = take(s.bins * 4);
+  for (int i = 0; i < 2; ++i) w.pairs[i] = take(N * (int64_t)sizeof(Pair));
   int64_t blocks = 0;  // of whichever vector the pointers' alignment allows
   for (int vec : {1, 2, 4, 8}) {
     const int64_t b = run_plan(N, D, vec).blocks;
@@ -965,19 +1021,26 @@ template <typename Src>
 inline void sort_pass(Src src, int64_t N, int pass, const SortPlan& s, char* ws, const GradWs& w, const Fill& z,
                       hipStream_t st) {
   uint32_t* counts = (uint32_t*)(ws + w.counts);
-  uint32_t* totals = (uint32_t*)(ws + w.totals);
+  uint32_t* totals = s.tiles <= kFewTiles ? nullptr : (uint32_t*)(ws + w.totals);
   const int shift = pass * s.width;
   int64_t fill = z.bytes / (kSortThreads * 16 * 4);
   fill = z.bytes == 0 ? 0 : fill < 1 ? 1 : fill > 2048 ? 2048 : fill;
-  hipLaunchKernelGGL(sort_count_kernel<Src>, dim3((unsigned)(s.blocks + fill)), dim3(kSortThreads), 0, st, src, N, shift,
-                     s.width, counts, s.blocks, z);
-  hipLaunchKernelGGL(sort_scan_kernel, dim3(1u << s.width), dim3(256), 0, st, counts, s.blocks, totals);
-  hipLaunchKernelGGL(sort_scatter_kernel<Src>, dim3((unsigned)s.blocks), dim3(kSortThreads), 0, st, src, N, shift,
-                     s.width, counts, s.blocks, totals, (uint32_t*)(ws + w.keys[pass & 1]),
-                     (uint32_t*)(ws + w.pos[pass & 1]));
+  auto go = [&](auto bins, auto items) {
+    constexpr int BINS = decltype(bins)::value, ITEMS = decltype(items)::value;
+    hipLaunchKernelGGL((sort_count_kernel<Src, BINS, ITEMS>), dim3((unsigned)(s.tiles + fill)), dim3(kSortThreads), 0, st,
+                       src, N, shift, s.width, counts, s.tiles, z);
+    if (totals) hipLaunchKernelGGL(sort_scan_kernel, dim3(1u << s.width), dim3(256), 0, st, counts, s.tiles, totals);
+    hipLaunchKernelGGL((sort_scatter_kernel<Src, BINS, ITEMS>), dim3((unsigned)s.tiles), dim3(kSortThreads), 0, st, src, N,
+                       shift, s.width, counts, s.tiles, totals, (Pair*)(ws + w.pairs[pass & 1]));
+  };
+  using std::integral_constant;
+  if (s.bins == 256 && s.items == 8) go(integral_constant<int, 256>{}, integral_constant<int, 8>{});
+  else if (s.bins == 256) go(integral_constant<int, 256>{}, integral_constant<int, 16>{});
+  else if (s.items == 8) go(integral_constant<int, 1024>{}, integral_constant<int, 8>{});
+  else go(integral_constant<int, 1024>{}, integral_constant<int, 16>{});
 }
 
-// sorts the ids and clears the gradient; which of the two buffers holds the pairs
+// sorts the ids and clears the gradient; returns which of the two buffers holds the pairs
 template <typename IT>
 inline int sort_ids(const IT* ids, int64_t N, int64_t V, int64_t pad, char* ws, const GradWs& w, const Fill& z,
                     hipStream_t st) {
@@ -991,14 +1054,13 @@ inline int sort_ids(const IT* ids, int64_t N, int64_t V, int64_t pad, char* ws, 
     auto* k = narrow ? rank_sort_kernel<IT, uint32_t> : rank_sort_kernel<IT, uint64_t>;
     hipLaunchKernelGGL(k, dim3((unsigned)(blocks + fill)), dim3(kRankThreads),
                        (unsigned)((N + 255) / 256 * 256 * (narrow ? 4 : 8)), st, src, (int)N, blocks,
-                       (uint32_t*)(ws + w.keys[0]), (uint32_t*)(ws + w.pos[0]), z);
+                       (Pair*)(ws + w.pairs[0]), z);
     return 0;
   }
   for (int pass = 0; pass < s.passes; ++pass) {
     const int from = (pass - 1) & 1;
     if (pass == 0) sort_pass(src, N, pass, s, ws, w, z, st);
-    else sort_pass(KeyFromPairs{(const uint32_t*)(ws + w.keys[from]), (const uint32_t*)(ws + w.pos[from])}, N, pass, s, ws,
-                   w, Fill{nullptr, 0, 0}, st);
+    else sort_pass(KeyFromPairs{(const Pair*)(ws + w.pairs[from])}, N, pass, s, ws, w, Fill{nullptr, 0, 0}, st);
   }
   return (s.passes - 1) & 1;
 }
@@ -1074,7 +1136,7 @@ int yanerf_embedding_forward(const void* table, int table_type, int64_t table_st
     return D % vec == 0 && table_stride % vec == 0 && aligned(table, vec * type_bytes(table_type)) &&
            aligned(out, vec * type_bytes(out_type));
   };
-  const int64_t vec = fits(wide) ? wide : fits(4) ? 4 : 0;
+  const int64_t vec = fits(wide) ? wide : fits(4) ? 4 : fits(2) ? 2 : 0;
   const bool nt = streams_past_cache(N * D * type_bytes(out_type));
   with_type(table_type, [&](auto tt) {
     with_type(out_type, [&](auto ot) {
@@ -1085,7 +1147,9 @@ int yanerf_embedding_forward(const void* table, int table_type, int64_t table_st
         if (vec) {
           constexpr int W = 16 / (sizeof(TT) > sizeof(OT) ? sizeof(TT) : sizeof(OT));
           const int rows = tile_rows(N, D / vec, 256 * kUnroll, 1);
-          auto* k = vec == 4 ? (nt ? embedding_rows_of_vectors_kernel<TT, OT, IT, 4, true>
+          auto* k = vec == 2   ? (nt ? embedding_rows_of_vectors_kernel<TT, OT, IT, 2, true>
+                                     : embedding_rows_of_vectors_kernel<TT, OT, IT, 2, false>)
+                    : vec == 4 ? (nt ? embedding_rows_of_vectors_kernel<TT, OT, IT, 4, true>
                                    : embedding_rows_of_vectors_kernel<TT, OT, IT, 4, false>)
                              : (nt ? embedding_rows_of_vectors_kernel<TT, OT, IT, W, true>
                                    : embedding_rows_of_vectors_kernel<TT, OT, IT, W, false>);
@@ -1153,13 +1217,13 @@ int yanerf_embedding_backward(const void* g, int g_type, const void* ids, int id
     const RunPlan r = run_plan(N, D, VEC);
     int at = 0;
     with_index(id_bytes, [&](auto it) { at = sort_ids((const decltype(it)*)ids, N, V, padding_idx, ws, w, z, st); });
-    const SortedPairs src{(const uint32_t*)(ws + w.keys[at]), (const uint32_t*)(ws + w.pos[at]), (uint32_t)V};
+    const SortedPairs src{(const Pair*)(ws + w.pairs[at]), (uint32_t)V};
     float *heads = (float*)(ws + w.heads), *tails = (float*)(ws + w.tails);
     const dim3 grid((unsigned)(r.blocks * r.chunks));
     hipLaunchKernelGGL((run_sum_kernel<GT, TT, VEC>), grid, dim3(kRunThreads), 0, st, (const GT*)g, src, N, D, r, m, f,
                        (TT*)grad_table, heads, tails);
     if (r.blocks > 1)
-      hipLaunchKernelGGL((run_join_kernel<TT, VEC>), grid, dim3(kRunThreads), 0, st, src.keys, N, (uint32_t)V, D, r, f,
+      hipLaunchKernelGGL((run_join_kernel<TT, VEC>), grid, dim3(kRunThreads), 0, st, src.pairs, N, (uint32_t)V, D, r, f,
                          (TT*)grad_table, heads, tails);
   };
   with_type(g_type, [&](auto gt) {
