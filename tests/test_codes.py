@@ -38,7 +38,7 @@ def err():
 
 def test_dropout_c_refusals():
     L = _C.lib()
-    for args, msg in [((D16, 3, 8, 0.5), "type"), ((D16, 0, -1, 0.5), "range"), ((D16, 0, 1 << 39, 0.5), "range"),
+    for args, msg in [((D16, 3, 8, 0.5), "type"), ((D16, 0, -1, 0.5), "range"), ((D16, 0, (1 << 36) + 1, 0.5), "range"),
                       ((D16, 0, 8, -0.1), "probability"), ((D16, 0, 8, 1.5), "probability"),
                       ((D16, 0, 8, float("nan")), "probability"), ((None, 0, 8, 0.5), "null")]:
         assert L.yanerf_dropout(*args, 1, 2, None, None, D16, None) == 1
@@ -64,8 +64,8 @@ def bwd(**kw):
 @pytest.mark.parametrize("call", [fwd, bwd])
 @pytest.mark.parametrize("kw,msg", [
     (dict(tt=7), "type"), (dict(ib=2), "ids of 2"), (dict(N=-1), "negative"), (dict(V=-1), "negative"),
-    (dict(D=-1), "negative"), (dict(N=1 << 31), "2^31"), (dict(V=1 << 31), "2^31"), (dict(N=1 << 30, D=1 << 9), "2^38"), (dict(D=(1 << 24) + 1), "2^24"),
-    (dict(V=1 << 30, D=1 << 9), "2^38"), (dict(scale=float("inf")), "scale"), (dict(scale=float("nan")), "scale"),
+    (dict(D=-1), "negative"), (dict(N=1 << 31), "2^31"), (dict(V=1 << 31), "2^31"), (dict(N=1 << 30, D=1 << 9), "2^36"), (dict(D=(1 << 24) + 1), "2^24"),
+    (dict(V=1 << 30, D=1 << 9), "2^36"), (dict(scale=float("inf")), "scale"), (dict(scale=float("nan")), "scale"),
     (dict(p=1.01), "probability"), (dict(p=float("nan")), "probability"), (dict(ids=None), "null")])
 def test_embedding_c_refusals(call, kw, msg):
     assert call(**kw) == 1

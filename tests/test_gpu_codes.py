@@ -93,11 +93,24 @@ def test_wide_rows_and_many_ids(ops):
     check_train(ops, 500000, 100000, 2, kind="zipf", p=0.3, seed=8)
 
 
+@pytest.mark.parametrize("d", [1, 2, 3, 4, 5, 6, 7, 8])
+@pytest.mark.parametrize("dtype", TYPES, ids=NAME.get)
+def test_short_rows_and_long_lists(ops, d, dtype):
+    """Rows of up to 16 bytes by more than 16384 ids: buckets of one tile and of many, empty ones, one that holds all."""
+    check_train(ops, 20000, 3000, d, dtype=dtype, seed=d)
+    check_train(ops, 70001, 200000, d, dtype=dtype, kind="zipf", p=0.3, pad=1, idt=torch.int32, seed=d + 1)
+    check_train(ops, 50000, 9000, d, dtype=dtype, kind="one", p=0.3, seed=d + 2)
+    check_train(ops, 50000, 7, d, dtype=dtype, kind="sorted", seed=d + 3)
+    check_train(ops, 100001, 2050, d, dtype=dtype, kind="ends", seed=d + 4)
+
+
 @pytest.mark.parametrize("out", TYPES, ids=NAME.get)
 @pytest.mark.parametrize("dtype", TYPES, ids=NAME.get)
 def test_type_pairs(ops, dtype, out):
     for d in (2, 7, 48, 320):
         check_train(ops, 500, 60, d, dtype=dtype, out=out, scale=1.5, p=0.2, seed=d)
+        check_train(ops, 6000, 600, d, dtype=dtype, out=out, scale=1.5, p=0.2, seed=d)
+        check_train(ops, 18000, 600, d, dtype=dtype, out=out, scale=1.5, p=0.2, seed=d)
 
 
 @pytest.mark.parametrize("p", [0.0, 1e-9, 1e-4, 0.5, 0.999, 1.0 - 1e-12, 1.0])

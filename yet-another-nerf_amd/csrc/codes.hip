@@ -305,7 +305,7 @@ __global__ __launch_bounds__(256) void embedding_any_rows_kernel(const TT* table
 
 // ------------------------------------------------------------------------------------------ sort
 // Stable sorts of (id, position) pairs by id. Ids that take no part in the gradient (outside the table, the padding row)
-// get the key V, which sorts last.
+// get a key past the table (`none`), which sorts last.
 struct Pair {
   uint32_t key, pos;
 };
@@ -315,9 +315,10 @@ template <typename IT>
 struct KeyFromIds {
   const IT* ids;
   int64_t V, pad;
+  uint32_t none;
   __device__ __forceinline__ Pair at(int64_t i) const {
     const int64_t id = (int64_t)ids[i];
-    return {(uint32_t)((id < 0 || id >= V || id == pad) ? V : id), (uint32_t)i};
+    return {id < 0 || id >= V || id == pad ? none : (uint32_t)id, (uint32_t)i};
   }
 };
 struct KeyFromPairs {
@@ -455,10 +456,15 @@ __device__ __forceinline__ uint64_t wave_match(uint32_t digit, bool valid) {
   return ((uint64_t)hi << 32) | lo;
 }
 
-template <typename Src, int BINS, int ITEMS>
+struct StorePairs {
+  Pair* out;
+  __device__ __forceinline__ void operator()(int64_t to, Pair p) const { store_pair(out + to, p); }
+};
+
+template <typename Src, typename Dst, int BINS, int ITEMS>
 __global__ __launch_bounds__(kSortThreads) void sort_scatter_kernel(Src src, int64_t N, int shift, int width,
                                                                     const uint32_t* counts, int64_t tiles,
-                                                                    const uint32_t* totals, Pair* out) {
+                                                                    const uint32_t* totals, Dst dst) {
   constexpr int PER = BINS / kSortThreads, TILE = kSortThreads * ITEMS, BITS = BINS == 256 ? 8 : 10;
   __shared__ volatile uint32_t cnt[kSortWaves][BINS];  // a wave's count of each digit so far, then its first slot
   __shared__ uint32_t delta[BINS];                     // place in the output less place in the tile
@@ -543,7 +549,7 @@ __global__ __launch_bounds__(kSortThreads) void sort_scatter_kernel(Src src, int
     const uint32_t i = tid + j * kSortThreads;
     if (i < held) {
       const Pair q = __builtin_bit_cast(Pair, sorted[i]);
-      store_pair(out + (delta[(q.key >> shift) & mask] + i), q);
+      dst((int64_t)(delta[(q.key >> shift) & mask] + i), q);
     }
   }
 }
@@ -898,7 +904,7 @@ struct RunPlan {
   int piece;       // positions a group
   int64_t span, blocks;  // positions a workgroup, workgroups
 };
-constexpr int kRunThreads = 256;
+constexpr int kRunThreads = 256, kRunSpan = 2048;
 
 inline RunPlan run_plan(int64_t N, int64_t D, int vec) {
   RunPlan r;
@@ -910,31 +916,46 @@ inline RunPlan run_plan(int64_t N, int64_t D, int vec) {
   // enough workgroups for the chip, else longer pieces: fewer runs are cut
   const int64_t want = 2048 / r.chunks > 0 ? 2048 / r.chunks : 1;
   int64_t t = (N + groups * want - 1) / (groups * want);
-  t = t < 8 ? 8 : t > 64 ? 64 : t;
-  while ((N + groups * t - 1) / (groups * t) * r.chunks > (1 << 22)) t *= 2;
-  r.piece = (int)((t + 7) / 8 * 8);
+  const int64_t most = kRunSpan / groups < 64 ? kRunSpan / groups : 64;
+  t = t < 8 ? 8 : t > most ? most : t;
+  r.piece = (int)(t / 8 * 8);
   r.span = groups * r.piece;
   r.blocks = (N + r.span - 1) / r.span;
   return r;
 }
 
-struct SortedPairs {
-  const Pair* pairs;
+// a workgroup's span of the sorted pairs and their neighbours at both ends, in LDS; a gap after every 8 keeps the groups'
+// pieces, which start at multiples of 8, on different banks
+struct StagedPairs {
+  const uint64_t* lds;
+  int64_t base;
   uint32_t V;
+  static __device__ __forceinline__ int slot(int i) { return i + (i >> 3); }
   __device__ __forceinline__ uint32_t none() const { return V; }
-  __device__ __forceinline__ uint32_t key(int64_t i) const { return pairs[i].key; }
-  __device__ __forceinline__ Pair pair(int64_t i) const { return KeyFromPairs{pairs}.at(i); }
+  __device__ __forceinline__ Pair pair(int64_t i) const {
+    return __builtin_bit_cast(Pair, lds[slot((int)(i - base) + 8)]);
+  }
+  __device__ __forceinline__ uint32_t key(int64_t i) const { return pair(i).key; }
   __device__ __forceinline__ int64_t row(uint32_t key) const { return key; }
 };
 
 template <typename GT, typename TT, int VEC>
-__global__ __launch_bounds__(kRunThreads) void run_sum_kernel(const GT* g, SortedPairs src, int64_t N, int64_t D, RunPlan r,
-                                                              Mask m, float f, TT* grad, float* heads, float* tails) {
+__global__ __launch_bounds__(kRunThreads) void run_sum_kernel(const GT* g, const Pair* pairs, uint32_t V, int64_t N,
+                                                              int64_t D, RunPlan r, Mask m, float f, TT* grad,
+                                                              float* heads, float* tails) {
   __shared__ RunEnds<kRunThreads, VEC> ends;
+  __shared__ uint64_t staged[(kRunSpan + 16) / 8 * 9];
   const int64_t block = blockIdx.x % (uint32_t)r.blocks, chunk = blockIdx.x / (uint32_t)r.blocks;
   const int64_t d = ((chunk << r.lg) + (threadIdx.x & ((1 << r.lg) - 1))) * VEC;
-  sum_runs<kRunThreads, GT, TT, VEC>(ends, src, N, block * r.span, r.piece, r.lg, g, D, d, m, mask_offset(m), f, grad,
-                                     heads + block * D, tails + block * D);
+  const int64_t base = block * r.span;
+  const uint64_t* in = (const uint64_t*)pairs;
+  for (int k = threadIdx.x; k < r.span; k += kRunThreads)
+    if (base + k < N) staged[StagedPairs::slot(k + 8)] = in[base + k];
+  if (threadIdx.x == 0 && base > 0) staged[StagedPairs::slot(7)] = in[base - 1];
+  if (threadIdx.x == 1 && base + r.span < N) staged[StagedPairs::slot((int)r.span + 8)] = in[base + r.span];
+  __syncthreads();
+  sum_runs<kRunThreads, GT, TT, VEC>(ends, StagedPairs{staged, base, V}, N, base, r.piece, r.lg, g, D, d, m,
+                                     mask_offset(m), f, grad, heads + block * D, tails + block * D);
 }
 
 // first position of [lo, hi) whose key is not below v
@@ -989,6 +1010,185 @@ __global__ __launch_bounds__(kRunThreads) void run_join_kernel(const Pair* pairs
   write_row<TT, VEC>(grad, D, key, d, f, s);
 }
 
+// ---- long id lists of short rows (up to 16 bytes of g): gathering such rows one by one would fetch a cache line for each.
+// One partition by ranges of table rows carries the rows of g along, dropout applied; then a workgroup streams a tile of a
+// bucket, each wave into its own LDS table of the bucket's rows. Lanes of a wave that hold the same row add one after the
+// other in the order of the lanes, so that the sums' order is the ids' alone. A bucket of more than one tile leaves its
+// tiles' tables to a second launch. Every row of a bucket is written, so the gradient needs no zeros beforehand.
+constexpr int kBucketThreads = 512, kBucketWaves = kBucketThreads / 64;
+constexpr int64_t kBucketTile = 8192;    // positions a workgroup
+constexpr int64_t kBucketFloats = 2048;  // a wave's table
+
+struct BucketPlan {
+  int lrows;        // log2 of a bucket's rows
+  int64_t buckets;  // 0: the path does not fit
+  int64_t max_tiles;
+  int dm;           // elements a row of the tables and of the carried rows, a power of two
+};
+
+inline BucketPlan bucket_plan(int64_t N, int64_t V, int64_t D, int64_t g_bytes) {
+  BucketPlan b{0, 0, 0, 1};
+  if (D * g_bytes > 16) return b;
+  while (b.dm < D) b.dm *= 2;
+  // up to 1023 buckets (and one for the ids that take no part), none expected to hold less than half a tile
+  int64_t most = N / (kBucketTile / 2);
+  most = most < 1 ? 1 : most > 1023 ? 1023 : most;
+  while (((V + (1ll << b.lrows) - 1) >> b.lrows) > most && ((2ll << b.lrows) * b.dm <= kBucketFloats)) ++b.lrows;
+  const int64_t n = (V + (1ll << b.lrows) - 1) >> b.lrows;
+  if (n > 1023) return b;
+  b.buckets = n;
+  b.max_tiles = n + N / kBucketTile;
+  return b;
+}
+
+// the carried rows: DM elements of E bytes each, raw
+template <typename E, int DM>
+struct alignas(sizeof(E) * DM) Row {
+  E e[DM];
+};
+template <typename E, int DM>
+struct StoreRows {
+  const E* g;
+  int D;
+  Mask m;
+  uint32_t* keys;
+  Row<E, DM>* rows;
+  __device__ __forceinline__ void operator()(int64_t to, Pair p) const {
+    Row<E, DM> r;
+    const int64_t e = (int64_t)p.pos * D;
+#pragma unroll
+    for (int k = 0; k < DM; ++k) r.e[k] = k < D ? g[e + k] : (E)0;
+    if (m.mode != 0) {
+      const uint64_t off = mask_offset(m);
+      Keep4 keep = keep_group(m, off, (uint64_t)e >> 2);
+#pragma unroll
+      for (int k = 0; k < DM; ++k) {
+        if (k > 0 && ((e + k) & 3) == 0) keep = keep_group(m, off, (uint64_t)(e + k) >> 2);
+        const bool lo = (e + k) & 1 ? keep.k[1] : keep.k[0], hi = (e + k) & 1 ? keep.k[3] : keep.k[2];
+        if (!((e + k) & 2 ? hi : lo)) r.e[k] = (E)0;
+      }
+    }
+    keys[to] = p.key;
+    rows[to] = r;
+  }
+};
+
+// first position, positions, and the tiles before it, of the bucket that holds tile `tile`
+struct BucketTile {
+  uint32_t bucket, first, count, tile, tiles, tiles_before;
+};
+
+template <typename GT, typename TT, int DM>
+__global__ __launch_bounds__(kBucketThreads) void bucket_sum_kernel(const uint32_t* keys, const Row<GT, DM>* rows,
+                                                                    const uint32_t* totals, BucketPlan b, int64_t V, int D,
+                                                                    float f, TT* grad, float* partial,
+                                                                    BucketTile* multi) {
+  extern __shared__ float table[];  // [wave][row of the bucket][DM]
+  __shared__ uint32_t part[kBucketWaves];
+  __shared__ BucketTile me;
+  const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63;
+  const int floats = DM << b.lrows;
+  for (int k = tid; k < kBucketWaves * floats; k += kBucketThreads) table[k] = 0.0f;
+  if (tid == 0) me.bucket = 0xffffffffu;
+  // which bucket, which of its tiles: 2 buckets a lane
+  uint32_t cnt[2], nt[2], all;
+#pragma unroll
+  for (int k = 0; k < 2; ++k) {
+    cnt[k] = tid * 2 + k < b.buckets ? totals[tid * 2 + k] : 0u;
+    nt[k] = tid * 2 + k < b.buckets ? (cnt[k] > 0 ? (cnt[k] + (uint32_t)kBucketTile - 1) / (uint32_t)kBucketTile : 1u) : 0u;
+  }
+  uint32_t first = block_exclusive_scan<kBucketWaves>(cnt[0] + cnt[1], part, all);
+  uint32_t tile0 = block_exclusive_scan<kBucketWaves>(nt[0] + nt[1], part, all);
+#pragma unroll
+  for (int k = 0; k < 2; ++k) {
+    if (blockIdx.x >= tile0 && blockIdx.x < tile0 + nt[k])
+      me = {(uint32_t)(tid * 2 + k), first, cnt[k], blockIdx.x - tile0, nt[k], tile0};
+    first += cnt[k];
+    tile0 += nt[k];
+  }
+  __syncthreads();
+  const BucketTile t = me;
+  if (t.bucket == 0xffffffffu) return;  // fewer tiles than the most there can be
+  if (t.tile == 0 && tid == 0) multi[t.bucket] = t;
+  // the wave's consecutive positions, 64 at a time
+  constexpr int kPer = (int)(kBucketTile / kBucketWaves);
+  const uint32_t begin = t.tile * (uint32_t)kBucketTile + wave * kPer;
+  const uint32_t end = begin + kPer < t.count ? begin + kPer : t.count;
+  float* mine = table + wave * floats;
+  constexpr int U = 4;
+  for (uint32_t i0 = begin; i0 < end; i0 += 64 * U) {
+    uint32_t slot[U];
+    Row<GT, DM> r[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const uint32_t i = i0 + u * 64 + lane;
+      slot[u] = 0;
+      if (i < end) {
+        slot[u] = keys[t.first + i] & ((1u << b.lrows) - 1);
+        r[u] = rows[t.first + i];
+      }
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const bool valid = i0 + u * 64 + lane < end;
+      const uint64_t peers = wave_match<11>(slot[u], valid);
+      int turn = valid ? __popcll(peers & ((1ull << lane) - 1)) : -1;
+      for (int now = 0; __ballot(turn >= now); ++now) {
+        if (turn == now) {
+          volatile float* a = mine + slot[u] * DM;
+#pragma unroll
+          for (int k = 0; k < DM; ++k) a[k] = a[k] + (float)r[u].e[k];
+        }
+        __builtin_amdgcn_wave_barrier();
+      }
+    }
+  }
+  __syncthreads();
+  const int64_t row0 = (int64_t)t.bucket << b.lrows;
+  for (int k = tid; k < floats; k += kBucketThreads) {
+    float s = 0.0f;
+#pragma unroll
+    for (int w = 0; w < kBucketWaves; ++w) s += table[w * floats + k];
+    if (t.tiles > 1) {
+      partial[(int64_t)blockIdx.x * floats + k] = s;
+    } else {
+      const int64_t row = row0 + k / DM;
+      const int d = k % DM;
+      if (row < V && d < D) grad[row * D + d] = (TT)(s * f);
+    }
+  }
+}
+
+// buckets of more than one tile: their tiles' tables, added in order; `split` workgroups a bucket
+template <typename TT, int DM>
+__global__ __launch_bounds__(256) void bucket_join_kernel(const float* partial, const BucketTile* multi, BucketPlan b,
+                                                          int split, int64_t V, int D, float f, TT* grad) {
+  __shared__ float sums[256];
+  const uint32_t bucket = blockIdx.x / split;
+  const BucketTile t = multi[bucket];
+  if (t.tiles < 2) return;
+  const int floats = DM << b.lrows;
+  const int out = threadIdx.x & 63, part = threadIdx.x >> 6;  // 4 parts of the tiles
+  const uint32_t per = (t.tiles + 3) / 4;
+  const uint32_t begin = t.tiles_before + part * per, stop = t.tiles_before + t.tiles;
+  const uint32_t end = begin + per < stop ? begin + per : stop;
+  for (int k0 = (blockIdx.x % split) * 64; k0 < floats; k0 += split * 64) {
+    const int k = k0 + out;
+    float s = 0.0f;
+    if (k < floats) {
+#pragma unroll 8
+      for (uint32_t q = begin; q < end; ++q) s += partial[(int64_t)q * floats + k];
+    }
+    __syncthreads();
+    sums[threadIdx.x] = s;
+    __syncthreads();
+    const int64_t row = ((int64_t)t.bucket << b.lrows) + k / DM;
+    const int d = k % DM;
+    if (part == 0 && k < floats && row < V && d < D)
+      grad[row * D + d] = (TT)((((sums[out] + sums[64 + out]) + sums[128 + out]) + sums[192 + out]) * f);
+  }
+}
+
 // ------------------------------------------------------------------------------------------ workspace
 struct GradWs {
   int64_t counts, totals, pairs[2], heads, tails, bytes;
@@ -1017,6 +1217,31 @@ inline GradWs grad_ws(int64_t N, int64_t V, int64_t D) {
   return w;
 }
 
+struct BucketWs {
+  int64_t counts, totals, keys, rows, partial, multi, bytes;
+};
+
+constexpr int kBucketItems = 16;
+inline int64_t partition_tiles(int64_t N) { return (N + kSortThreads * kBucketItems - 1) / (kSortThreads * kBucketItems); }
+
+inline BucketWs bucket_ws(int64_t N, const BucketPlan& b, int64_t g_bytes) {
+  BucketWs w;
+  int64_t at = 0;
+  auto take = [&](int64_t bytes) {
+    const int64_t r = at;
+    at += (bytes + 255) / 256 * 256;
+    return r;
+  };
+  w.counts = take(1024 * partition_tiles(N) * 4);
+  w.totals = take(1024 * 4);
+  w.keys = take(N * 4);
+  w.rows = take(N * b.dm * g_bytes);
+  w.partial = take(b.max_tiles * ((int64_t)b.dm << b.lrows) * 4);
+  w.multi = take(1024 * (int64_t)sizeof(BucketTile));
+  w.bytes = at;
+  return w;
+}
+
 template <typename Src>
 inline void sort_pass(Src src, int64_t N, int pass, const SortPlan& s, char* ws, const GradWs& w, const Fill& z,
                       hipStream_t st) {
@@ -1030,8 +1255,8 @@ inline void sort_pass(Src src, int64_t N, int pass, const SortPlan& s, char* ws,
     hipLaunchKernelGGL((sort_count_kernel<Src, BINS, ITEMS>), dim3((unsigned)(s.tiles + fill)), dim3(kSortThreads), 0, st,
                        src, N, shift, s.width, counts, s.tiles, z);
     if (totals) hipLaunchKernelGGL(sort_scan_kernel, dim3(1u << s.width), dim3(256), 0, st, counts, s.tiles, totals);
-    hipLaunchKernelGGL((sort_scatter_kernel<Src, BINS, ITEMS>), dim3((unsigned)s.tiles), dim3(kSortThreads), 0, st, src, N,
-                       shift, s.width, counts, s.tiles, totals, (Pair*)(ws + w.pairs[pass & 1]));
+    hipLaunchKernelGGL((sort_scatter_kernel<Src, StorePairs, BINS, ITEMS>), dim3((unsigned)s.tiles), dim3(kSortThreads), 0,
+                       st, src, N, shift, s.width, counts, s.tiles, totals, StorePairs{(Pair*)(ws + w.pairs[pass & 1])});
   };
   using std::integral_constant;
   if (s.bins == 256 && s.items == 8) go(integral_constant<int, 256>{}, integral_constant<int, 8>{});
@@ -1045,7 +1270,7 @@ template <typename IT>
 inline int sort_ids(const IT* ids, int64_t N, int64_t V, int64_t pad, char* ws, const GradWs& w, const Fill& z,
                     hipStream_t st) {
   const SortPlan s = sort_plan(N, V);
-  const KeyFromIds<IT> src{ids, V, pad};
+  const KeyFromIds<IT> src{ids, V, pad, (uint32_t)V};
   if (N <= kRankMax) {
     const int blocks = (int)((N + kRankTile - 1) / kRankTile);
     int64_t fill = z.bytes / (kRankThreads * 16 * 2);
@@ -1065,12 +1290,37 @@ inline int sort_ids(const IT* ids, int64_t N, int64_t V, int64_t pad, char* ws, 
   return (s.passes - 1) & 1;
 }
 
+template <typename GT, typename TT, int DM, typename IT>
+inline void bucket_gradient(const GT* g, const IT* ids, int64_t N, int64_t V, int64_t D, int64_t pad, const BucketPlan& b,
+                            const Mask& m, float f, TT* grad, char* ws, hipStream_t st) {
+  typedef typename std::conditional<sizeof(GT) == 4, uint32_t, uint16_t>::type E;
+  const BucketWs w = bucket_ws(N, b, sizeof(GT));
+  uint32_t *counts = (uint32_t*)(ws + w.counts), *totals = (uint32_t*)(ws + w.totals), *keys = (uint32_t*)(ws + w.keys);
+  const int64_t tiles = partition_tiles(N);
+  const KeyFromIds<IT> src{ids, V, pad, (uint32_t)(b.buckets << b.lrows)};
+  hipLaunchKernelGGL((sort_count_kernel<KeyFromIds<IT>, 1024, kBucketItems>), dim3((unsigned)tiles), dim3(kSortThreads), 0,
+                     st, src, N, b.lrows, 10, counts, tiles, Fill{nullptr, 0, 0});
+  hipLaunchKernelGGL(sort_scan_kernel, dim3(1024), dim3(256), 0, st, counts, tiles, totals);
+  const StoreRows<E, DM> dst{(const E*)g, (int)D, m, keys, (Row<E, DM>*)(ws + w.rows)};
+  hipLaunchKernelGGL((sort_scatter_kernel<KeyFromIds<IT>, StoreRows<E, DM>, 1024, kBucketItems>), dim3((unsigned)tiles),
+                     dim3(kSortThreads), 0, st, src, N, b.lrows, 10, counts, tiles, totals, dst);
+  const unsigned lds = (unsigned)(kBucketWaves * ((int64_t)DM << b.lrows) * 4);
+  float* partial = (float*)(ws + w.partial);
+  BucketTile* multi = (BucketTile*)(ws + w.multi);
+  hipLaunchKernelGGL((bucket_sum_kernel<GT, TT, DM>), dim3((unsigned)b.max_tiles), dim3(kBucketThreads), lds, st, keys,
+                     (const Row<GT, DM>*)(ws + w.rows), totals, b, V, (int)D, f, grad, partial, multi);
+  int64_t split = 2048 / b.buckets, most = (((int64_t)DM << b.lrows) + 63) / 64;
+  split = split < 1 ? 1 : split > most ? most : split;
+  hipLaunchKernelGGL((bucket_join_kernel<TT, DM>), dim3((unsigned)(b.buckets * split)), dim3(256), 0, st, partial, multi, b,
+                     (int)split, V, (int)D, f, grad);
+}
+
 // sizes that the kernels' 32-bit positions and keys, and the grids, hold
 inline int embedding_sizes_ok(const char* what, int64_t N, int64_t V, int64_t D) {
   YN_CHECK(N >= 0 && V >= 0 && D >= 0, "%s: negative size", what);
   YN_CHECK(N < (1ll << 31) && V < (1ll << 31), "%s: N=%lld or V=%lld is 2^31 or more", what, (long long)N, (long long)V);
   YN_CHECK(D <= (1ll << 24), "%s: D=%lld is more than 2^24", what, (long long)D);
-  YN_CHECK(D == 0 || (N <= (1ll << 38) / D && V <= (1ll << 38) / D), "%s: more than 2^38 elements", what);
+  YN_CHECK(D == 0 || (N <= (1ll << 36) / D && V <= (1ll << 36) / D), "%s: more than 2^36 elements", what);
   return 0;
 }
 // rows a workgroup takes, so that it has about `work` units of `per_row` each (fewer where N of them leave CUs idle)
@@ -1096,7 +1346,7 @@ extern "C" {
 int yanerf_dropout(const void* x, int type, int64_t n, double p, uint64_t seed, uint64_t offset,
                    const uint64_t* rng_base, uint64_t* rng_used, void* y, void* stream) {
   YN_CHECK(type_ok(type), "dropout: unknown element type %d", type);
-  YN_CHECK(n >= 0 && n <= (1ll << 38), "dropout: n=%lld out of range", (long long)n);
+  YN_CHECK(n >= 0 && n <= (1ll << 36), "dropout: n=%lld out of range", (long long)n);
   if (mask_args_ok("dropout", p)) return 1;
   if (n == 0) return 0;
   YN_CHECK(x && y, "dropout: null pointer");
@@ -1171,7 +1421,16 @@ int yanerf_embedding_forward(const void* table, int table_type, int64_t table_st
 
 int64_t yanerf_embedding_bwd_workspace_bytes(int64_t N, int64_t V, int64_t D) {
   if (embedding_sizes_ok("embedding_bwd_workspace", N, V, D)) return -1;
-  return N == 0 || V == 0 || D == 0 ? 0 : grad_ws(N, V, D).bytes;
+  if (N == 0 || V == 0 || D == 0) return 0;
+  int64_t bytes = grad_ws(N, V, D).bytes;
+  for (int64_t gb : {2, 4}) {  // of whichever type g has
+    const BucketPlan b = bucket_plan(N, V, D, gb);
+    if (b.buckets) {
+      const int64_t n = bucket_ws(N, b, gb).bytes;
+      bytes = n > bytes ? n : bytes;
+    }
+  }
+  return bytes;
 }
 
 int yanerf_embedding_backward(const void* g, int g_type, const void* ids, int id_bytes, int64_t N, int64_t V,
@@ -1213,17 +1472,33 @@ int yanerf_embedding_backward(const void* g, int g_type, const void* ids, int id
                          (TT*)grad_table);
       return;
     }
+    const BucketPlan b = bucket_plan(N, V, D, gb);
+    if (N > kRankMax && b.buckets) {
+      with_index(id_bytes, [&](auto it) {
+        using IT = decltype(it);
+        auto go = [&](auto dm) {
+          bucket_gradient<GT, TT, decltype(dm)::value>((const GT*)g, (const IT*)ids, N, V, D, padding_idx, b, m, f,
+                                                       (TT*)grad_table, ws, st);
+        };
+        using std::integral_constant;
+        if (b.dm == 1) go(integral_constant<int, 1>{});
+        else if (b.dm == 2) go(integral_constant<int, 2>{});
+        else if (b.dm == 4) go(integral_constant<int, 4>{});
+        else if constexpr (sizeof(GT) == 2) go(integral_constant<int, 8>{});
+      });
+      return;
+    }
     const GradWs w = grad_ws(N, V, D);
     const RunPlan r = run_plan(N, D, VEC);
     int at = 0;
     with_index(id_bytes, [&](auto it) { at = sort_ids((const decltype(it)*)ids, N, V, padding_idx, ws, w, z, st); });
-    const SortedPairs src{(const Pair*)(ws + w.pairs[at]), (uint32_t)V};
+    const Pair* pairs = (const Pair*)(ws + w.pairs[at]);
     float *heads = (float*)(ws + w.heads), *tails = (float*)(ws + w.tails);
     const dim3 grid((unsigned)(r.blocks * r.chunks));
-    hipLaunchKernelGGL((run_sum_kernel<GT, TT, VEC>), grid, dim3(kRunThreads), 0, st, (const GT*)g, src, N, D, r, m, f,
-                       (TT*)grad_table, heads, tails);
+    hipLaunchKernelGGL((run_sum_kernel<GT, TT, VEC>), grid, dim3(kRunThreads), 0, st, (const GT*)g, pairs, (uint32_t)V, N, D, r,
+                       m, f, (TT*)grad_table, heads, tails);
     if (r.blocks > 1)
-      hipLaunchKernelGGL((run_join_kernel<TT, VEC>), grid, dim3(kRunThreads), 0, st, src.pairs, N, (uint32_t)V, D, r, f,
+      hipLaunchKernelGGL((run_join_kernel<TT, VEC>), grid, dim3(kRunThreads), 0, st, pairs, N, (uint32_t)V, D, r, f,
                          (TT*)grad_table, heads, tails);
   };
   with_type(g_type, [&](auto gt) {
