@@ -379,8 +379,10 @@ __global__ __launch_bounds__(kSortThreads) void sort_count_kernel(Src src, int64
     fill_zeros(z, (blockIdx.x - tiles) * kSortThreads + threadIdx.x, (int64_t)(gridDim.x - tiles) * kSortThreads);
     return;
   }
-  __shared__ uint32_t hist[BINS];
-  for (int k = threadIdx.x; k < BINS; k += kSortThreads) hist[k] = 0;
+  // neighbouring ids often share a digit: copies of the counts, by lane, keep them from waiting for one another
+  constexpr int COPIES = 8;
+  __shared__ uint32_t hist[BINS * COPIES];
+  for (int k = threadIdx.x; k < BINS * COPIES; k += kSortThreads) hist[k] = 0;
   __syncthreads();
   const uint32_t mask = (1u << width) - 1;
   const int64_t base = (int64_t)blockIdx.x * (kSortThreads * ITEMS) + threadIdx.x;
@@ -389,9 +391,14 @@ __global__ __launch_bounds__(kSortThreads) void sort_count_kernel(Src src, int64
   for (int j = 0; j < ITEMS; ++j) key[j] = base + j * kSortThreads < N ? src.at(base + j * kSortThreads).key : 0u;
 #pragma unroll
   for (int j = 0; j < ITEMS; ++j)
-    if (base + j * kSortThreads < N) atomicAdd(&hist[(key[j] >> shift) & mask], 1u);
+    if (base + j * kSortThreads < N) atomicAdd(&hist[((key[j] >> shift) & mask) * COPIES + threadIdx.x % COPIES], 1u);
   __syncthreads();
-  for (int k = threadIdx.x; k <= (int)mask; k += kSortThreads) counts[k * tiles + blockIdx.x] = hist[k];
+  for (int k = threadIdx.x; k < BINS; k += kSortThreads) {
+    uint32_t sum = 0;
+#pragma unroll
+    for (int c = 0; c < COPIES; ++c) sum += hist[k * COPIES + c];
+    counts[(int64_t)blockIdx.x * BINS + k] = sum;
+  }
 }
 
 // sum of v over the lanes before this one, of the whole workgroup's in `total`; part has a slot a wave
@@ -417,28 +424,34 @@ __device__ __forceinline__ uint32_t block_exclusive_scan(uint32_t v, uint32_t* p
   return before + inc - v;
 }
 
-// exclusive scan of counts[digit][0 .. tiles) in place, one workgroup a digit; its sum into totals[digit]
-__global__ __launch_bounds__(256) void sort_scan_kernel(uint32_t* counts, int64_t tiles, uint32_t* totals) {
-  __shared__ uint32_t part[4];
-  uint32_t* c = counts + (int64_t)blockIdx.x * tiles;
-  uint32_t run = 0;
-  for (int64_t b0 = 0; b0 < tiles; b0 += 1024) {
-    const int64_t b = b0 + threadIdx.x * 4;
-    uint32_t v[4], sum = 0, total;
-#pragma unroll
-    for (int k = 0; k < 4; ++k) {
-      v[k] = b + k < tiles ? c[b + k] : 0u;
-      sum += v[k];
-    }
-    uint32_t at = run + block_exclusive_scan<4>(sum, part, total);
-#pragma unroll
-    for (int k = 0; k < 4; ++k) {
-      if (b + k < tiles) c[b + k] = at;
-      at += v[k];
-    }
-    run += total;
+// exclusive scan of counts[0 .. tiles)[digit] in place, 16 digits a workgroup, whose 64 parts take consecutive tiles; the
+// digits' sums into totals
+constexpr int kScanDigits = 16, kScanParts = 64, kScanThreads = kScanDigits * kScanParts;
+__global__ __launch_bounds__(kScanThreads) void sort_scan_kernel(uint32_t* counts, int64_t tiles, int bins,
+                                                                 uint32_t* totals) {
+  __shared__ uint32_t sums[kScanParts][kScanDigits];
+  const int dig = threadIdx.x % kScanDigits, part = threadIdx.x / kScanDigits;
+  const int64_t per = (tiles + kScanParts - 1) / kScanParts;
+  const int64_t begin = part * per, end = begin + per < tiles ? begin + per : tiles;
+  uint32_t* c = counts + blockIdx.x * kScanDigits + dig;
+  uint32_t sum = 0;
+#pragma unroll 8
+  for (int64_t t = begin; t < end; ++t) sum += c[t * bins];
+  sums[part][dig] = sum;
+  __syncthreads();
+  uint32_t at = 0, total = 0;
+#pragma unroll 16
+  for (int q = 0; q < kScanParts; ++q) {
+    at += q < part ? sums[q][dig] : 0u;
+    total += sums[q][dig];
   }
-  if (threadIdx.x == 0) totals[blockIdx.x] = run;
+#pragma unroll 8
+  for (int64_t t = begin; t < end; ++t) {
+    const uint32_t v = c[t * bins];
+    c[t * bins] = at;
+    at += v;
+  }
+  if (part == 0) totals[blockIdx.x * kScanDigits + dig] = total;
 }
 
 // lanes of this wave whose digit equals this lane's
@@ -466,9 +479,12 @@ __global__ __launch_bounds__(kSortThreads) void sort_scatter_kernel(Src src, int
                                                                     const uint32_t* counts, int64_t tiles,
                                                                     const uint32_t* totals, Dst dst) {
   constexpr int PER = BINS / kSortThreads, TILE = kSortThreads * ITEMS, BITS = BINS == 256 ? 8 : 10;
-  __shared__ volatile uint32_t cnt[kSortWaves][BINS];  // a wave's count of each digit so far, then its first slot
-  __shared__ uint32_t delta[BINS];                     // place in the output less place in the tile
-  __shared__ uint64_t sorted[TILE];
+  __shared__ union {
+    uint32_t cnt[kSortWaves][BINS];  // a wave's count of each digit so far, then its first slot
+    uint64_t sorted[TILE];           // the tile in order, once every lane knows its slots
+  } u;
+  volatile uint32_t(*cnt)[BINS] = u.cnt;
+  __shared__ uint32_t delta[BINS];  // place in the output less place in the tile
   __shared__ uint32_t part[kSortWaves];
   const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63;
   const uint32_t mask = (1u << width) - 1;
@@ -485,14 +501,15 @@ __global__ __launch_bounds__(kSortThreads) void sort_scatter_kernel(Src src, int
     const uint32_t dig = tid * PER + k;
     uint32_t before = 0, total = 0;
     if (dig <= mask) {
-      const uint32_t* c = counts + (int64_t)dig * tiles;
+      const uint32_t* c = counts + dig;
       if (totals) {
-        before = c[blockIdx.x];
+        before = c[(int64_t)blockIdx.x * BINS];
         total = totals[dig];
       } else {
-        for (int64_t t = 0; t < tiles; ++t) {
-          const uint32_t v = c[t];
-          before += t < blockIdx.x ? v : 0u;
+#pragma unroll 8
+        for (int t = 0; t < (int)tiles; ++t) {
+          const uint32_t v = c[t * BINS];
+          before += t < (int)blockIdx.x ? v : 0u;
           total += v;
         }
       }
@@ -539,70 +556,99 @@ __global__ __launch_bounds__(kSortThreads) void sort_scatter_kernel(Src src, int
   }
   __syncthreads();
 #pragma unroll
+  for (int j = 0; j < ITEMS; ++j) rank[j] += cnt[wave][(p[j].key >> shift) & mask];
+  __syncthreads();
+#pragma unroll
   for (int j = 0; j < ITEMS; ++j)
-    if (mine + j * 64 < N)
-      sorted[cnt[wave][(p[j].key >> shift) & mask] + rank[j]] = __builtin_bit_cast(uint64_t, p[j]);
+    if (mine + j * 64 < N) u.sorted[rank[j]] = __builtin_bit_cast(uint64_t, p[j]);
   __syncthreads();
   const uint32_t held = (uint32_t)(N - base < TILE ? N - base : TILE);
 #pragma unroll
   for (int j = 0; j < ITEMS; ++j) {
     const uint32_t i = tid + j * kSortThreads;
     if (i < held) {
-      const Pair q = __builtin_bit_cast(Pair, sorted[i]);
+      const Pair q = __builtin_bit_cast(Pair, u.sorted[i]);
       dst((int64_t)(delta[(q.key >> shift) & mask] + i), q);
     }
   }
 }
 
-// Short lists are sorted in one launch: the place of a pair is the number of pairs below it, counted against all of them.
-// A workgroup holds every pair in LDS as (key << 14) | index, so that they all differ; a wave takes kRankItems pairs at a
-// time, and each comparison of one with 64 others is one v_cmp, whose lanes the scalar unit counts. 16384 ids: 2.7e8
-// comparisons, 16 k vector cycles a SIMD. Workgroups beyond the first `blocks` write the gradient's zeros meanwhile.
+// Short lists are sorted in one launch: the place of a pair is the number of pairs below it. Every workgroup places
+// kRankTile pairs and holds all of them in LDS, as (key << 14) | index, so that they all differ. It deals them into bins by
+// the leading bits of the key (LDS atomics: the order inside a bin does not matter, only its members do); a pair's place is
+// then the bin's start and the count of the bin's members below it. A wave compares one pair with 64 others in one v_cmp,
+// whose lanes the scalar unit counts. Counting against all pairs instead of a bin's: 18 us for 10007 ids, 8 with bins.
+// Workgroups beyond the first `blocks` write the gradient's zeros meanwhile.
 constexpr int kIndexBits = 14;
 constexpr int64_t kRankMax = 1 << kIndexBits;
-constexpr int kRankThreads = 1024, kRankItems = 4, kRankTile = kRankThreads / 64 * kRankItems;
+constexpr int kRankThreads = 1024, kRankWaves = kRankThreads / 64, kRankItems = 4, kRankTile = kRankWaves * kRankItems;
+constexpr int kRankBinBits = 11, kRankBins = 1 << kRankBinBits;
 
+// LDS: all pairs by bin
 template <typename IT, typename P>
-__global__ __launch_bounds__(kRankThreads) void rank_sort_kernel(KeyFromIds<IT> src, int N, int blocks, Pair* out,
-                                                                 Fill z) {
+__global__ __launch_bounds__(kRankThreads) void rank_sort_kernel(KeyFromIds<IT> src, int N, int blocks, int bin_shift,
+                                                                 Pair* out, Fill z) {
   if ((int)blockIdx.x >= blocks) {
     fill_zeros(z, (int64_t)(blockIdx.x - blocks) * kRankThreads + threadIdx.x,
                (int64_t)(gridDim.x - blocks) * kRankThreads);
     return;
   }
   extern __shared__ __attribute__((aligned(16))) char rank_lds[];
-  P* pairs = (P*)rank_lds;
-  const int padded = (N + 255) / 256 * 256;
-  for (int i = threadIdx.x; i < padded; i += kRankThreads)
-    pairs[i] = i < N ? ((P)src.at(i).key << kIndexBits) | (P)i : ~(P)0;  // no pair is below another than these
+  P* binned = (P*)rank_lds;
+  // a bin is dealt out in COPIES parts, by lane: word frequencies fill some bins with a third of the ids, and atomics on
+  // one address wait for one another
+  constexpr int COPIES = sizeof(P) == 4 ? 8 : 2, PER = kRankBins * COPIES / kRankThreads;
+  __shared__ uint32_t start[kRankBins + 1], next[kRankBins * COPIES];
+  __shared__ uint32_t part[kRankWaves];
+  const int tid = threadIdx.x, lane = tid & 63, copy = lane % COPIES;
+  constexpr int R = (int)(kRankMax / kRankThreads);
+  for (int k = tid; k < kRankBins * COPIES; k += kRankThreads) next[k] = 0;
   __syncthreads();
-  const int lane = threadIdx.x & 63;
-  const int first = blockIdx.x * kRankTile + (threadIdx.x >> 6) * kRankItems;
-  P item[kRankItems];
-  int rank[kRankItems];
+  uint32_t key[R];
+#pragma unroll
+  for (int j = 0; j < R; ++j) key[j] = tid + j * kRankThreads < N ? src.at(tid + j * kRankThreads).key : 0u;
+#pragma unroll
+  for (int j = 0; j < R; ++j)
+    if (tid + j * kRankThreads < N) atomicAdd(&next[(key[j] >> bin_shift) * COPIES + copy], 1u);
+  __syncthreads();
+  uint32_t c[PER], sum = 0, all;
+#pragma unroll
+  for (int k = 0; k < PER; ++k) {
+    c[k] = next[tid * PER + k];
+    sum += c[k];
+  }
+  uint32_t at = block_exclusive_scan<kRankWaves>(sum, part, all);
+#pragma unroll
+  for (int k = 0; k < PER; ++k) {
+    next[tid * PER + k] = at;
+    if ((tid * PER + k) % COPIES == 0) start[(tid * PER + k) / COPIES] = at;
+    at += c[k];
+  }
+  if (tid == kRankThreads - 1) start[kRankBins] = at;
+  __syncthreads();
+#pragma unroll
+  for (int j = 0; j < R; ++j) {
+    const int i = tid + j * kRankThreads;
+    if (i < N) binned[atomicAdd(&next[(key[j] >> bin_shift) * COPIES + copy], 1u)] = ((P)key[j] << kIndexBits) | (P)i;
+  }
+  __syncthreads();
+  const int first = blockIdx.x * kRankTile + (tid >> 6) * kRankItems;
 #pragma unroll
   for (int t = 0; t < kRankItems; ++t) {
-    const P p = pairs[first + t < padded ? first + t : 0];
-    if constexpr (sizeof(P) == 4) {
-      item[t] = __builtin_amdgcn_readfirstlane(p);
-    } else {
-      item[t] = ((P)(uint32_t)__builtin_amdgcn_readfirstlane((uint32_t)(p >> 32)) << 32) |
-                (uint32_t)__builtin_amdgcn_readfirstlane((uint32_t)p);
+    if (first + t >= N) return;
+    const uint32_t k = __builtin_amdgcn_readfirstlane(src.at(first + t).key);
+    const P item = ((P)k << kIndexBits) | (P)(first + t);
+    const uint32_t begin = __builtin_amdgcn_readfirstlane(start[k >> bin_shift]);
+    const uint32_t end = __builtin_amdgcn_readfirstlane(start[(k >> bin_shift) + 1]);
+    uint32_t rank = begin;
+    for (uint32_t i = begin; i < end; i += 256) {
+      P other[4];
+#pragma unroll
+      for (int u = 0; u < 4; ++u) other[u] = i + u * 64 + lane < end ? binned[i + u * 64 + lane] : ~(P)0;
+#pragma unroll
+      for (int u = 0; u < 4; ++u) rank += __popcll(__ballot(other[u] < item));
     }
-    rank[t] = 0;
-  }
-  for (int i = lane; i < padded; i += 256) {
-    P other[4];
-#pragma unroll
-    for (int u = 0; u < 4; ++u) other[u] = pairs[i + u * 64];
-#pragma unroll
-    for (int u = 0; u < 4; ++u)
-#pragma unroll
-      for (int t = 0; t < kRankItems; ++t) rank[t] += __popcll(__ballot(other[u] < item[t]));
-  }
-#pragma unroll
-  for (int t = 0; t < kRankItems; ++t) {
-    if (lane == t && first + t < N) store_pair(out + rank[t], {(uint32_t)(item[t] >> kIndexBits), (uint32_t)(first + t)});
+    if (lane == 0) store_pair(out + rank, {k, (uint32_t)(first + t)});
   }
 }
 
@@ -1013,7 +1059,7 @@ __global__ __launch_bounds__(kRunThreads) void run_join_kernel(const Pair* pairs
 // ---- long id lists of short rows (up to 16 bytes of g): gathering such rows one by one would fetch a cache line for each.
 // One partition by ranges of table rows carries the rows of g along, dropout applied; then a workgroup streams a tile of a
 // bucket, each wave into its own LDS table of the bucket's rows. Lanes of a wave that hold the same row add one after the
-// other in the order of the lanes, so that the sums' order is the ids' alone. A bucket of more than one tile leaves its
+// other in the order of the lanes, so that the ids alone fix the sums' order. A bucket of more than one tile leaves its
 // tiles' tables to a second launch. Every row of a bucket is written, so the gradient needs no zeros beforehand.
 constexpr int kBucketThreads = 512, kBucketWaves = kBucketThreads / 64;
 constexpr int64_t kBucketTile = 8192;    // positions a workgroup
@@ -1110,29 +1156,29 @@ __global__ __launch_bounds__(kBucketThreads) void bucket_sum_kernel(const uint32
   const BucketTile t = me;
   if (t.bucket == 0xffffffffu) return;  // fewer tiles than the most there can be
   if (t.tile == 0 && tid == 0) multi[t.bucket] = t;
-  // the wave's consecutive positions, 64 at a time
-  constexpr int kPer = (int)(kBucketTile / kBucketWaves);
-  const uint32_t begin = t.tile * (uint32_t)kBucketTile + wave * kPer;
-  const uint32_t end = begin + kPer < t.count ? begin + kPer : t.count;
+  // a wave's step takes 8 consecutive positions from each of 8 places of its part: neighbours often name the same row, and
+  // lanes with the same row wait for one another, while 8 positions still make a whole sector to load
+  constexpr int kPart = (int)(kBucketTile / kBucketWaves), kPlace = kPart / 8, U = 4;
+  const uint32_t begin = t.tile * (uint32_t)kBucketTile + wave * kPart;
   float* mine = table + wave * floats;
-  constexpr int U = 4;
-  for (uint32_t i0 = begin; i0 < end; i0 += 64 * U) {
+  for (int s0 = 0; s0 < kPlace / 8 && begin < t.count; s0 += U) {
     uint32_t slot[U];
+    bool valid[U];
     Row<GT, DM> r[U];
 #pragma unroll
     for (int u = 0; u < U; ++u) {
-      const uint32_t i = i0 + u * 64 + lane;
+      const uint32_t i = begin + (lane >> 3) * kPlace + (s0 + u) * 8 + (lane & 7);
+      valid[u] = i < t.count;
       slot[u] = 0;
-      if (i < end) {
+      if (valid[u]) {
         slot[u] = keys[t.first + i] & ((1u << b.lrows) - 1);
         r[u] = rows[t.first + i];
       }
     }
 #pragma unroll
     for (int u = 0; u < U; ++u) {
-      const bool valid = i0 + u * 64 + lane < end;
-      const uint64_t peers = wave_match<11>(slot[u], valid);
-      int turn = valid ? __popcll(peers & ((1ull << lane) - 1)) : -1;
+      const uint64_t peers = wave_match<11>(slot[u], valid[u]);
+      const int turn = valid[u] ? __popcll(peers & ((1ull << lane) - 1)) : -1;
       for (int now = 0; __ballot(turn >= now); ++now) {
         if (turn == now) {
           volatile float* a = mine + slot[u] * DM;
@@ -1254,7 +1300,8 @@ inline void sort_pass(Src src, int64_t N, int pass, const SortPlan& s, char* ws,
     constexpr int BINS = decltype(bins)::value, ITEMS = decltype(items)::value;
     hipLaunchKernelGGL((sort_count_kernel<Src, BINS, ITEMS>), dim3((unsigned)(s.tiles + fill)), dim3(kSortThreads), 0, st,
                        src, N, shift, s.width, counts, s.tiles, z);
-    if (totals) hipLaunchKernelGGL(sort_scan_kernel, dim3(1u << s.width), dim3(256), 0, st, counts, s.tiles, totals);
+    if (totals) hipLaunchKernelGGL(sort_scan_kernel, dim3(BINS / kScanDigits), dim3(kScanThreads), 0, st, counts, s.tiles,
+                                   BINS, totals);
     hipLaunchKernelGGL((sort_scatter_kernel<Src, StorePairs, BINS, ITEMS>), dim3((unsigned)s.tiles), dim3(kSortThreads), 0,
                        st, src, N, shift, s.width, counts, s.tiles, totals, StorePairs{(Pair*)(ws + w.pairs[pass & 1])});
   };
@@ -1277,9 +1324,10 @@ inline int sort_ids(const IT* ids, int64_t N, int64_t V, int64_t pad, char* ws, 
     fill = fill < 1 ? 1 : fill > 1024 ? 1024 : fill;
     const bool narrow = V < (1ll << (32 - kIndexBits));  // keys 0 .. V beside the index in 32 bits
     auto* k = narrow ? rank_sort_kernel<IT, uint32_t> : rank_sort_kernel<IT, uint64_t>;
-    hipLaunchKernelGGL(k, dim3((unsigned)(blocks + fill)), dim3(kRankThreads),
-                       (unsigned)((N + 255) / 256 * 256 * (narrow ? 4 : 8)), st, src, (int)N, blocks,
-                       (Pair*)(ws + w.pairs[0]), z);
+    int bin_shift = 0;
+    while ((V >> bin_shift) >= kRankBins) ++bin_shift;
+    hipLaunchKernelGGL(k, dim3((unsigned)(blocks + fill)), dim3(kRankThreads), (unsigned)(N * (narrow ? 4 : 8)), st, src,
+                       (int)N, blocks, bin_shift, (Pair*)(ws + w.pairs[0]), z);
     return 0;
   }
   for (int pass = 0; pass < s.passes; ++pass) {
@@ -1300,7 +1348,7 @@ inline void bucket_gradient(const GT* g, const IT* ids, int64_t N, int64_t V, in
   const KeyFromIds<IT> src{ids, V, pad, (uint32_t)(b.buckets << b.lrows)};
   hipLaunchKernelGGL((sort_count_kernel<KeyFromIds<IT>, 1024, kBucketItems>), dim3((unsigned)tiles), dim3(kSortThreads), 0,
                      st, src, N, b.lrows, 10, counts, tiles, Fill{nullptr, 0, 0});
-  hipLaunchKernelGGL(sort_scan_kernel, dim3(1024), dim3(256), 0, st, counts, tiles, totals);
+  hipLaunchKernelGGL(sort_scan_kernel, dim3(1024 / kScanDigits), dim3(kScanThreads), 0, st, counts, tiles, 1024, totals);
   const StoreRows<E, DM> dst{(const E*)g, (int)D, m, keys, (Row<E, DM>*)(ws + w.rows)};
   hipLaunchKernelGGL((sort_scatter_kernel<KeyFromIds<IT>, StoreRows<E, DM>, 1024, kBucketItems>), dim3((unsigned)tiles),
                      dim3(kSortThreads), 0, st, src, N, b.lrows, 10, counts, tiles, totals, dst);
