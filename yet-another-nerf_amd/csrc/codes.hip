@@ -329,25 +329,6 @@ struct KeyFromPairs {
 };
 __device__ __forceinline__ void store_pair(Pair* to, Pair p) { *(uint64_t*)to = __builtin_bit_cast(uint64_t, p); }
 
-// the gradient's zeros, written beside the sort's first launch: rows that no id names keep them
-struct Fill {
-  char* p;
-  int64_t bytes;
-  int wide;  // p is 16-byte aligned
-};
-__device__ __forceinline__ void fill_zeros(const Fill& z, int64_t worker, int64_t workers) {
-  typedef uint32_t v4 __attribute__((ext_vector_type(4)));
-  int64_t done = 0;
-  if (z.wide) {
-    for (int64_t i = worker; i < z.bytes / 16; i += workers) ((v4*)z.p)[i] = v4{0, 0, 0, 0};
-    done = z.bytes / 16 * 16;
-  }
-  for (int64_t i = done / 2 + worker; i < z.bytes / 2; i += workers) ((uint16_t*)z.p)[i] = 0;
-}
-__global__ __launch_bounds__(256) void fill_kernel(Fill z) {
-  fill_zeros(z, (int64_t)blockIdx.x * 256 + threadIdx.x, (int64_t)gridDim.x * 256);
-}
-
 // Long lists: least-significant-digit radix sort, digits of up to 10 bits. A pass counts the digits of each tile, scans each
 // digit's counts over the tiles, and scatters: a wave ranks equal digits by ballots, so that equal keys keep their order,
 // and a tile's pairs are first put in order in LDS, so that they leave as runs and not one by one. With no more than
@@ -374,11 +355,7 @@ inline SortPlan sort_plan(int64_t N, int64_t V) {
 
 template <typename Src, int BINS, int ITEMS>
 __global__ __launch_bounds__(kSortThreads) void sort_count_kernel(Src src, int64_t N, int shift, int width,
-                                                                  uint32_t* counts, int64_t tiles, Fill z) {
-  if (blockIdx.x >= tiles) {
-    fill_zeros(z, (blockIdx.x - tiles) * kSortThreads + threadIdx.x, (int64_t)(gridDim.x - tiles) * kSortThreads);
-    return;
-  }
+                                                                  uint32_t* counts) {
   // neighbouring ids often share a digit: copies of the counts, by lane, keep them from waiting for one another
   constexpr int COPIES = 8;
   __shared__ uint32_t hist[BINS * COPIES];
@@ -574,30 +551,28 @@ __global__ __launch_bounds__(kSortThreads) void sort_scatter_kernel(Src src, int
 }
 
 // Short lists are sorted in one launch: the place of a pair is the number of pairs below it. Every workgroup places
-// kRankTile pairs and holds all of them in LDS, as (key << 14) | index, so that they all differ. It deals them into bins by
-// the leading bits of the key (LDS atomics: the order inside a bin does not matter, only its members do); a pair's place is
-// then the bin's start and the count of the bin's members below it. A wave compares one pair with 64 others in one v_cmp,
-// whose lanes the scalar unit counts. Counting against all pairs instead of a bin's: 18 us for 10007 ids, 8 with bins.
-// Workgroups beyond the first `blocks` write the gradient's zeros meanwhile.
+// kRankTile pairs and holds all of them in LDS, as (key << 14) | index, so that they all differ. It deals them into bins
+// (LDS atomics: the order inside a bin does not matter, only its members do); a pair's place is then the bin's start and the
+// count of the bin's members below it. A wave compares one pair with 64 others in one v_cmp, whose lanes the scalar unit
+// counts. Bins are as wide as 1/64 of their keys: word frequencies, which fall with the id, would put a third of the ids
+// into the first of 2048 equal bins (38 us for 16384 ids; counting against all pairs 37).
 constexpr int kIndexBits = 14;
 constexpr int64_t kRankMax = 1 << kIndexBits;
 constexpr int kRankThreads = 1024, kRankWaves = kRankThreads / 64, kRankItems = 4, kRankTile = kRankWaves * kRankItems;
-constexpr int kRankBinBits = 11, kRankBins = 1 << kRankBinBits;
+constexpr int kRankBins = 2048;
+__device__ __forceinline__ uint32_t rank_bin(uint32_t key) {  // at most 1727, rising with the key
+  const int e = key < 64 ? 0 : 25 - __builtin_clz(key);
+  return (e << 6) + (key >> e);
+}
 
 // LDS: all pairs by bin
 template <typename IT, typename P>
-__global__ __launch_bounds__(kRankThreads) void rank_sort_kernel(KeyFromIds<IT> src, int N, int blocks, int bin_shift,
-                                                                 Pair* out, Fill z) {
-  if ((int)blockIdx.x >= blocks) {
-    fill_zeros(z, (int64_t)(blockIdx.x - blocks) * kRankThreads + threadIdx.x,
-               (int64_t)(gridDim.x - blocks) * kRankThreads);
-    return;
-  }
+__global__ __launch_bounds__(kRankThreads) void rank_sort_kernel(KeyFromIds<IT> src, int N, Pair* out) {
   extern __shared__ __attribute__((aligned(16))) char rank_lds[];
   P* binned = (P*)rank_lds;
   // a bin is dealt out in COPIES parts, by lane: word frequencies fill some bins with a third of the ids, and atomics on
   // one address wait for one another
-  constexpr int COPIES = sizeof(P) == 4 ? 8 : 2, PER = kRankBins * COPIES / kRankThreads;
+  constexpr int COPIES = sizeof(P) == 4 ? 4 : 2, PER = kRankBins * COPIES / kRankThreads;
   __shared__ uint32_t start[kRankBins + 1], next[kRankBins * COPIES];
   __shared__ uint32_t part[kRankWaves];
   const int tid = threadIdx.x, lane = tid & 63, copy = lane % COPIES;
@@ -609,7 +584,7 @@ __global__ __launch_bounds__(kRankThreads) void rank_sort_kernel(KeyFromIds<IT> 
   for (int j = 0; j < R; ++j) key[j] = tid + j * kRankThreads < N ? src.at(tid + j * kRankThreads).key : 0u;
 #pragma unroll
   for (int j = 0; j < R; ++j)
-    if (tid + j * kRankThreads < N) atomicAdd(&next[(key[j] >> bin_shift) * COPIES + copy], 1u);
+    if (tid + j * kRankThreads < N) atomicAdd(&next[rank_bin(key[j]) * COPIES + copy], 1u);
   __syncthreads();
   uint32_t c[PER], sum = 0, all;
 #pragma unroll
@@ -629,24 +604,27 @@ __global__ __launch_bounds__(kRankThreads) void rank_sort_kernel(KeyFromIds<IT> 
 #pragma unroll
   for (int j = 0; j < R; ++j) {
     const int i = tid + j * kRankThreads;
-    if (i < N) binned[atomicAdd(&next[(key[j] >> bin_shift) * COPIES + copy], 1u)] = ((P)key[j] << kIndexBits) | (P)i;
+    if (i < N) binned[atomicAdd(&next[rank_bin(key[j]) * COPIES + copy], 1u)] = ((P)key[j] << kIndexBits) | (P)i;
   }
   __syncthreads();
   const int first = blockIdx.x * kRankTile + (tid >> 6) * kRankItems;
+  uint32_t item[kRankItems];
+#pragma unroll
+  for (int t = 0; t < kRankItems; ++t) item[t] = src.at(first + t < N ? first + t : N - 1).key;
 #pragma unroll
   for (int t = 0; t < kRankItems; ++t) {
     if (first + t >= N) return;
-    const uint32_t k = __builtin_amdgcn_readfirstlane(src.at(first + t).key);
-    const P item = ((P)k << kIndexBits) | (P)(first + t);
-    const uint32_t begin = __builtin_amdgcn_readfirstlane(start[k >> bin_shift]);
-    const uint32_t end = __builtin_amdgcn_readfirstlane(start[(k >> bin_shift) + 1]);
+    const uint32_t k = __builtin_amdgcn_readfirstlane(item[t]);
+    const P mine = ((P)k << kIndexBits) | (P)(first + t);
+    const uint32_t begin = __builtin_amdgcn_readfirstlane(start[rank_bin(k)]);
+    const uint32_t end = __builtin_amdgcn_readfirstlane(start[rank_bin(k) + 1]);
     uint32_t rank = begin;
     for (uint32_t i = begin; i < end; i += 256) {
       P other[4];
 #pragma unroll
       for (int u = 0; u < 4; ++u) other[u] = i + u * 64 + lane < end ? binned[i + u * 64 + lane] : ~(P)0;
 #pragma unroll
-      for (int u = 0; u < 4; ++u) rank += __popcll(__ballot(other[u] < item));
+      for (int u = 0; u < 4; ++u) rank += __popcll(__ballot(other[u] < mine));
     }
     if (lane == 0) store_pair(out + rank, {k, (uint32_t)(first + t)});
   }
@@ -985,12 +963,46 @@ struct StagedPairs {
   __device__ __forceinline__ int64_t row(uint32_t key) const { return key; }
 };
 
+// first position of [lo, hi) whose key is not below v
+__device__ __forceinline__ int64_t lower_bound(const Pair* pairs, int64_t lo, int64_t hi, uint32_t v) {
+  while (lo < hi) {
+    const int64_t mid = (lo + hi) >> 1;
+    if (pairs[mid].key < v) lo = mid + 1;
+    else hi = mid;
+  }
+  return lo;
+}
+
+__global__ __launch_bounds__(256) void zeros_kernel(uint16_t* p, int64_t n) {
+  for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < n; i += (int64_t)gridDim.x * 256) p[i] = 0;
+}
+
+// Workgroups beyond the first r.blocks * r.chunks write zeros to the rows that no pair names, `rows` consecutive ones each
+// (clearing the whole gradient beforehand writes the named rows twice, and could not share the chip with the sums).
+constexpr int kAbsentRows = 1024;
+
 template <typename GT, typename TT, int VEC>
 __global__ __launch_bounds__(kRunThreads) void run_sum_kernel(const GT* g, const Pair* pairs, uint32_t V, int64_t N,
                                                               int64_t D, RunPlan r, Mask m, float f, TT* grad,
-                                                              float* heads, float* tails) {
+                                                              float* heads, float* tails, int rows, Div dv) {
   __shared__ RunEnds<kRunThreads, VEC> ends;
   __shared__ uint64_t staged[(kRunSpan + 16) / 8 * 9];
+  const uint32_t sums = (uint32_t)(r.blocks * r.chunks);
+  if (blockIdx.x >= sums) {
+    uint8_t* named = (uint8_t*)staged;
+    const int64_t row0 = (int64_t)(blockIdx.x - sums) * rows;
+    const int here = (int)(V - row0 < rows ? V - row0 : rows);
+    for (int k = threadIdx.x; k < here; k += kRunThreads) {
+      const uint32_t row = (uint32_t)(row0 + k);
+      const int64_t at = lower_bound(pairs, 0, N, row);
+      named[k] = at < N && pairs[at].key == row;
+    }
+    __syncthreads();
+    const float zero[VEC] = {};
+    for (uint32_t t = threadIdx.x; t < (uint32_t)here * dv.d; t += kRunThreads)
+      if (!named[div_by(t, dv)]) store_vec<TT, VEC, (VEC > 1), false>(grad + row0 * D + (int64_t)t * VEC, zero);
+    return;
+  }
   const int64_t block = blockIdx.x % (uint32_t)r.blocks, chunk = blockIdx.x / (uint32_t)r.blocks;
   const int64_t d = ((chunk << r.lg) + (threadIdx.x & ((1 << r.lg) - 1))) * VEC;
   const int64_t base = block * r.span;
@@ -1002,16 +1014,6 @@ __global__ __launch_bounds__(kRunThreads) void run_sum_kernel(const GT* g, const
   __syncthreads();
   sum_runs<kRunThreads, GT, TT, VEC>(ends, StagedPairs{staged, base, V}, N, base, r.piece, r.lg, g, D, d, m,
                                      mask_offset(m), f, grad, heads + block * D, tails + block * D);
-}
-
-// first position of [lo, hi) whose key is not below v
-__device__ __forceinline__ int64_t lower_bound(const Pair* pairs, int64_t lo, int64_t hi, uint32_t v) {
-  while (lo < hi) {
-    const int64_t mid = (lo + hi) >> 1;
-    if (pairs[mid].key < v) lo = mid + 1;
-    else hi = mid;
-  }
-  return lo;
 }
 
 // the run that workgroup b of run_sum_kernel started and did not end: its tail and the heads of the workgroups after it
@@ -1289,17 +1291,14 @@ inline BucketWs bucket_ws(int64_t N, const BucketPlan& b, int64_t g_bytes) {
 }
 
 template <typename Src>
-inline void sort_pass(Src src, int64_t N, int pass, const SortPlan& s, char* ws, const GradWs& w, const Fill& z,
-                      hipStream_t st) {
+inline void sort_pass(Src src, int64_t N, int pass, const SortPlan& s, char* ws, const GradWs& w, hipStream_t st) {
   uint32_t* counts = (uint32_t*)(ws + w.counts);
   uint32_t* totals = s.tiles <= kFewTiles ? nullptr : (uint32_t*)(ws + w.totals);
   const int shift = pass * s.width;
-  int64_t fill = z.bytes / (kSortThreads * 16 * 4);
-  fill = z.bytes == 0 ? 0 : fill < 1 ? 1 : fill > 2048 ? 2048 : fill;
   auto go = [&](auto bins, auto items) {
     constexpr int BINS = decltype(bins)::value, ITEMS = decltype(items)::value;
-    hipLaunchKernelGGL((sort_count_kernel<Src, BINS, ITEMS>), dim3((unsigned)(s.tiles + fill)), dim3(kSortThreads), 0, st,
-                       src, N, shift, s.width, counts, s.tiles, z);
+    hipLaunchKernelGGL((sort_count_kernel<Src, BINS, ITEMS>), dim3((unsigned)s.tiles), dim3(kSortThreads), 0, st, src, N,
+                       shift, s.width, counts);
     if (totals) hipLaunchKernelGGL(sort_scan_kernel, dim3(BINS / kScanDigits), dim3(kScanThreads), 0, st, counts, s.tiles,
                                    BINS, totals);
     hipLaunchKernelGGL((sort_scatter_kernel<Src, StorePairs, BINS, ITEMS>), dim3((unsigned)s.tiles), dim3(kSortThreads), 0,
@@ -1312,28 +1311,22 @@ inline void sort_pass(Src src, int64_t N, int pass, const SortPlan& s, char* ws,
   else go(integral_constant<int, 1024>{}, integral_constant<int, 16>{});
 }
 
-// sorts the ids and clears the gradient; returns which of the two buffers holds the pairs
+// sorts the ids; returns which of the two buffers holds the pairs
 template <typename IT>
-inline int sort_ids(const IT* ids, int64_t N, int64_t V, int64_t pad, char* ws, const GradWs& w, const Fill& z,
-                    hipStream_t st) {
+inline int sort_ids(const IT* ids, int64_t N, int64_t V, int64_t pad, char* ws, const GradWs& w, hipStream_t st) {
   const SortPlan s = sort_plan(N, V);
   const KeyFromIds<IT> src{ids, V, pad, (uint32_t)V};
   if (N <= kRankMax) {
-    const int blocks = (int)((N + kRankTile - 1) / kRankTile);
-    int64_t fill = z.bytes / (kRankThreads * 16 * 2);
-    fill = fill < 1 ? 1 : fill > 1024 ? 1024 : fill;
     const bool narrow = V < (1ll << (32 - kIndexBits));  // keys 0 .. V beside the index in 32 bits
     auto* k = narrow ? rank_sort_kernel<IT, uint32_t> : rank_sort_kernel<IT, uint64_t>;
-    int bin_shift = 0;
-    while ((V >> bin_shift) >= kRankBins) ++bin_shift;
-    hipLaunchKernelGGL(k, dim3((unsigned)(blocks + fill)), dim3(kRankThreads), (unsigned)(N * (narrow ? 4 : 8)), st, src,
-                       (int)N, blocks, bin_shift, (Pair*)(ws + w.pairs[0]), z);
+    hipLaunchKernelGGL(k, dim3((unsigned)((N + kRankTile - 1) / kRankTile)), dim3(kRankThreads),
+                       (unsigned)(N * (narrow ? 4 : 8)), st, src, (int)N, (Pair*)(ws + w.pairs[0]));
     return 0;
   }
   for (int pass = 0; pass < s.passes; ++pass) {
     const int from = (pass - 1) & 1;
-    if (pass == 0) sort_pass(src, N, pass, s, ws, w, z, st);
-    else sort_pass(KeyFromPairs{(const Pair*)(ws + w.pairs[from])}, N, pass, s, ws, w, Fill{nullptr, 0, 0}, st);
+    if (pass == 0) sort_pass(src, N, pass, s, ws, w, st);
+    else sort_pass(KeyFromPairs{(const Pair*)(ws + w.pairs[from])}, N, pass, s, ws, w, st);
   }
   return (s.passes - 1) & 1;
 }
@@ -1347,7 +1340,7 @@ inline void bucket_gradient(const GT* g, const IT* ids, int64_t N, int64_t V, in
   const int64_t tiles = partition_tiles(N);
   const KeyFromIds<IT> src{ids, V, pad, (uint32_t)(b.buckets << b.lrows)};
   hipLaunchKernelGGL((sort_count_kernel<KeyFromIds<IT>, 1024, kBucketItems>), dim3((unsigned)tiles), dim3(kSortThreads), 0,
-                     st, src, N, b.lrows, 10, counts, tiles, Fill{nullptr, 0, 0});
+                     st, src, N, b.lrows, 10, counts);
   hipLaunchKernelGGL(sort_scan_kernel, dim3(1024 / kScanDigits), dim3(kScanThreads), 0, st, counts, tiles, 1024, totals);
   const StoreRows<E, DM> dst{(const E*)g, (int)D, m, keys, (Row<E, DM>*)(ws + w.rows)};
   hipLaunchKernelGGL((sort_scatter_kernel<KeyFromIds<IT>, StoreRows<E, DM>, 1024, kBucketItems>), dim3((unsigned)tiles),
@@ -1499,9 +1492,9 @@ int yanerf_embedding_backward(const void* g, int g_type, const void* ids, int id
   const float f = (float)(scale * mask_scale(p, m));
   hipStream_t st = as_stream(stream);
   char* ws = (char*)workspace;
-  const Fill z{(char*)grad_table, V * D * type_bytes(table_type), aligned(grad_table, 16)};
   if (N == 0) {
-    hipLaunchKernelGGL(fill_kernel, grid_for((z.bytes + 4095) / 4096), dim3(256), 0, st, z);
+    const int64_t halves = V * D * type_bytes(table_type) / 2;
+    hipLaunchKernelGGL(zeros_kernel, grid_for((halves + 2047) / 2048), dim3(256), 0, st, (uint16_t*)grad_table, halves);
     YN_LAUNCH_CHECK("embedding_backward");
     return 0;
   }
@@ -1539,14 +1532,16 @@ int yanerf_embedding_backward(const void* g, int g_type, const void* ids, int id
     const GradWs w = grad_ws(N, V, D);
     const RunPlan r = run_plan(N, D, VEC);
     int at = 0;
-    with_index(id_bytes, [&](auto it) { at = sort_ids((const decltype(it)*)ids, N, V, padding_idx, ws, w, z, st); });
+    with_index(id_bytes, [&](auto it) { at = sort_ids((const decltype(it)*)ids, N, V, padding_idx, ws, w, st); });
     const Pair* pairs = (const Pair*)(ws + w.pairs[at]);
     float *heads = (float*)(ws + w.heads), *tails = (float*)(ws + w.tails);
-    const dim3 grid((unsigned)(r.blocks * r.chunks));
-    hipLaunchKernelGGL((run_sum_kernel<GT, TT, VEC>), grid, dim3(kRunThreads), 0, st, (const GT*)g, pairs, (uint32_t)V, N, D, r,
-                       m, f, (TT*)grad_table, heads, tails);
+    int64_t rows = 65536 / (D * tb) < V / 512 ? 65536 / (D * tb) : V / 512;  // 64 KB of zeros, or two workgroups a CU
+    rows = rows < 1 ? 1 : rows > kAbsentRows ? kAbsentRows : rows;
+    const unsigned sums = (unsigned)(r.blocks * r.chunks), zeros = (unsigned)((V + rows - 1) / rows);
+    hipLaunchKernelGGL((run_sum_kernel<GT, TT, VEC>), dim3(sums + zeros), dim3(kRunThreads), 0, st, (const GT*)g, pairs,
+                       (uint32_t)V, N, D, r, m, f, (TT*)grad_table, heads, tails, (int)rows, make_div(D / VEC));
     if (r.blocks > 1)
-      hipLaunchKernelGGL((run_join_kernel<TT, VEC>), grid, dim3(kRunThreads), 0, st, pairs, N, (uint32_t)V, D, r, f,
+      hipLaunchKernelGGL((run_join_kernel<TT, VEC>), dim3(sums), dim3(kRunThreads), 0, st, pairs, N, (uint32_t)V, D, r, f,
                          (TT*)grad_table, heads, tails);
   };
   with_type(g_type, [&](auto gt) {
