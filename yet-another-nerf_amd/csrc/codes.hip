@@ -333,11 +333,14 @@ __device__ __forceinline__ void store_pair(Pair* to, Pair p) { *(uint64_t*)to = 
 // digit's counts over the tiles, and scatters: a wave ranks equal digits by ballots, so that equal keys keep their order,
 // and a tile's pairs are first put in order in LDS, so that they leave as runs and not one by one. With no more than
 // kFewTiles tiles the scatter reads the counts of all of them itself and the scan's launch is left out.
-constexpr int kSortThreads = 256, kSortWaves = kSortThreads / 64;
 constexpr int64_t kFewTiles = 64;
+// lanes and pairs a lane: small tiles while they are few, else 4096 by 8 waves (6.3 M pairs, 1024 bins: 512 x 8 52 us,
+// 256 x 16 55, 1024 x 8 61, 512 x 16 71, 1024 x 16 109)
+constexpr int kFewThreads = 256, kFewItems = 8, kTileThreads = 512, kTileItems = 8;
 
 struct SortPlan {
-  int passes, width, bins, items;
+  int passes, width, bins;
+  bool few;
   int64_t tiles;
 };
 
@@ -348,29 +351,29 @@ inline SortPlan sort_plan(int64_t N, int64_t V) {
   s.passes = (bits + 9) / 10;
   s.width = (bits + s.passes - 1) / s.passes;
   s.bins = s.width <= 8 ? 256 : 1024;
-  s.items = N <= kFewTiles * kSortThreads * 8 ? 8 : 16;
-  s.tiles = (N + kSortThreads * s.items - 1) / (kSortThreads * s.items);
+  s.few = N <= kFewTiles * kFewThreads * kFewItems;
+  const int64_t tile = s.few ? kFewThreads * kFewItems : kTileThreads * kTileItems;
+  s.tiles = (N + tile - 1) / tile;
   return s;
 }
 
-template <typename Src, int BINS, int ITEMS>
-__global__ __launch_bounds__(kSortThreads) void sort_count_kernel(Src src, int64_t N, int shift, int width,
-                                                                  uint32_t* counts) {
+template <typename Src, int BINS, int THREADS, int ITEMS>
+__global__ __launch_bounds__(THREADS) void sort_count_kernel(Src src, int64_t N, int shift, int width, uint32_t* counts) {
   // neighbouring ids often share a digit: copies of the counts, by lane, keep them from waiting for one another
-  constexpr int COPIES = 8;
+  constexpr int COPIES = 4;
   __shared__ uint32_t hist[BINS * COPIES];
-  for (int k = threadIdx.x; k < BINS * COPIES; k += kSortThreads) hist[k] = 0;
+  for (int k = threadIdx.x; k < BINS * COPIES; k += THREADS) hist[k] = 0;
   __syncthreads();
   const uint32_t mask = (1u << width) - 1;
-  const int64_t base = (int64_t)blockIdx.x * (kSortThreads * ITEMS) + threadIdx.x;
+  const int64_t base = (int64_t)blockIdx.x * (THREADS * ITEMS) + threadIdx.x;
   uint32_t key[ITEMS];
 #pragma unroll
-  for (int j = 0; j < ITEMS; ++j) key[j] = base + j * kSortThreads < N ? src.at(base + j * kSortThreads).key : 0u;
+  for (int j = 0; j < ITEMS; ++j) key[j] = base + j * THREADS < N ? src.at(base + j * THREADS).key : 0u;
 #pragma unroll
   for (int j = 0; j < ITEMS; ++j)
-    if (base + j * kSortThreads < N) atomicAdd(&hist[((key[j] >> shift) & mask) * COPIES + threadIdx.x % COPIES], 1u);
+    if (base + j * THREADS < N) atomicAdd(&hist[((key[j] >> shift) & mask) * COPIES + threadIdx.x % COPIES], 1u);
   __syncthreads();
-  for (int k = threadIdx.x; k < BINS; k += kSortThreads) {
+  for (int k = threadIdx.x; k < BINS; k += THREADS) {
     uint32_t sum = 0;
 #pragma unroll
     for (int c = 0; c < COPIES; ++c) sum += hist[k * COPIES + c];
@@ -431,6 +434,13 @@ __global__ __launch_bounds__(kScanThreads) void sort_scan_kernel(uint32_t* count
   if (part == 0) totals[blockIdx.x * kScanDigits + dig] = total;
 }
 
+// what the wave's lanes wrote to LDS before is what they read from it after (LDS serves a wave in order; this keeps the
+// compiler to it)
+__device__ __forceinline__ void wave_fence() {
+  __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+  __builtin_amdgcn_wave_barrier();
+}
+
 // lanes of this wave whose digit equals this lane's
 template <int BITS>
 __device__ __forceinline__ uint64_t wave_match(uint32_t digit, bool valid) {
@@ -451,21 +461,21 @@ struct StorePairs {
   __device__ __forceinline__ void operator()(int64_t to, Pair p) const { store_pair(out + to, p); }
 };
 
-template <typename Src, typename Dst, int BINS, int ITEMS>
-__global__ __launch_bounds__(kSortThreads) void sort_scatter_kernel(Src src, int64_t N, int shift, int width,
-                                                                    const uint32_t* counts, int64_t tiles,
-                                                                    const uint32_t* totals, Dst dst) {
-  constexpr int PER = BINS / kSortThreads, TILE = kSortThreads * ITEMS, BITS = BINS == 256 ? 8 : 10;
+template <typename Src, typename Dst, int BINS, int THREADS, int ITEMS>
+__global__ __launch_bounds__(THREADS) void sort_scatter_kernel(Src src, int64_t N, int shift, int width,
+                                                               const uint32_t* counts, int64_t tiles,
+                                                               const uint32_t* totals, Dst dst) {
+  constexpr int WAVES = THREADS / 64, PER = (BINS + THREADS - 1) / THREADS, TILE = THREADS * ITEMS;
+  constexpr int BITS = BINS == 256 ? 8 : 10;
   __shared__ union {
-    uint32_t cnt[kSortWaves][BINS];  // a wave's count of each digit so far, then its first slot
+    uint32_t cnt[WAVES][BINS];  // a wave's count of each digit so far, then its first slot
     uint64_t sorted[TILE];           // the tile in order, once every lane knows its slots
   } u;
-  volatile uint32_t(*cnt)[BINS] = u.cnt;
   __shared__ uint32_t delta[BINS];  // place in the output less place in the tile
-  __shared__ uint32_t part[kSortWaves];
+  __shared__ uint32_t part[WAVES];
   const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63;
   const uint32_t mask = (1u << width) - 1;
-  for (int k = tid; k < kSortWaves * BINS; k += kSortThreads) (&cnt[0][0])[k] = 0;
+  for (int k = tid; k < WAVES * BINS; k += THREADS) (&u.cnt[0][0])[k] = 0;
   const int64_t base = (int64_t)blockIdx.x * TILE;
   const int64_t mine = base + wave * (64 * ITEMS) + lane;
   Pair p[ITEMS];
@@ -494,7 +504,7 @@ __global__ __launch_bounds__(kSortThreads) void sort_scatter_kernel(Src src, int
     place[k] = sum + before;
     sum += total;
   }
-  const uint32_t digit_base = block_exclusive_scan<kSortWaves>(sum, part, all);
+  const uint32_t digit_base = block_exclusive_scan<WAVES>(sum, part, all);
   __syncthreads();
   uint32_t rank[ITEMS];
 #pragma unroll
@@ -503,11 +513,11 @@ __global__ __launch_bounds__(kSortThreads) void sort_scatter_kernel(Src src, int
     const uint32_t dig = (p[j].key >> shift) & mask;
     const uint64_t peers = wave_match<BITS>(dig, valid);
     const uint32_t below = __popcll(peers & ((1ull << lane) - 1));
-    const uint32_t before = cnt[wave][dig];
+    const uint32_t before = u.cnt[wave][dig];
     rank[j] = before + below;
-    __builtin_amdgcn_wave_barrier();
-    if (valid && below == 0) cnt[wave][dig] = before + __popcll(peers);
-    __builtin_amdgcn_wave_barrier();
+    wave_fence();
+    if (valid && below == 0) u.cnt[wave][dig] = before + __popcll(peers);
+    wave_fence();
   }
   __syncthreads();
   sum = 0;
@@ -515,25 +525,28 @@ __global__ __launch_bounds__(kSortThreads) void sort_scatter_kernel(Src src, int
 #pragma unroll
   for (int k = 0; k < PER; ++k) {
     here[k] = sum;
+    if (tid * PER + k < BINS) {
 #pragma unroll
-    for (int w = 0; w < kSortWaves; ++w) sum += cnt[w][tid * PER + k];
+      for (int w = 0; w < WAVES; ++w) sum += u.cnt[w][tid * PER + k];
+    }
   }
-  const uint32_t first = block_exclusive_scan<kSortWaves>(sum, part, all);
+  const uint32_t first = block_exclusive_scan<WAVES>(sum, part, all);
 #pragma unroll
   for (int k = 0; k < PER; ++k) {
     const int dig = tid * PER + k;
+    if (dig >= BINS) break;
     uint32_t at = first + here[k];
     delta[dig] = digit_base + place[k] - at;
 #pragma unroll
-    for (int w = 0; w < kSortWaves; ++w) {
-      const uint32_t c = cnt[w][dig];
-      cnt[w][dig] = at;
+    for (int w = 0; w < WAVES; ++w) {
+      const uint32_t c = u.cnt[w][dig];
+      u.cnt[w][dig] = at;
       at += c;
     }
   }
   __syncthreads();
 #pragma unroll
-  for (int j = 0; j < ITEMS; ++j) rank[j] += cnt[wave][(p[j].key >> shift) & mask];
+  for (int j = 0; j < ITEMS; ++j) rank[j] += u.cnt[wave][(p[j].key >> shift) & mask];
   __syncthreads();
 #pragma unroll
   for (int j = 0; j < ITEMS; ++j)
@@ -542,7 +555,7 @@ __global__ __launch_bounds__(kSortThreads) void sort_scatter_kernel(Src src, int
   const uint32_t held = (uint32_t)(N - base < TILE ? N - base : TILE);
 #pragma unroll
   for (int j = 0; j < ITEMS; ++j) {
-    const uint32_t i = tid + j * kSortThreads;
+    const uint32_t i = tid + j * THREADS;
     if (i < held) {
       const Pair q = __builtin_bit_cast(Pair, u.sorted[i]);
       dst((int64_t)(delta[(q.key >> shift) & mask] + i), q);
@@ -1162,7 +1175,6 @@ __global__ __launch_bounds__(kBucketThreads) void bucket_sum_kernel(const uint32
   // lanes with the same row wait for one another, while 8 positions still make a whole sector to load
   constexpr int kPart = (int)(kBucketTile / kBucketWaves), kPlace = kPart / 8, U = 4;
   const uint32_t begin = t.tile * (uint32_t)kBucketTile + wave * kPart;
-  float* mine = table + wave * floats;
   for (int s0 = 0; s0 < kPlace / 8 && begin < t.count; s0 += U) {
     uint32_t slot[U];
     bool valid[U];
@@ -1183,11 +1195,11 @@ __global__ __launch_bounds__(kBucketThreads) void bucket_sum_kernel(const uint32
       const int turn = valid[u] ? __popcll(peers & ((1ull << lane) - 1)) : -1;
       for (int now = 0; __ballot(turn >= now); ++now) {
         if (turn == now) {
-          volatile float* a = mine + slot[u] * DM;
+          float* a = table + wave * floats + slot[u] * DM;
 #pragma unroll
-          for (int k = 0; k < DM; ++k) a[k] = a[k] + (float)r[u].e[k];
+          for (int k = 0; k < DM; ++k) a[k] += (float)r[u].e[k];
         }
-        __builtin_amdgcn_wave_barrier();
+        wave_fence();
       }
     }
   }
@@ -1269,8 +1281,7 @@ struct BucketWs {
   int64_t counts, totals, keys, rows, partial, multi, bytes;
 };
 
-constexpr int kBucketItems = 16;
-inline int64_t partition_tiles(int64_t N) { return (N + kSortThreads * kBucketItems - 1) / (kSortThreads * kBucketItems); }
+inline int64_t partition_tiles(int64_t N) { return (N + kTileThreads * kTileItems - 1) / (kTileThreads * kTileItems); }
 
 inline BucketWs bucket_ws(int64_t N, const BucketPlan& b, int64_t g_bytes) {
   BucketWs w;
@@ -1295,20 +1306,24 @@ inline void sort_pass(Src src, int64_t N, int pass, const SortPlan& s, char* ws,
   uint32_t* counts = (uint32_t*)(ws + w.counts);
   uint32_t* totals = s.tiles <= kFewTiles ? nullptr : (uint32_t*)(ws + w.totals);
   const int shift = pass * s.width;
-  auto go = [&](auto bins, auto items) {
-    constexpr int BINS = decltype(bins)::value, ITEMS = decltype(items)::value;
-    hipLaunchKernelGGL((sort_count_kernel<Src, BINS, ITEMS>), dim3((unsigned)s.tiles), dim3(kSortThreads), 0, st, src, N,
-                       shift, s.width, counts);
-    if (totals) hipLaunchKernelGGL(sort_scan_kernel, dim3(BINS / kScanDigits), dim3(kScanThreads), 0, st, counts, s.tiles,
-                                   BINS, totals);
-    hipLaunchKernelGGL((sort_scatter_kernel<Src, StorePairs, BINS, ITEMS>), dim3((unsigned)s.tiles), dim3(kSortThreads), 0,
-                       st, src, N, shift, s.width, counts, s.tiles, totals, StorePairs{(Pair*)(ws + w.pairs[pass & 1])});
+  auto go = [&](auto bins, auto threads, auto items) {
+    constexpr int BINS = decltype(bins)::value, THREADS = decltype(threads)::value, ITEMS = decltype(items)::value;
+    hipLaunchKernelGGL((sort_count_kernel<Src, BINS, THREADS, ITEMS>), dim3((unsigned)s.tiles), dim3(THREADS), 0, st, src,
+                       N, shift, s.width, counts);
+    if (totals)
+      hipLaunchKernelGGL(sort_scan_kernel, dim3(BINS / kScanDigits), dim3(kScanThreads), 0, st, counts, s.tiles, BINS,
+                         totals);
+    hipLaunchKernelGGL((sort_scatter_kernel<Src, StorePairs, BINS, THREADS, ITEMS>), dim3((unsigned)s.tiles),
+                       dim3(THREADS), 0, st, src, N, shift, s.width, counts, s.tiles, totals,
+                       StorePairs{(Pair*)(ws + w.pairs[pass & 1])});
   };
   using std::integral_constant;
-  if (s.bins == 256 && s.items == 8) go(integral_constant<int, 256>{}, integral_constant<int, 8>{});
-  else if (s.bins == 256) go(integral_constant<int, 256>{}, integral_constant<int, 16>{});
-  else if (s.items == 8) go(integral_constant<int, 1024>{}, integral_constant<int, 8>{});
-  else go(integral_constant<int, 1024>{}, integral_constant<int, 16>{});
+  auto sized = [&](auto bins) {
+    if (s.few) go(bins, integral_constant<int, kFewThreads>{}, integral_constant<int, kFewItems>{});
+    else go(bins, integral_constant<int, kTileThreads>{}, integral_constant<int, kTileItems>{});
+  };
+  if (s.bins == 256) sized(integral_constant<int, 256>{});
+  else sized(integral_constant<int, 1024>{});
 }
 
 // sorts the ids; returns which of the two buffers holds the pairs
@@ -1339,12 +1354,12 @@ inline void bucket_gradient(const GT* g, const IT* ids, int64_t N, int64_t V, in
   uint32_t *counts = (uint32_t*)(ws + w.counts), *totals = (uint32_t*)(ws + w.totals), *keys = (uint32_t*)(ws + w.keys);
   const int64_t tiles = partition_tiles(N);
   const KeyFromIds<IT> src{ids, V, pad, (uint32_t)(b.buckets << b.lrows)};
-  hipLaunchKernelGGL((sort_count_kernel<KeyFromIds<IT>, 1024, kBucketItems>), dim3((unsigned)tiles), dim3(kSortThreads), 0,
-                     st, src, N, b.lrows, 10, counts);
+  hipLaunchKernelGGL((sort_count_kernel<KeyFromIds<IT>, 1024, kTileThreads, kTileItems>), dim3((unsigned)tiles),
+                     dim3(kTileThreads), 0, st, src, N, b.lrows, 10, counts);
   hipLaunchKernelGGL(sort_scan_kernel, dim3(1024 / kScanDigits), dim3(kScanThreads), 0, st, counts, tiles, 1024, totals);
   const StoreRows<E, DM> dst{(const E*)g, (int)D, m, keys, (Row<E, DM>*)(ws + w.rows)};
-  hipLaunchKernelGGL((sort_scatter_kernel<KeyFromIds<IT>, StoreRows<E, DM>, 1024, kBucketItems>), dim3((unsigned)tiles),
-                     dim3(kSortThreads), 0, st, src, N, b.lrows, 10, counts, tiles, totals, dst);
+  hipLaunchKernelGGL((sort_scatter_kernel<KeyFromIds<IT>, StoreRows<E, DM>, 1024, kTileThreads, kTileItems>),
+                     dim3((unsigned)tiles), dim3(kTileThreads), 0, st, src, N, b.lrows, 10, counts, tiles, totals, dst);
   const unsigned lds = (unsigned)(kBucketWaves * ((int64_t)DM << b.lrows) * 4);
   float* partial = (float*)(ws + w.partial);
   BucketTile* multi = (BucketTile*)(ws + w.multi);
