@@ -77,6 +77,7 @@ def test_embedding_c_refusals_of_one_direction():
                     (dict(ot=-1), "type"), (dict(stride=-4), "stride")]:
         assert fwd(**kw) == 1 and msg in err(), kw
     for kw, msg in [(dict(g=None), "null"), (dict(grad=None), "null"), (dict(ws=None), "null"), (dict(gt=9), "type"),
+                    (dict(ws=ctypes.c_void_p(24)), "16 bytes"),
                     (dict(pad=5), "padding_idx"), (dict(pad=-2), "padding_idx")]:
         assert bwd(**kw) == 1 and msg in err(), kw
     assert fwd(N=0, table=None, ids=None, out=None) == 0 and fwd(D=0, table=None, ids=None, out=None) == 0
@@ -86,6 +87,20 @@ def test_embedding_c_refusals_of_one_direction():
     assert L.yanerf_embedding_bwd_workspace_bytes(1 << 31, 5, 4) == -1
     assert L.yanerf_embedding_bwd_workspace_bytes(0, 5, 4) == 0
     assert L.yanerf_embedding_bwd_workspace_bytes(1000, 5, 4) > 0
+
+
+def test_workspace_query_over_the_range():
+    """Every allowed size has a plan, from one id, row and column to the largest, and the workspace stays within what the
+    pairs (16 bytes an id), a few copies of g's rows in fp32 and the smaller tables need."""
+    L = _C.lib()
+    for n in (1, 2, 4096, 4097, 16384, 16385, 131072, 10 ** 6, 2 ** 31 - 1):
+        for v in (1, 2, 17, 100, 128, 129, 1023, 1024, 50000, 10 ** 6, 2 ** 31 - 1):
+            for d in (1, 2, 3, 7, 8, 9, 48, 65, 1000, 1024, 1001, 2 ** 24 - 1, 2 ** 24):
+                if n * d > 2 ** 36 or v * d > 2 ** 36:
+                    assert L.yanerf_embedding_bwd_workspace_bytes(n, v, d) == -1
+                    continue
+                b = L.yanerf_embedding_bwd_workspace_bytes(n, v, d)
+                assert 0 < b <= 64 * n + 16 * n * d + 2 ** 16 * d + 2 ** 26, (n, v, d, b)
 
 
 def test_code_table_arguments():

@@ -76,12 +76,32 @@ def test_counts(ops, n, kind):
     check_train(ops, n, 300, 40, dtype=BF16, kind=kind, p=0.1, seed=n % 97)
 
 
-@pytest.mark.parametrize("v", [1, 2, 3, 17, 100, 127, 128, 255, 256, 257, 511, 512, 513, 1024, 32767, 32768, 65535, 65536, 300000])
+@pytest.mark.parametrize("v", [1, 2, 3, 17, 32, 33, 100, 127, 128, 255, 256, 257, 511, 512, 513, 1024, 32767, 32768, 65535, 65536, 300000])
 @pytest.mark.parametrize("n", [1, 700, 9001, 40000])
 def test_tables(ops, v, n):
     check_train(ops, n, v, 4, seed=v % 89)
     check_train(ops, n, v, 3, kind="zipf", idt=torch.int32, pad=v // 2, seed=v % 89)
     check_train(ops, n, v, 24, dtype=F16, kind="uniform", p=0.5, pad=-1, seed=v % 89)
+
+
+def test_ranks_of_wide_keys(ops):
+    """Up to 16384 ids are ranked in LDS: ids beyond 2^18 need 64-bit pairs, and all ids in one row fill one bin."""
+    for v in ((1 << 18) - 1, 1 << 18, 5000000):
+        for kind in ("uniform", "zipf", "one"):
+            check_train(ops, 16384, v, 5, kind=kind, seed=v % 13)
+    for v in (40, 1000, 60000):
+        check_train(ops, 16384, v, 20, kind="one", seed=v % 13)
+        check_train(ops, 16383, v, 20, kind="ends", p=0.1, seed=v % 13)
+
+
+def test_tables_around_the_path_limits(ops):
+    """Gradients around 32 MB, where short id lists leave the one-launch path, and row sizes around 16 bytes."""
+    for v in (16383, 16384, 16385):
+        check_train(ops, 3000, v, 512, kind="zipf", seed=v % 7)
+        check_train(ops, 3000, v, 1024, dtype=BF16, kind="uniform", p=0.1, seed=v % 7)
+    for n in (16384, 16385):
+        for d in (4, 5):
+            check_train(ops, n, 900, d, seed=d)
 
 
 def test_wide_rows_and_many_ids(ops):
@@ -269,7 +289,8 @@ def test_double_backward_is_refused(ops):
         gx.sum().backward()
 
 
-def test_past_32_bits(ops):
+@pytest.mark.parametrize("small_rows", [11, 40])
+def test_past_32_bits(ops, small_rows):
     """A table and an output of more than 2^32 elements: rows behind that line are read, written and (the mask's counter)
     drawn at their own place."""
     v, d = 70000, 65536
@@ -279,8 +300,8 @@ def test_past_32_bits(ops):
     ids = torch.tensor([v - 1, 0, v - 3, v - 2, 1], device=DEV)
     assert torch.equal(ops.embedding(table, ids), table[ids])
     del table
-    small = rand(11, d, dtype=BF16)
-    ids = some_ids(v, 11)
+    small = rand(small_rows, d, dtype=BF16)
+    ids = some_ids(v, small_rows)
     y = ops.embedding(small, ids, dropout=0.5, rng=(5, 6), scale=0.5)
     for n in (0, 65535, 65536, v - 1):
         keep = R.philox_words(n * d // 4, d // 4, 5, 6) >= np.uint64(1 << 31)
@@ -296,14 +317,14 @@ def test_past_32_bits(ops):
     leaf = small.clone().requires_grad_()
     out = ops.embedding(leaf, ids)
     (gt,) = torch.autograd.grad(out, leaf, y)
-    want = torch.zeros(11, d, dtype=torch.float64, device=DEV)
-    size = torch.zeros(11, d, dtype=torch.float64, device=DEV)
-    for k in range(11):
+    want = torch.zeros(small_rows, d, dtype=torch.float64, device=DEV)
+    size = torch.zeros(small_rows, d, dtype=torch.float64, device=DEV)
+    for k in range(small_rows):
         sel = (ids == k).nonzero().flatten()
         for part in sel.split(1024):
             want[k] += y[part].double().sum(0)
             size[k] += y[part].double().abs().sum(0)
-    bound = 1.01 * (ids.bincount(minlength=11)[:, None].double() * 2.0 ** -24) * size
+    bound = 1.01 * (ids.bincount(minlength=small_rows)[:, None].double() * 2.0 ** -24) * size
     assert ((gt.double() - want).abs() <= bound + (want.abs() + bound) * (2.0 ** -8 + 2.0 ** -22)).all()
 
 

@@ -9,8 +9,14 @@
 // T = round(p 2^32): forward and backward evaluate it anew, so no mask is stored or read. A dropped element is 0
 // whatever its input holds. Products and sums are fp32; each output is rounded once.
 //
-// The gradient sorts the positions by id with a stable sort, so the terms of a row are added in an order that only the
-// ids fix: no float atomics, the same bits on every run.
+// The gradient groups the positions of each row with stable sorts, so the terms of a row are added in an order that the ids
+// alone fix: no float atomics, the same bits on every run. Which way depends on the sizes:
+//
+//   N <= 4096, gradient <= 32 MB            one launch, each workgroup picks the ids of its own rows (own_rows_kernel)
+//   V <= 32                                 one pass over g with a table a lane (dense_sum_kernel)
+//   N > 16384, rows of g of <= 16 bytes     one partition that carries the rows along (bucket_sum_kernel)
+//   the rest                                a sort of (id, position) pairs, then sums over pieces of the sorted list
+//                                           (rank_sort_kernel to N = 16384, sort_scatter_kernel beyond; run_sum_kernel)
 #include <cmath>
 #include <type_traits>
 
@@ -469,7 +475,7 @@ __global__ __launch_bounds__(THREADS) void sort_scatter_kernel(Src src, int64_t 
   constexpr int BITS = BINS == 256 ? 8 : 10;
   __shared__ union {
     uint32_t cnt[WAVES][BINS];  // a wave's count of each digit so far, then its first slot
-    uint64_t sorted[TILE];           // the tile in order, once every lane knows its slots
+    uint64_t sorted[TILE];      // the tile in order, once every lane knows its slots
   } u;
   __shared__ uint32_t delta[BINS];  // place in the output less place in the tile
   __shared__ uint32_t part[WAVES];
@@ -573,14 +579,26 @@ constexpr int kIndexBits = 14;
 constexpr int64_t kRankMax = 1 << kIndexBits;
 constexpr int kRankThreads = 1024, kRankWaves = kRankThreads / 64, kRankItems = 4, kRankTile = kRankWaves * kRankItems;
 constexpr int kRankBins = 2048;
-__device__ __forceinline__ uint32_t rank_bin(uint32_t key) {  // at most 1727, rising with the key
-  const int e = key < 64 ? 0 : 25 - __builtin_clz(key);
-  return (e << 6) + (key >> e);
+// The bin of a pair, rising with it: of 1 / 64 of the key (at most 1727), or, where a small table leaves bins over, of the
+// key and the leading `index_bits` bits of the index (a row that every id names would otherwise fill one bin).
+struct RankBins {
+  int index_bits;
+  __device__ __forceinline__ uint32_t operator()(uint32_t key, uint32_t index) const {
+    if (index_bits) return (key << index_bits) | (index >> (kIndexBits - index_bits));
+    const int e = key < 64 ? 0 : 25 - __builtin_clz(key);
+    return (e << 6) + (key >> e);
+  }
+};
+inline RankBins rank_bins(int64_t V) {  // keys 0 .. V
+  int b = kIndexBits;
+  while (b > 0 && ((V + 1) << b) > kRankBins) --b;
+  return {b};
 }
 
 // LDS: all pairs by bin
 template <typename IT, typename P>
-__global__ __launch_bounds__(kRankThreads) void rank_sort_kernel(KeyFromIds<IT> src, int N, Pair* out) {
+__global__ __launch_bounds__(kRankThreads) void rank_sort_kernel(KeyFromIds<IT> src, int N, RankBins bins,
+                                                                 Pair* out) {
   extern __shared__ __attribute__((aligned(16))) char rank_lds[];
   P* binned = (P*)rank_lds;
   // a bin is dealt out in COPIES parts, by lane: word frequencies fill some bins with a third of the ids, and atomics on
@@ -597,7 +615,7 @@ __global__ __launch_bounds__(kRankThreads) void rank_sort_kernel(KeyFromIds<IT> 
   for (int j = 0; j < R; ++j) key[j] = tid + j * kRankThreads < N ? src.at(tid + j * kRankThreads).key : 0u;
 #pragma unroll
   for (int j = 0; j < R; ++j)
-    if (tid + j * kRankThreads < N) atomicAdd(&next[rank_bin(key[j]) * COPIES + copy], 1u);
+    if (tid + j * kRankThreads < N) atomicAdd(&next[bins(key[j], tid + j * kRankThreads) * COPIES + copy], 1u);
   __syncthreads();
   uint32_t c[PER], sum = 0, all;
 #pragma unroll
@@ -617,7 +635,7 @@ __global__ __launch_bounds__(kRankThreads) void rank_sort_kernel(KeyFromIds<IT> 
 #pragma unroll
   for (int j = 0; j < R; ++j) {
     const int i = tid + j * kRankThreads;
-    if (i < N) binned[atomicAdd(&next[rank_bin(key[j]) * COPIES + copy], 1u)] = ((P)key[j] << kIndexBits) | (P)i;
+    if (i < N) binned[atomicAdd(&next[bins(key[j], i) * COPIES + copy], 1u)] = ((P)key[j] << kIndexBits) | (P)i;
   }
   __syncthreads();
   const int first = blockIdx.x * kRankTile + (tid >> 6) * kRankItems;
@@ -629,8 +647,9 @@ __global__ __launch_bounds__(kRankThreads) void rank_sort_kernel(KeyFromIds<IT> 
     if (first + t >= N) return;
     const uint32_t k = __builtin_amdgcn_readfirstlane(item[t]);
     const P mine = ((P)k << kIndexBits) | (P)(first + t);
-    const uint32_t begin = __builtin_amdgcn_readfirstlane(start[rank_bin(k)]);
-    const uint32_t end = __builtin_amdgcn_readfirstlane(start[rank_bin(k) + 1]);
+    const uint32_t bin = bins(k, first + t);
+    const uint32_t begin = __builtin_amdgcn_readfirstlane(start[bin]);
+    const uint32_t end = __builtin_amdgcn_readfirstlane(start[bin + 1]);
     uint32_t rank = begin;
     for (uint32_t i = begin; i < end; i += 256) {
       P other[4];
@@ -675,8 +694,8 @@ struct RunEnds {
 
 // Adds the sorted positions [0, N) of `src` that this workgroup's groups hold: group q the `piece` from base + q * piece.
 // src.pair(i) holds the key that orders the runs and the row of g, src.row(key) is the row of the table; a key of
-// src.none() takes no part. The runs that enter or leave the workgroup's span go to heads / tails [D], which a workgroup with the whole of
-// [0, N) never writes.
+// src.none() takes no part. The runs that enter or leave the workgroup's span go to heads / tails [D], which a workgroup
+// with the whole of [0, N) never writes.
 template <int THREADS, typename GT, typename TT, int VEC, typename Src>
 __device__ __forceinline__ void sum_runs(RunEnds<THREADS, VEC>& ends, const Src& src, int64_t N, int64_t base, int piece,
                                          int lg, const GT* g, int64_t D, int64_t d, const Mask& m, uint64_t off, float f,
@@ -777,6 +796,7 @@ __device__ __forceinline__ void sum_runs(RunEnds<THREADS, VEC>& ends, const Src&
 // word frequencies favour, spread over the chip. What it costs is that each workgroup reads every id (from L2).
 constexpr int kOwnThreads = 512, kOwnWaves = kOwnThreads / 64;
 constexpr int64_t kOwnMax = 4096;  // ids
+constexpr int64_t kOwnTable = 32ll << 20;  // bytes of the gradient
 
 struct OwnPlan {
   int lg;           // log2 of the lanes a group
@@ -790,12 +810,15 @@ struct OwnPlan {
 inline OwnPlan own_plan(int64_t N, int64_t V, int64_t D, int vec, int64_t g_bytes, int64_t t_bytes) {
   OwnPlan o;
   const int64_t dv = (D + vec - 1) / vec;
-  o.lg = 0;
-  while (o.lg < 4 && (1ll << o.lg) < dv) ++o.lg;  // up to 16 lanes: 256 bytes of a row
-  while (o.lg < 6 && ((dv + (1 << o.lg) - 1) >> o.lg) > 64) ++o.lg;
-  o.chunks = (dv + (1 << o.lg) - 1) >> o.lg;
   o.lgroup = 0;
   while (((int64_t)1 << o.lgroup) * D * t_bytes < 128 && ((int64_t)1 << o.lgroup) < V) ++o.lgroup;
+  // up to 16 lanes, 256 bytes of a row; fewer, but 4, where a small table would leave CUs idle
+  const int64_t groups = (V + (1ll << o.lgroup) - 1) >> o.lgroup;
+  o.lg = 0;
+  while (o.lg < 4 && (1ll << o.lg) < dv) ++o.lg;
+  while (o.lg > 2 && ((dv + (1 << o.lg) - 1) >> o.lg) * groups < 64) --o.lg;
+  while (o.lg < 6 && ((dv + (1 << o.lg) - 1) >> o.lg) > 256) ++o.lg;
+  o.chunks = (dv + (1 << o.lg) - 1) >> o.lg;
   // owners: one for every 32 KB of zeros or 8 KB of gradient rows, up to 1024 workgroups
   const int64_t most = 1024 / o.chunks > 1 ? 1024 / o.chunks : 1;
   int64_t want = V * D * t_bytes / 32768;
@@ -810,9 +833,10 @@ inline OwnPlan own_plan(int64_t N, int64_t V, int64_t D, int vec, int64_t g_byte
   o.lds = (int64_t)o.cap * 4 + (o.slots + 31) / 32 * 4;
   return o;
 }
-// the list packs (slot, index) into 32 bits, and list and presence bits share the LDS with RunEnds
-inline bool own_fits(int64_t N, const OwnPlan& o) {
-  return N <= kOwnMax && o.slots < (1ll << (32 - kIndexBits)) && o.lds <= 100 * 1024;
+// the list packs (slot, index) into 32 bits, and list and presence bits share the LDS with RunEnds; large tables are left
+// to the sorted path, whose zeros stream faster
+inline bool own_fits(int64_t N, int64_t table_bytes, const OwnPlan& o) {
+  return N <= kOwnMax && table_bytes <= kOwnTable && o.slots < (1ll << (32 - kIndexBits)) && o.lds <= 100 * 1024;
 }
 
 struct OwnList {
@@ -932,6 +956,115 @@ __global__ __launch_bounds__(kOwnThreads) void own_rows_kernel(const GT* g, cons
   const int64_t d = d0 + (tid & ((1 << o.lg) - 1)) * VEC;
   const int piece = (M + groups - 1) / groups;
   sum_runs<kOwnThreads, GT, TT, VEC>(ends, src, M, 0, piece, o.lg, g, D, d, m, mask_offset(m), f, grad, nullptr, nullptr);
+}
+
+// ---- many ids of a small table: no sort. Every lane keeps a table of its own in LDS (all rows, its vector of columns) and
+// adds the rows of g it is given, which are consecutive for a workgroup and so read once, in order and whole; lanes that
+// hold the same columns are then added in order, and the workgroups' tables in a second launch. Neither the ids nor their
+// distribution change what it costs. Tables of up to 32 rows, whose LDS lets a lane have 4 columns (a row more would halve
+// them: 100 rows with 1 column a lane, 10^6 ids of 16 columns, took 104 us, sorting 73).
+constexpr int kDenseThreads = 256;
+constexpr int64_t kDenseRows = 32;
+
+struct DensePlan {
+  int vec;             // elements a lane, 0: the path does not fit
+  int lg;              // log2 of the lanes a row of g
+  int64_t chunks;      // column chunks
+  int64_t rows, blocks;  // rows of g a workgroup, workgroups a chunk
+  int64_t lds;
+};
+
+// vec: the most that the pointers and D allow; this path takes up to 4
+inline DensePlan dense_plan(int64_t N, int64_t V, int64_t D, int vec) {
+  DensePlan p{0, 0, 0, 0, 0, 0};
+  vec = vec < 4 ? vec : 4;
+  if (N <= kOwnMax || V > kDenseRows) return p;
+  p.vec = vec;
+  p.lds = V * kDenseThreads * vec * 4;
+  const int64_t dv = (D + vec - 1) / vec;
+  while (p.lg < 6 && (1ll << p.lg) < dv) ++p.lg;
+  p.chunks = (dv + (1 << p.lg) - 1) >> p.lg;
+  // as many workgroups as the chip holds at once, but 4 rows a lane
+  int64_t per_cu = 160 * 1024 / p.lds;
+  per_cu = per_cu > 8 ? 8 : per_cu;
+  int64_t want = 256 * per_cu / p.chunks;
+  want = want < 1 ? 1 : want;
+  const int64_t least = (kDenseThreads >> p.lg) * 4;
+  p.rows = (N + want - 1) / want;
+  p.rows = p.rows > least ? p.rows : least;
+  p.blocks = (N + p.rows - 1) / p.rows;
+  return p;
+}
+
+template <typename GT, int VEC>
+__global__ __launch_bounds__(kDenseThreads) void dense_sum_kernel(const GT* g, const void* ids, int id_bytes, int64_t N,
+                                                                  int64_t V, int64_t D, int64_t pad, DensePlan p, Mask m,
+                                                                  float* partial) {
+  extern __shared__ float dense_table[];  // [row][lane][VEC]
+  const int tid = threadIdx.x, groups = kDenseThreads >> p.lg, group = tid >> p.lg, sub = tid & ((1 << p.lg) - 1);
+  const int64_t block = blockIdx.x % (uint32_t)p.blocks, chunk = blockIdx.x / (uint32_t)p.blocks;
+  const int64_t d = ((chunk << p.lg) + sub) * VEC;
+  for (int v = 0; v < (int)V; ++v)
+#pragma unroll
+    for (int k = 0; k < VEC; ++k) dense_table[(v * kDenseThreads + tid) * VEC + k] = 0.0f;
+  const uint64_t off = mask_offset(m);
+  const int64_t begin = block * p.rows, end = begin + p.rows < N ? begin + p.rows : N;
+  constexpr int U = 8;
+  for (int64_t n0 = begin + group; n0 < end; n0 += groups * U) {
+    int64_t id[U];
+    float v[U][VEC];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int64_t n = n0 + u * groups;
+      id[u] = -1;
+      if (n < end && d < D) {
+        id[u] = id_bytes == 8 ? ((const int64_t*)ids)[n] : (int64_t)((const int32_t*)ids)[n];
+        load_vec<GT, VEC, (VEC > 1), false>(g + n * D + d, v[u]);
+      }
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      if (id[u] < 0 || id[u] >= V || id[u] == pad) continue;
+      if (m.mode != 0) apply_keep<VEC>(m, off, (n0 + u * groups) * D + d, v[u]);
+      float* a = dense_table + ((int)id[u] * kDenseThreads + tid) * VEC;
+#pragma unroll
+      for (int k = 0; k < VEC; ++k) a[k] += v[u][k];
+    }
+  }
+  __syncthreads();
+  for (int t = tid; t < (int)V << p.lg; t += kDenseThreads) {
+    const int v = t >> p.lg, c = t & ((1 << p.lg) - 1);
+    const int64_t e = ((chunk << p.lg) + c) * VEC;
+    if (e >= D) continue;
+    float s[VEC] = {};
+    for (int q = 0; q < groups; ++q) {
+#pragma unroll
+      for (int k = 0; k < VEC; ++k) s[k] += dense_table[(v * kDenseThreads + (q << p.lg) + c) * VEC + k];
+    }
+#pragma unroll
+    for (int k = 0; k < VEC; ++k) partial[block * V * D + v * D + e + k] = s[k];
+  }
+}
+
+// grad[k] = f * (the workgroups' tables in order), 2^lo elements a workgroup, whose other lanes take consecutive workgroups
+constexpr int kDenseJoinThreads = 1024;
+template <typename TT>
+__global__ __launch_bounds__(kDenseJoinThreads) void dense_join_kernel(const float* partial, int64_t blocks, int64_t n, int lo,
+                                                                       float f, TT* grad) {
+  __shared__ float sums[kDenseJoinThreads];
+  const int out = threadIdx.x & ((1 << lo) - 1), part = threadIdx.x >> lo, parts = kDenseJoinThreads >> lo;
+  const int64_t k = ((int64_t)blockIdx.x << lo) + out;
+  const int64_t per = (blocks + parts - 1) / parts, begin = part * per, end = begin + per < blocks ? begin + per : blocks;
+  float s = 0.0f;
+  if (k < n) {
+#pragma unroll 8
+    for (int64_t b = begin; b < end; ++b) s += partial[b * n + k];
+  }
+  sums[threadIdx.x] = s;
+  __syncthreads();
+  if (part != 0 || k >= n) return;
+  for (int q = 1; q < parts; ++q) s += sums[(q << lo) + out];
+  grad[k] = (TT)(s * f);
 }
 
 // ---- long id lists: the sorted pairs in memory, a workgroup's runs cut by its neighbours' joined in a second launch
@@ -1335,7 +1468,8 @@ inline int sort_ids(const IT* ids, int64_t N, int64_t V, int64_t pad, char* ws, 
     const bool narrow = V < (1ll << (32 - kIndexBits));  // keys 0 .. V beside the index in 32 bits
     auto* k = narrow ? rank_sort_kernel<IT, uint32_t> : rank_sort_kernel<IT, uint64_t>;
     hipLaunchKernelGGL(k, dim3((unsigned)((N + kRankTile - 1) / kRankTile)), dim3(kRankThreads),
-                       (unsigned)(N * (narrow ? 4 : 8)), st, src, (int)N, (Pair*)(ws + w.pairs[0]));
+                       (unsigned)(N * (narrow ? 4 : 8)), st, src, (int)N, rank_bins(V),
+                       (Pair*)(ws + w.pairs[0]));
     return 0;
   }
   for (int pass = 0; pass < s.passes; ++pass) {
@@ -1479,6 +1613,10 @@ int64_t yanerf_embedding_bwd_workspace_bytes(int64_t N, int64_t V, int64_t D) {
   if (embedding_sizes_ok("embedding_bwd_workspace", N, V, D)) return -1;
   if (N == 0 || V == 0 || D == 0) return 0;
   int64_t bytes = grad_ws(N, V, D).bytes;
+  for (int vec : {1, 2, 4}) {
+    const DensePlan p = dense_plan(N, V, D, vec);
+    if (p.vec && p.blocks * V * D * 4 > bytes) bytes = p.blocks * V * D * 4;
+  }
   for (int64_t gb : {2, 4}) {  // of whichever type g has
     const BucketPlan b = bucket_plan(N, V, D, gb);
     if (b.buckets) {
@@ -1503,6 +1641,7 @@ int yanerf_embedding_backward(const void* g, int g_type, const void* ids, int id
   if (V == 0 || D == 0) return 0;
   YN_CHECK(grad_table, "embedding_backward: null pointer");
   YN_CHECK(N == 0 || (g && ids && workspace), "embedding_backward: null pointer");
+  YN_CHECK(aligned(workspace, 16), "embedding_backward: the workspace is not aligned to 16 bytes");
   const Mask m = make_mask(p, seed, offset, rng_base);
   const float f = (float)(scale * mask_scale(p, m));
   hipStream_t st = as_stream(stream);
@@ -1522,13 +1661,32 @@ int yanerf_embedding_backward(const void* g, int g_type, const void* ids, int id
     using TT = decltype(tt);
     constexpr int VEC = decltype(vc)::value;
     const OwnPlan o = own_plan(N < kOwnMax ? N : kOwnMax, V, D, VEC, gb, tb);
-    if (own_fits(N, o)) {
+    if (own_fits(N, V * D * tb, o)) {
       hipLaunchKernelGGL((own_rows_kernel<GT, TT, VEC>), dim3((unsigned)(o.chunks << o.lown)), dim3(kOwnThreads),
                          (unsigned)o.lds, st, (const GT*)g, ids, id_bytes, (int)N, V, D, padding_idx, o, m, f,
                          (TT*)grad_table);
       return;
     }
     const BucketPlan b = bucket_plan(N, V, D, gb);
+    const DensePlan p = dense_plan(N, V, D, VEC);
+    if (p.vec) {
+      float* partial = (float*)ws;
+      auto go = [&](auto dc) {
+        constexpr int DV = decltype(dc)::value;
+        if constexpr (DV <= VEC)
+          hipLaunchKernelGGL((dense_sum_kernel<GT, DV>), dim3((unsigned)(p.blocks * p.chunks)), dim3(kDenseThreads),
+                             (unsigned)p.lds, st, (const GT*)g, ids, id_bytes, N, V, D, padding_idx, p, m, partial);
+      };
+      using std::integral_constant;
+      if (p.vec == 1) go(integral_constant<int, 1>{});
+      else if (p.vec == 2) go(integral_constant<int, 2>{});
+      else go(integral_constant<int, 4>{});
+      int lo = 0;
+      while (lo < 6 && (1ll << lo) < V * D) ++lo;
+      hipLaunchKernelGGL((dense_join_kernel<TT>), dim3((unsigned)((V * D + (1 << lo) - 1) >> lo)), dim3(kDenseJoinThreads),
+                         0, st, partial, p.blocks, V * D, lo, f, (TT*)grad_table);
+      return;
+    }
     if (N > kRankMax && b.buckets) {
       with_index(id_bytes, [&](auto it) {
         using IT = decltype(it);

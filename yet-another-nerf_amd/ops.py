@@ -587,7 +587,9 @@ _ID_FLAGS: dict = {}  # device -> sticky int32 flag of ids outside their table (
 def _id_flag(dev) -> Optional[torch.Tensor]:
     f = _ID_FLAGS.get(dev)
     if f is None and not torch.cuda.is_current_stream_capturing():  # a capture's memory is the graph's own
-        f = _ID_FLAGS[dev] = torch.zeros(1, dtype=torch.int32, device=dev)
+        f = torch.zeros(1, dtype=torch.int32, device=dev)
+        torch.cuda.current_stream(dev).synchronize()  # cleared before any stream's lookup can set it
+        _ID_FLAGS[dev] = f
     return f
 
 
