@@ -54,7 +54,9 @@ __device__ __forceinline__ u4 philox(uint64_t seed, uint64_t ctr_hi, uint64_t ct
   for (int i = 0; i < 10; ++i) {
     // one 32 x 32 -> 64 multiply each (v_mad_u64_u32): __umulhi and a low product are two of them
     const uint64_t p0 = (uint64_t)0xD2511F53u * c0, p1 = (uint64_t)0xCD9E8D57u * c2;
-    uint32_t n0 = (uint32_t)(p1 >> 32) ^ c1 ^ k0, n1 = (uint32_t)p1, n2 = (uint32_t)(p0 >> 32) ^ c3 ^ k1, n3 = (uint32_t)p0;
+    // and one v_bitop3_b32 (truth table 0x96: a ^ b ^ c) each
+    const uint32_t n0 = __builtin_amdgcn_bitop3_b32((uint32_t)(p1 >> 32), c1, k0, 0x96), n1 = (uint32_t)p1;
+    const uint32_t n2 = __builtin_amdgcn_bitop3_b32((uint32_t)(p0 >> 32), c3, k1, 0x96), n3 = (uint32_t)p0;
     c0 = n0; c1 = n1; c2 = n2; c3 = n3;
     k0 += 0x9E3779B9u; k1 += 0xBB67AE85u;
   }
