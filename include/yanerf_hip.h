@@ -285,8 +285,8 @@ int yanerf_embedding_forward(const void* table, int table_type, int64_t table_st
                              int64_t N, int64_t V, int64_t D, double scale, double p, uint64_t seed, uint64_t offset,
                              const uint64_t* rng_base, uint64_t* rng_used, void* out, int out_type, int* oob,
                              void* stream);
-/* Bytes of yanerf_embedding_backward's workspace (16-byte aligned, its contents need not be set), -1 for sizes out of
- * range. */
+/* Bytes of yanerf_embedding_backward's workspace (16-byte aligned, its contents need not be set; it may be NULL where
+ * they are 0), -1 for sizes out of range. */
 int64_t yanerf_embedding_bwd_workspace_bytes(int64_t N, int64_t V, int64_t D);
 /* grad_table[v][d] = scale / (1 - p) * sum over n with ids[n] = v of keep(n D + d) g[n][d]: every row is written, rows
  * that no id names and row padding_idx (-1: none; its lookup is that of any row) with zeros. Ids outside [0, V) take no part. The order of each sum

@@ -76,7 +76,7 @@ def test_embedding_c_refusals_of_one_direction():
     for kw, msg in [(dict(table=None), "null"), (dict(out=None), "null"), (dict(V=0), "empty table"),
                     (dict(ot=-1), "type"), (dict(stride=-4), "stride")]:
         assert fwd(**kw) == 1 and msg in err(), kw
-    for kw, msg in [(dict(g=None), "null"), (dict(grad=None), "null"), (dict(ws=None), "null"), (dict(gt=9), "type"),
+    for kw, msg in [(dict(g=None), "null"), (dict(grad=None), "null"), (dict(ws=None, N=5000), "null"), (dict(gt=9), "type"),
                     (dict(ws=ctypes.c_void_p(24)), "16 bytes"),
                     (dict(pad=5), "padding_idx"), (dict(pad=-2), "padding_idx")]:
         assert bwd(**kw) == 1 and msg in err(), kw
@@ -86,7 +86,8 @@ def test_embedding_c_refusals_of_one_direction():
     assert L.yanerf_embedding_bwd_workspace_bytes(-1, 5, 4) == -1
     assert L.yanerf_embedding_bwd_workspace_bytes(1 << 31, 5, 4) == -1
     assert L.yanerf_embedding_bwd_workspace_bytes(0, 5, 4) == 0
-    assert L.yanerf_embedding_bwd_workspace_bytes(1000, 5, 4) > 0
+    assert L.yanerf_embedding_bwd_workspace_bytes(1000, 5, 4) == 0  # one launch, nothing kept between
+    assert L.yanerf_embedding_bwd_workspace_bytes(5000, 5, 4) > 0
 
 
 def test_workspace_query_over_the_range():
@@ -100,7 +101,7 @@ def test_workspace_query_over_the_range():
                     assert L.yanerf_embedding_bwd_workspace_bytes(n, v, d) == -1
                     continue
                 b = L.yanerf_embedding_bwd_workspace_bytes(n, v, d)
-                assert 0 < b <= 64 * n + 16 * n * d + 2 ** 16 * d + 2 ** 26, (n, v, d, b)
+                assert (0 if n <= 4096 else 1) <= b <= 64 * n + 16 * n * d + 2 ** 16 * d + 2 ** 26, (n, v, d, b)
 
 
 def test_code_table_arguments():

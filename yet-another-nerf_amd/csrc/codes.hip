@@ -839,6 +839,11 @@ inline bool own_fits(int64_t N, int64_t table_bytes, const OwnPlan& o) {
   return N <= kOwnMax && table_bytes <= kOwnTable && o.slots < (1ll << (32 - kIndexBits)) && o.lds <= 100 * 1024;
 }
 
+// own_fits whatever the types and alignments (slots are at most V + 64 then): no workspace
+inline bool own_always(int64_t N, int64_t V, int64_t D) {
+  return N <= kOwnMax && V <= (1 << 17) && V * D * 4 <= kOwnTable;
+}
+
 struct OwnList {
   const uint32_t* list;
   OwnPlan o;
@@ -1611,7 +1616,7 @@ int yanerf_embedding_forward(const void* table, int table_type, int64_t table_st
 
 int64_t yanerf_embedding_bwd_workspace_bytes(int64_t N, int64_t V, int64_t D) {
   if (embedding_sizes_ok("embedding_bwd_workspace", N, V, D)) return -1;
-  if (N == 0 || V == 0 || D == 0) return 0;
+  if (N == 0 || V == 0 || D == 0 || own_always(N, V, D)) return 0;
   int64_t bytes = grad_ws(N, V, D).bytes;
   for (int vec : {1, 2, 4}) {
     const DensePlan p = dense_plan(N, V, D, vec);
@@ -1640,7 +1645,7 @@ int yanerf_embedding_backward(const void* g, int g_type, const void* ids, int id
            (long long)padding_idx);
   if (V == 0 || D == 0) return 0;
   YN_CHECK(grad_table, "embedding_backward: null pointer");
-  YN_CHECK(N == 0 || (g && ids && workspace), "embedding_backward: null pointer");
+  YN_CHECK(N == 0 || (g && ids && (workspace || own_always(N, V, D))), "embedding_backward: null pointer");
   YN_CHECK(aligned(workspace, 16), "embedding_backward: the workspace is not aligned to 16 bytes");
   const Mask m = make_mask(p, seed, offset, rng_base);
   const float f = (float)(scale * mask_scale(p, m));

@@ -7,7 +7,7 @@ from __future__ import annotations
 
 import ctypes
 import math
-from contextlib import contextmanager, nullcontext
+from contextlib import contextmanager
 from dataclasses import dataclass
 from typing import List, Optional, Sequence, Tuple
 
@@ -479,22 +479,10 @@ def adam_step(params: torch.Tensor, grads: torch.Tensor, exp_avg: torch.Tensor, 
 
 
 # ----------------------------------------------------------------------------------------- learned codes
+# Calls here are short next to their launches, so the checks are written for the host's time: device indices in place of
+# device objects, no autograd node where no gradient is wanted.
 _TYPES = {torch.float32: _C.TYPE_F32, torch.bfloat16: _C.TYPE_BF16, torch.float16: _C.TYPE_F16}
 _U64 = 0xFFFFFFFFFFFFFFFF
-
-
-def _code_type(what: str, dtype: torch.dtype) -> int:
-    if dtype not in _TYPES:
-        raise TypeError(f"{what}: element type {dtype} is not supported (float32, bfloat16, float16)")
-    return _TYPES[dtype]
-
-
-def _probability(what: str, p) -> float:
-    p = float(p)
-    if not 0.0 <= p <= 1.0:
-        raise ValueError(f"{what}: dropout probability {p} is not in [0, 1]")
-    return p
-
 
 _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)  # of a device, without a Stream object (3-14 us)
 
@@ -519,41 +507,59 @@ def _once(backward):
     return call
 
 
-def _mask_rng(what: str, p: float, rng, rng_base: Optional[torch.Tensor], dev: torch.device, n: int):
-    """(seed, offset) of a dropout mask over n elements; (0, 0) where none is drawn (p 0)."""
+def _code_type(what: str, dtype: torch.dtype) -> int:
+    t = _TYPES.get(dtype)
+    if t is None:
+        raise TypeError(f"{what}: element type {dtype} is not supported (float32, bfloat16, float16)")
+    return t
+
+
+def _mask(what: str, p, rng, rng_base: Optional[torch.Tensor], dev: int, n: int):
+    """(p, seed, offset, rng_base) of a dropout mask over n elements, checked; no draw where p is 0."""
+    p = float(p)
+    if not 0.0 <= p <= 1.0:
+        raise ValueError(f"{what}: dropout probability {p} is not in [0, 1]")
     if rng_base is not None:
         _dev(rng_base)
-        if rng_base.numel() != 1 or rng_base.dtype not in (torch.int64, torch.uint64) or rng_base.device != dev:
-            raise ValueError(f"{what}: rng_base must be one int64 / uint64 element on {dev}")
+        if rng_base.numel() != 1 or rng_base.dtype not in (torch.int64, torch.uint64) or rng_base.get_device() != dev:
+            raise ValueError(f"{what}: rng_base must be one int64 / uint64 element on cuda:{dev}")
     if p == 0.0:
-        return 0, 0
+        return 0.0, 0, 0, None
     if rng is None:
-        return RNG.next(n)
-    seed, off = rng
-    return int(seed) & _U64, int(off) & _U64
+        seed, off = RNG.next(n)
+    else:
+        seed, off = rng
+    return p, int(seed) & _U64, int(off) & _U64, rng_base
 
 
-def _mask_args(ctx, p: float, seed: int, offset: int, rng_base: Optional[torch.Tensor], keep: bool):
-    """The mask arguments of a forward's entry point; ctx.mask gets its backward's. With an rng_base, whose value may have
-    moved on by then, the backward adds the offset that the forward's kernel left in `used`."""
-    if rng_base is None or p == 0.0:
-        ctx.mask = (p, seed, offset, None)
+def _mask_args(ctx, mask):
+    """The mask arguments of a forward's entry point; ctx.mask (where there is a backward) gets that one's. With an
+    rng_base, whose value may have moved on by then, the backward adds the offset that the forward's kernel left in
+    ctx.used."""
+    p, seed, offset, base = mask
+    if base is None:
+        if ctx is not None:
+            ctx.mask = (p, seed, offset, None)
         return p, seed, offset, None, None
-    if not keep:
-        return p, seed, offset, rng_base.data_ptr(), None
-    ctx.used = torch.empty(1, dtype=torch.int64, device=rng_base.device)
+    if ctx is None:
+        return p, seed, offset, base.data_ptr(), None
+    ctx.used = torch.empty(1, dtype=torch.int64, device=base.device)
     ctx.mask = (p, seed, 0, ctx.used.data_ptr())
-    return p, seed, offset, rng_base.data_ptr(), ctx.used.data_ptr()
+    return p, seed, offset, base.data_ptr(), ctx.used.data_ptr()
+
+
+def _dropout_forward(ctx, x, mask):
+    x = x.contiguous()
+    y = torch.empty_like(x)
+    _launch(x.get_device(), _C.lib().yanerf_dropout, x.data_ptr(), _TYPES[x.dtype], x.numel(), *_mask_args(ctx, mask),
+            y.data_ptr())
+    return y
 
 
 class _DropoutFn(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, mask):
-        x = x.contiguous()
-        y = torch.empty_like(x)
-        _launch(x.get_device(), _C.lib().yanerf_dropout, x.data_ptr(), _TYPES[x.dtype], x.numel(),
-                *_mask_args(ctx, *mask, ctx.needs_input_grad[0]), y.data_ptr())
-        return y
+        return _dropout_forward(ctx, x, mask)
 
     @staticmethod
     @_once
@@ -576,28 +582,33 @@ def dropout(x: torch.Tensor, p: float, *, rng: Optional[Tuple[int, int]] = None,
     step advances it, so each replay draws another mask; the backward uses the forward's, also if the base has moved)."""
     _dev(x)
     _code_type("dropout", x.dtype)
-    p = _probability("dropout", p)
-    seed, off = _mask_rng("dropout", p, rng, rng_base, x.device, x.numel())
-    return _DropoutFn.apply(x, (p, seed, off, rng_base))
+    mask = _mask("dropout", p, rng, rng_base, x.get_device(), x.numel())
+    if x.requires_grad and torch.is_grad_enabled():
+        return _DropoutFn.apply(x, mask)
+    return _dropout_forward(None, x, mask)
 
 
-_ID_FLAGS: dict = {}  # device -> sticky int32 flag of ids outside their table (set by the lookup's kernel, cleared here)
+_ID_FLAGS: dict = {}  # device index -> sticky int32 flag of ids outside their table (set by the lookup's kernel, cleared
+# where it is reported)
 
 
-def _id_flag(dev) -> Optional[torch.Tensor]:
+def _id_flag(dev: int) -> Optional[int]:
+    """The address of the flag; none yet inside a capture, whose memory is the graph's own."""
     f = _ID_FLAGS.get(dev)
-    if f is None and not torch.cuda.is_current_stream_capturing():  # a capture's memory is the graph's own
-        f = torch.zeros(1, dtype=torch.int32, device=dev)
+    if f is None:
+        if torch.cuda.is_current_stream_capturing():
+            return None
+        f = torch.zeros(1, dtype=torch.int32, device=f"cuda:{dev}")
         torch.cuda.current_stream(dev).synchronize()  # cleared before any stream's lookup can set it
         _ID_FLAGS[dev] = f
-    return f
+    return f.data_ptr()
 
 
 def check_embedding_ids(dev) -> None:
     """Raise if any lookup on `dev` since the last check met an id outside its table (one host read-back for any number
     of lookups; skipped while a stream is being captured into a graph)."""
-    dev = torch.device(dev)
-    f = _ID_FLAGS.get(dev if dev.index is not None else torch.device(dev.type, torch.cuda.current_device()))
+    index = dev if isinstance(dev, int) else torch.device(dev).index
+    f = _ID_FLAGS.get(torch.cuda.current_device() if index is None else index)
     if f is None or torch.cuda.is_current_stream_capturing():
         return
     if int(f.item()):
@@ -605,24 +616,24 @@ def check_embedding_ids(dev) -> None:
         raise IndexError("embedding: an id lies outside its table")
 
 
+def _embedding_forward(ctx, table, ids, scale, mask, out_dtype):
+    V, D = table.shape
+    if D > 1 and table.stride(1) != 1:
+        table = table.contiguous()
+    dev = table.get_device()
+    out = table.new_empty((*ids.shape, D), dtype=out_dtype)
+    _launch(dev, _C.lib().yanerf_embedding_forward, table.data_ptr(), _TYPES[table.dtype], table.stride(0), ids.data_ptr(),
+            ids.element_size(), ids.numel(), V, D, scale, *_mask_args(ctx, mask), out.data_ptr(), _TYPES[out_dtype],
+            _id_flag(dev))
+    return out
+
+
 class _EmbeddingFn(torch.autograd.Function):
     @staticmethod
     def forward(ctx, table, ids, scale, padding_idx, mask, out_dtype):
-        V, D = table.shape
-        if D > 1 and table.stride(1) != 1:
-            table = table.contiguous()
-        ids = ids.contiguous()
-        out = torch.empty(*ids.shape, D, dtype=out_dtype, device=table.device)
-        keep = ctx.needs_input_grad[0]
-        flag = _id_flag(table.device)
-        _launch(table.get_device(), _C.lib().yanerf_embedding_forward, table.data_ptr(), _TYPES[table.dtype],
-                table.stride(0), ids.data_ptr(), ids.element_size(), ids.numel(), V, D, scale,
-                *_mask_args(ctx, *mask, keep), out.data_ptr(), _TYPES[out_dtype],
-                None if flag is None else flag.data_ptr())
-        if keep:
-            ctx.dims = (V, D, table.dtype, scale, padding_idx)
-            ctx.save_for_backward(ids)
-        return out
+        ctx.save_for_backward(ids)
+        ctx.dims = (*table.shape, table.dtype, scale, padding_idx)
+        return _embedding_forward(ctx, table, ids, scale, mask, out_dtype)
 
     @staticmethod
     @_once
@@ -631,11 +642,13 @@ class _EmbeddingFn(torch.autograd.Function):
         (ids,) = ctx.saved_tensors
         N = ids.numel()
         g = g.contiguous()
-        grad = torch.empty(V, D, dtype=dtype, device=g.device)
+        grad = g.new_empty((V, D), dtype=dtype)
         L = _C.lib()
-        ws = torch.empty(L.yanerf_embedding_bwd_workspace_bytes(N, V, D), dtype=torch.uint8, device=g.device)
+        nb = L.yanerf_embedding_bwd_workspace_bytes(N, V, D)
+        ws = g.new_empty(nb, dtype=torch.uint8) if nb else None
         _launch(g.get_device(), L.yanerf_embedding_backward, g.data_ptr(), _TYPES[g.dtype], ids.data_ptr(),
-                ids.element_size(), N, V, D, pad, scale, *ctx.mask, grad.data_ptr(), _TYPES[dtype], ws.data_ptr())
+                ids.element_size(), N, V, D, pad, scale, *ctx.mask, grad.data_ptr(), _TYPES[dtype],
+                ws.data_ptr() if nb else None)
         return grad, None, None, None, None, None
 
 
@@ -648,7 +661,7 @@ def embedding(table: torch.Tensor, ids: torch.Tensor, *, scale: float = 1.0, pad
 
     The gradient of the table sums the rows' gradients in fp32 in an order fixed by the ids (sorted, no float atomics:
     the same bits on every run) and is dense: zeros for rows that no id names and for row `padding_idx` (which may count
-    from the end, as in torch.nn.Embedding).
+    from the end, as in torch.nn.Embedding; its lookup is that of any row).
 
     An id outside [0, V) gives a zero row and sets a flag that `check_embedding_ids` reads back and raises on: here when
     `check` (a host synchronisation; a loop over ids that it made itself passes check=False), never inside a graph
@@ -656,12 +669,15 @@ def embedding(table: torch.Tensor, ids: torch.Tensor, *, scale: float = 1.0, pad
     _dev(table, ids)
     if table.dim() != 2:
         raise ValueError(f"embedding: the table must be [V, D], got {tuple(table.shape)}")
-    out_dtype = table.dtype if out_dtype is None else out_dtype
     _code_type("embedding", table.dtype)
-    _code_type("embedding", out_dtype)
-    if ids.dtype not in (torch.int32, torch.int64):
+    if out_dtype is None:
+        out_dtype = table.dtype
+    else:
+        _code_type("embedding", out_dtype)
+    if ids.dtype is not torch.int64 and ids.dtype is not torch.int32:
         raise TypeError(f"embedding: ids must be int32 or int64, got {ids.dtype}")
-    if ids.device != table.device:
+    dev = table.get_device()
+    if ids.get_device() != dev:
         raise RuntimeError(f"embedding: ids on {ids.device}, table on {table.device}")
     V, D = table.shape
     if V == 0 and ids.numel():
@@ -674,9 +690,12 @@ def embedding(table: torch.Tensor, ids: torch.Tensor, *, scale: float = 1.0, pad
     scale = float(scale)
     if not math.isfinite(scale):
         raise ValueError("embedding: scale is not finite")
-    p = _probability("embedding", dropout)
-    seed, off = _mask_rng("embedding", p, rng, rng_base, table.device, ids.numel() * D)
-    out = _EmbeddingFn.apply(table, ids, scale, pad, (p, seed, off, rng_base), out_dtype)
+    mask = _mask("embedding", dropout, rng, rng_base, dev, ids.numel() * D)
+    ids = ids.contiguous()
+    if table.requires_grad and torch.is_grad_enabled():
+        out = _EmbeddingFn.apply(table, ids, scale, pad, mask, out_dtype)
+    else:
+        out = _embedding_forward(None, table, ids, scale, mask, out_dtype)
     if check:
-        check_embedding_ids(table.device)
+        check_embedding_ids(dev)
     return out
