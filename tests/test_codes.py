@@ -125,6 +125,17 @@ def test_code_table_arguments():
         m(image_ids=torch.tensor([[1]]))
 
 
+def test_fused_trainer_refuses_codes():
+    """The fused trainer runs no feature extractor: a conditional config is refused and not trained without its codes."""
+    from yanerf_amd.train import NeRFTrainer
+    from yanerf_amd.utils.config import Config
+    cfg = Config.fromfile(str(yanerf_boot.PKG_DIR / "configs/nerf/lego.yml")).pipeline
+    cfg.model.latent_dim = 4
+    cfg.feature_extractor = [dict(type="CodeTable", num_codes=100, latent_dim=4)]
+    with pytest.raises(NotImplementedError, match="latent_dim"):
+        NeRFTrainer(cfg, device="cpu")
+
+
 def test_reference_mask_rate():
     """The keep rate of the definition's mask: 2^16 draws at p = 0.3, five standard deviations."""
     k = R.keep_mask(1 << 16, 0.3, 7, 9)

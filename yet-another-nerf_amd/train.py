@@ -283,6 +283,11 @@ class NeRFTrainer:
             if k not in ("loss_rgb_mse", "loss_prev_stage_rgb_mse") or float(v) != 1.0:
                 raise NotImplementedError(f"NeRFTrainer: loss_weights {dict(lw)} (the fused step computes "
                                           f"loss_rgb_mse + loss_prev_stage_rgb_mse); use the registry NeRFPipeline")
+        models = pipeline_cfg["model"]
+        for mc in [models] if isinstance(models, dict) else models:
+            if int(mc.get("latent_dim", 0) or 0) > 0:
+                raise NotImplementedError("NeRFTrainer: latent_dim > 0 (global codes, from a CodeTable or the caller) is "
+                                          "not fused; use the registry NeRFPipeline")
         if float(rs.get("scene_extent", 0.0) or 0.0) > 0.0:
             raise NotImplementedError("NeRFTrainer: scene_extent > 0 (ray_sampler.py:100-110) is not supported")
         if str(rs.get("sampling_mode_training", "mask_sample")) != "mask_sample":
