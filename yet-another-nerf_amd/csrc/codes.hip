@@ -436,11 +436,15 @@ __global__ __launch_bounds__(kScanThreads) void sort_scan_kernel(uint32_t* count
     at += q < part ? sums[q][dig] : 0u;
     total += sums[q][dig];
   }
-#pragma unroll 8
-  for (int64_t t = begin; t < end; ++t) {
-    const uint32_t v = c[t * bins];
-    c[t * bins] = at;
-    at += v;
+  for (int64_t t = begin; t < end; t += 8) {  // loads of 8 before their stores, which the compiler cannot move them past
+    uint32_t v[8];
+#pragma unroll
+    for (int k = 0; k < 8; ++k) v[k] = t + k < end ? c[(t + k) * bins] : 0u;
+#pragma unroll
+    for (int k = 0; k < 8; ++k) {
+      if (t + k < end) c[(t + k) * bins] = at;
+      at += v[k];
+    }
   }
   if (part == 0) totals[blockIdx.x * kScanDigits + dig] = total;
 }
