@@ -29,6 +29,33 @@ def test_entry_points_refuse_host_tensors():
         ops.embedding(torch.zeros(4, 2), torch.zeros(3, dtype=torch.int64))
 
 
+def test_torch_binding_loads_with_the_sources_build_id():
+    m = _C.torch_ops()
+    assert m.build_id() == _C.source_id(_C.TORCH_SOURCES)
+
+
+def test_torch_binding_refusals():
+    """The native checks, on host tensors below the Python entry points: nothing launches."""
+    m = _C.torch_ops()
+    t, i = torch.zeros(6, 4), torch.zeros(3, dtype=torch.int64)
+    for args, exc, msg in [((t[0], i), ValueError, "V, D"), ((t.double(), i), TypeError, "Double"),
+                           ((t, i.short()), TypeError, "int32 or int64"), ((t[:0], i), IndexError, "empty table")]:
+        with pytest.raises(exc, match=msg):
+            m.embedding(*args, 1.0, None, 0.0, 0, 0, None, -1, 0)
+    for kw, msg in [(dict(pad=6), "padding_idx"), (dict(pad=-7), "padding_idx"), (dict(scale=float("inf")), "scale"),
+                    (dict(p=1.5), "probability"), (dict(p=float("nan")), "probability"), (dict(base=t), "rng_base")]:
+        a = dict(scale=1.0, pad=None, p=0.0, base=None)
+        a.update(kw)
+        with pytest.raises(ValueError, match=msg):
+            m.embedding(t, i, a["scale"], a["pad"], a["p"], 0, 0, a["base"], -1, 0)
+    with pytest.raises(TypeError):
+        m.dropout(i, 0.5, 0, 0, None)
+    with pytest.raises(ValueError, match="probability"):
+        m.dropout(t, -0.5, 0, 0, None)
+    with pytest.raises(ValueError, match="rng_base"):
+        m.dropout(t, 0.5, 0, 0, torch.zeros(1, dtype=torch.int64))
+
+
 D16 = ctypes.c_void_p(16)
 
 

@@ -281,12 +281,56 @@ def test_gradient_against_differences(ops):
 
 
 def test_double_backward_is_refused(ops):
-    x = rand(8).requires_grad_()
-    y = ops.dropout(x, 0.5)
-    g = rand(8).requires_grad_()
-    (gx,) = torch.autograd.grad(y, x, g, create_graph=True)
+    x, t, i = rand(8).requires_grad_(), rand(5, 8).requires_grad_(), some_ids(8, 5)
+    for y, leaf in ((ops.dropout(x, 0.5), x), (ops.embedding(t, i), t)):
+        g = torch.randn_like(y, requires_grad=True)
+        with pytest.raises(RuntimeError, match="create_graph"):
+            torch.autograd.grad(y, leaf, g, create_graph=True)
+        (once,) = torch.autograd.grad(y, leaf, g.detach(), create_graph=True)  # nothing to differentiate again
+        assert not once.requires_grad
+
+
+def test_graph_is_freed_and_versions_are_checked(ops):
+    """A second backward through a freed graph and ids changed in place between forward and backward are errors, as for any
+    torch operation; retain_graph allows the first."""
+    t, i = rand(5, 8).requires_grad_(), some_ids(8, 5)
+    y = ops.embedding(t, i)
+    y.sum().backward(retain_graph=True)
+    first = t.grad.clone()
+    y.sum().backward()
+    assert torch.equal(t.grad, 2 * first)
     with pytest.raises(RuntimeError):
-        gx.sum().backward()
+        y.sum().backward()
+    y = ops.embedding(t, i)
+    i.fill_(1)
+    with pytest.raises(RuntimeError, match="modified by an inplace"):
+        y.sum().backward()
+    with torch.no_grad():
+        assert not ops.embedding(t, i).requires_grad and not ops.dropout(t, 0.5).requires_grad
+    z = ops.dropout(ops.embedding(t, i), 0.0)
+    z.sum().backward()
+    assert "Yanerf" in type(z.grad_fn).__name__ or "Yanerf" in z.grad_fn.name()
+
+
+def test_threads(ops):
+    """Lookups and backwards from several Python threads at once."""
+    import threading
+    t, i, g = rand(100, 16).requires_grad_(), some_ids(6000, 100), rand(6000, 16)
+    want = torch.autograd.grad(ops.embedding(t, i, dropout=0.1, rng=(1, 2)), t, g)[0]
+    out = [None] * 4
+
+    def work(k):
+        for _ in range(20):
+            out[k] = torch.autograd.grad(ops.embedding(t, i, dropout=0.1, rng=(1, 2), check=False), t, g)[0]
+        torch.cuda.synchronize()
+
+    threads = [threading.Thread(target=work, args=(k,)) for k in range(4)]
+    for x in threads:
+        x.start()
+    for x in threads:
+        x.join()
+    for o in out:
+        assert torch.equal(o, want)
 
 
 @pytest.mark.parametrize("small_rows", [11, 40])

@@ -7,6 +7,7 @@ from __future__ import annotations
 
 import ctypes
 import hashlib
+import importlib.util
 import os
 from ctypes import POINTER, Structure, c_char_p, c_double, c_float, c_int, c_int32, c_int64, c_uint32, c_uint64, c_void_p
 from pathlib import Path
@@ -17,11 +18,15 @@ LIB_PATH = Path(os.environ.get("YANERF_HIP_LIB", PKG / "libyanerf_hip.so"))
 SOURCES = [PKG / "csrc" / f for f in ("render.hip", "mlp.hip", "codes.hip", "common.hpp")] + [
     PKG.parent / "include" / "yanerf_hip.h", PKG / "csrc" / "Makefile"]
 
+# the autograd nodes of the learned codes (csrc/codes_torch.cpp): torch operations over the library's entry points
+TORCH_LIB_PATH = PKG / "_codes_torch.so"
+TORCH_SOURCES = [PKG / "csrc" / "codes_torch.cpp", PKG.parent / "include" / "yanerf_hip.h", PKG / "csrc" / "Makefile"]
 
-def source_id() -> str:
+
+def source_id(files=SOURCES) -> str:
     """SHA-256 prefix of the HIP sources in this tree (what a library built from them reports as its build id)."""
     h = hashlib.sha256()
-    for f in SOURCES:
+    for f in files:
         h.update(f.read_bytes())
     return h.hexdigest()[:16]
 
@@ -131,6 +136,34 @@ def lib():
                            f"`python -c \"import __graft_entry__ as g; g.build()\"`")
     _lib = L
     return L
+
+
+_torch_ops = None
+
+
+def torch_ops():
+    """Load (once) and return the torch binding of the learned codes, on the entry points of lib(); raise HipError if it is
+    absent or was built from other sources."""
+    global _torch_ops
+    if _torch_ops is not None:
+        return _torch_ops
+    import torch  # noqa: F401  (its libraries have to be loaded first)
+    L = lib()
+    rebuild = "`python -c \"import __graft_entry__ as g; g.build()\"` or `make -C yet-another-nerf_amd/csrc`"
+    if not TORCH_LIB_PATH.exists():
+        raise HipError(f"_codes_torch.so not found at {TORCH_LIB_PATH}; build it with {rebuild}")
+    spec = importlib.util.spec_from_file_location(__package__ + "._codes_torch", TORCH_LIB_PATH)
+    m = importlib.util.module_from_spec(spec)
+    spec.loader.exec_module(m)
+    built, src = m.build_id(), source_id(TORCH_SOURCES)
+    if built != src:
+        raise HipError(f"{TORCH_LIB_PATH} was built from other sources (build id {built}, sources {src}): rebuild it with "
+                       f"{rebuild}")
+    address = lambda fn: ctypes.cast(fn, c_void_p).value
+    m.bind(*(address(fn) for fn in (L.yanerf_last_error, L.yanerf_dropout, L.yanerf_embedding_forward,
+                                    L.yanerf_embedding_bwd_workspace_bytes, L.yanerf_embedding_backward)))
+    _torch_ops = m
+    return m
 
 
 def check(status: int, what: str) -> None:

@@ -342,8 +342,8 @@ __device__ __forceinline__ void store_pair(Pair* to, Pair p) { *(uint64_t*)to = 
 // digit's counts over the tiles, and scatters: a wave ranks equal digits by ballots, so that equal keys keep their order,
 // and a tile's pairs are first put in order in LDS, so that they leave as runs and not one by one. With no more than
 // kFewTiles tiles the scatter reads the counts of all of them itself and the scan's launch is left out. Bound by the
-// ranking's vector instructions (147 a pair of the wave, half the time) and the latency of its LDS counters: 2 M pairs of
-// 300000 rows, two passes of 10 bits: 5.5 + 5.6 + 17 us a pass.
+// ranking's vector instructions (half the time) and the latency of its LDS counters: 2 M pairs of 300000 rows, two passes of
+// 10 bits: 5.3 + 6.2 + 15.6 us a pass.
 constexpr int64_t kFewTiles = 64;
 // lanes and pairs a lane: small tiles while they are few, else 4096 by 8 waves (6.3 M pairs, 1024 bins: 512 x 8 52 us,
 // 256 x 16 55, 1024 x 8 61, 512 x 16 71, 1024 x 16 109)
@@ -456,13 +456,11 @@ __device__ __forceinline__ void wave_fence() {
   __builtin_amdgcn_wave_barrier();
 }
 
-// lanes of this wave whose digit equals this lane's
-template <int BITS>
-__device__ __forceinline__ uint64_t wave_match(uint32_t digit, bool valid) {
+// lanes of this wave whose digit, of `bits` bits, equals this lane's
+__device__ __forceinline__ uint64_t wave_match(uint32_t digit, int bits, bool valid) {
   const uint64_t all = __ballot(valid);
   uint32_t lo = (uint32_t)all, hi = (uint32_t)(all >> 32);
-#pragma unroll
-  for (int b = 0; b < BITS; ++b) {
+  for (int b = 0; b < bits; ++b) {
     const uint64_t bal = __ballot((digit >> b) & 1);
     const uint32_t same = (digit >> b) & 1 ? 0u : ~0u;
     lo &= (uint32_t)bal ^ same;
@@ -481,7 +479,6 @@ __global__ __launch_bounds__(THREADS) void sort_scatter_kernel(Src src, int64_t 
                                                                const uint32_t* counts, int64_t tiles,
                                                                const uint32_t* totals, Dst dst) {
   constexpr int WAVES = THREADS / 64, PER = (BINS + THREADS - 1) / THREADS, TILE = THREADS * ITEMS;
-  constexpr int BITS = BINS == 256 ? 8 : 10;
   __shared__ union {
     uint32_t cnt[WAVES][BINS];  // a wave's count of each digit so far, then its first slot
     uint64_t sorted[TILE];      // the tile in order, once every lane knows its slots
@@ -526,7 +523,7 @@ __global__ __launch_bounds__(THREADS) void sort_scatter_kernel(Src src, int64_t 
   for (int j = 0; j < ITEMS; ++j) {
     const bool valid = mine + j * 64 < N;
     const uint32_t dig = (p[j].key >> shift) & mask;
-    const uint64_t peers = wave_match<BITS>(dig, valid);
+    const uint64_t peers = wave_match(dig, width, valid);
     const uint32_t below = __popcll(peers & ((1ull << lane) - 1));
     const uint32_t before = u.cnt[wave][dig];
     rank[j] = before + below;
@@ -1229,7 +1226,7 @@ __global__ __launch_bounds__(kRunThreads) void run_join_kernel(const Pair* pairs
 // bucket, each wave into its own LDS table of the bucket's rows. Lanes of a wave that hold the same row add one after the
 // other in the order of the lanes, so that the ids alone fix the sums' order. A bucket of more than one tile leaves its
 // tiles' tables to a second launch. Every row of a bucket is written, so the gradient needs no zeros beforehand. 6.3 M ids of
-// 512000 x 2 fp32: count 12, scan 11, partition 48, sums 44, join 7 us (sorting pairs and gathering: 270 us); the partition
+// 512000 x 2 fp32: count 10, scan 11, partition 43, sums 46, join 7 us (sorting pairs and gathering: 270 us); the partition
 // is bound like the sort's scatter, the sums by the turns of the lanes that share a row.
 constexpr int kBucketThreads = 512, kBucketWaves = kBucketThreads / 64;
 constexpr int64_t kBucketTile = 8192;    // positions a workgroup
@@ -1346,7 +1343,7 @@ __global__ __launch_bounds__(kBucketThreads) void bucket_sum_kernel(const uint32
     }
 #pragma unroll
     for (int u = 0; u < U; ++u) {
-      const uint64_t peers = wave_match<11>(slot[u], valid[u]);
+      const uint64_t peers = wave_match(slot[u], b.lrows, valid[u]);
       const int turn = valid[u] ? __popcll(peers & ((1ull << lane) - 1)) : -1;
       for (int now = 0; __ballot(turn >= now); ++now) {
         if (turn == now) {

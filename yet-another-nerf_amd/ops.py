@@ -6,7 +6,6 @@ ROCm device tensors and raises otherwise: there is no CPU/torch fallback for the
 from __future__ import annotations
 
 import ctypes
-import math
 from contextlib import contextmanager
 from dataclasses import dataclass
 from typing import List, Optional, Sequence, Tuple
@@ -479,125 +478,45 @@ def adam_step(params: torch.Tensor, grads: torch.Tensor, exp_avg: torch.Tensor, 
 
 
 # ----------------------------------------------------------------------------------------- learned codes
-# Calls here are short next to their launches, so the checks are written for the host's time: device indices in place of
-# device objects, no autograd node where no gradient is wanted.
+# Their autograd nodes and checks of arguments are native (csrc/codes_torch.cpp): these calls are short next to what a node
+# in Python costs.
 _TYPES = {torch.float32: _C.TYPE_F32, torch.bfloat16: _C.TYPE_BF16, torch.float16: _C.TYPE_F16}
 _U64 = 0xFFFFFFFFFFFFFFFF
 
-_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)  # of a device, without a Stream object (3-14 us)
 
-
-def _launch(dev: int, entry, *args) -> None:
-    """entry(*args, stream) on device `dev` and its current stream, whichever device is current."""
-    if dev != torch.cuda.current_device():
-        with torch.cuda.device(dev):
-            return _launch(dev, entry, *args)
-    if entry(*args, _raw_stream(dev) if _raw_stream is not None else torch.cuda.current_stream(dev).cuda_stream):
-        _C.check(1, entry.__name__)
-
-
-def _once(backward):
-    """once_differentiable for a backward; its wrapper (1.4 us) is entered only where a graph of the backward is asked
-    for (create_graph=True)."""
-    wrapped = torch.autograd.function.once_differentiable(backward)
-
-    def call(ctx, g):
-        return wrapped(ctx, g) if torch.is_grad_enabled() else backward(ctx, g)
-
-    return call
-
-
-def _code_type(what: str, dtype: torch.dtype) -> int:
-    t = _TYPES.get(dtype)
-    if t is None:
-        raise TypeError(f"{what}: element type {dtype} is not supported (float32, bfloat16, float16)")
-    return t
-
-
-def _mask(what: str, p, rng, rng_base: Optional[torch.Tensor], dev: int, n: int):
-    """(p, seed, offset, rng_base) of a dropout mask over n elements, checked; no draw where p is 0."""
-    p = float(p)
-    if not 0.0 <= p <= 1.0:
-        raise ValueError(f"{what}: dropout probability {p} is not in [0, 1]")
-    if rng_base is not None:
-        _dev(rng_base)
-        if rng_base.numel() != 1 or rng_base.dtype not in (torch.int64, torch.uint64) or rng_base.get_device() != dev:
-            raise ValueError(f"{what}: rng_base must be one int64 / uint64 element on cuda:{dev}")
+def _mask_rng(p, rng: Optional[Tuple[int, int]], n: int) -> Tuple[int, int]:
+    """(seed, offset) of a dropout mask over n elements; none is drawn where p is 0."""
     if p == 0.0:
-        return 0.0, 0, 0, None
+        return 0, 0
     if rng is None:
-        seed, off = RNG.next(n)
-    else:
-        seed, off = rng
-    return p, int(seed) & _U64, int(off) & _U64, rng_base
-
-
-def _mask_args(ctx, mask):
-    """The mask arguments of a forward's entry point; ctx.mask (where there is a backward) gets that one's. With an
-    rng_base, whose value may have moved on by then, the backward adds the offset that the forward's kernel left in
-    ctx.used."""
-    p, seed, offset, base = mask
-    if base is None:
-        if ctx is not None:
-            ctx.mask = (p, seed, offset, None)
-        return p, seed, offset, None, None
-    if ctx is None:
-        return p, seed, offset, base.data_ptr(), None
-    ctx.used = torch.empty(1, dtype=torch.int64, device=base.device)
-    ctx.mask = (p, seed, 0, ctx.used.data_ptr())
-    return p, seed, offset, base.data_ptr(), ctx.used.data_ptr()
-
-
-def _dropout_forward(ctx, x, mask):
-    x = x.contiguous()
-    y = torch.empty_like(x)
-    _launch(x.get_device(), _C.lib().yanerf_dropout, x.data_ptr(), _TYPES[x.dtype], x.numel(), *_mask_args(ctx, mask),
-            y.data_ptr())
-    return y
-
-
-class _DropoutFn(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, x, mask):
-        return _dropout_forward(ctx, x, mask)
-
-    @staticmethod
-    @_once
-    def backward(ctx, g):
-        g = g.contiguous()
-        out = torch.empty_like(g)
-        _launch(g.get_device(), _C.lib().yanerf_dropout, g.data_ptr(), _TYPES[g.dtype], g.numel(), *ctx.mask, None,
-                out.data_ptr())
-        return out, None
+        return RNG.next(n)
+    seed, off = rng
+    return int(seed) & _U64, int(off) & _U64
 
 
 def dropout(x: torch.Tensor, p: float, *, rng: Optional[Tuple[int, int]] = None,
             rng_base: Optional[torch.Tensor] = None) -> torch.Tensor:
     """Zero each element of x (float32, bfloat16 or float16, any shape) with probability p and multiply the others by
     1 / (1 - p). The mask is a function of a Philox counter (include/yanerf_hip.h): it is never stored, and the backward
-    draws it again. A dropped element is 0 even where x is infinite or NaN.
+    draws it again. A dropped element is 0 even where x is infinite or NaN. Differentiable once.
 
     rng: the (seed, offset) of the mask; the default takes the next of the module stream, which follows
     torch.manual_seed. rng_base: one int64 element on x's device that is added to offset when the kernel runs (a captured
     step advances it, so each replay draws another mask; the backward uses the forward's, also if the base has moved)."""
     _dev(x)
-    _code_type("dropout", x.dtype)
-    mask = _mask("dropout", p, rng, rng_base, x.get_device(), x.numel())
-    if x.requires_grad and torch.is_grad_enabled():
-        return _DropoutFn.apply(x, mask)
-    return _dropout_forward(None, x, mask)
+    return _C.torch_ops().dropout(x, p, *_mask_rng(p, rng, x.numel()), rng_base)
 
 
 _ID_FLAGS: dict = {}  # device index -> sticky int32 flag of ids outside their table (set by the lookup's kernel, cleared
 # where it is reported)
 
 
-def _id_flag(dev: int) -> Optional[int]:
-    """The address of the flag; none yet inside a capture, whose memory is the graph's own."""
+def _id_flag(dev: int) -> int:
+    """The address of the flag; 0, none, before there is one inside a capture, whose memory is the graph's own."""
     f = _ID_FLAGS.get(dev)
     if f is None:
         if torch.cuda.is_current_stream_capturing():
-            return None
+            return 0
         f = torch.zeros(1, dtype=torch.int32, device=f"cuda:{dev}")
         torch.cuda.current_stream(dev).synchronize()  # cleared before any stream's lookup can set it
         _ID_FLAGS[dev] = f
@@ -616,42 +535,6 @@ def check_embedding_ids(dev) -> None:
         raise IndexError("embedding: an id lies outside its table")
 
 
-def _embedding_forward(ctx, table, ids, scale, mask, out_dtype):
-    V, D = table.shape
-    if D > 1 and table.stride(1) != 1:
-        table = table.contiguous()
-    dev = table.get_device()
-    out = table.new_empty((*ids.shape, D), dtype=out_dtype)
-    _launch(dev, _C.lib().yanerf_embedding_forward, table.data_ptr(), _TYPES[table.dtype], table.stride(0), ids.data_ptr(),
-            ids.element_size(), ids.numel(), V, D, scale, *_mask_args(ctx, mask), out.data_ptr(), _TYPES[out_dtype],
-            _id_flag(dev))
-    return out
-
-
-class _EmbeddingFn(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, table, ids, scale, padding_idx, mask, out_dtype):
-        ctx.save_for_backward(ids)
-        ctx.dims = (*table.shape, table.dtype, scale, padding_idx)
-        return _embedding_forward(ctx, table, ids, scale, mask, out_dtype)
-
-    @staticmethod
-    @_once
-    def backward(ctx, g):
-        V, D, dtype, scale, pad = ctx.dims
-        (ids,) = ctx.saved_tensors
-        N = ids.numel()
-        g = g.contiguous()
-        grad = g.new_empty((V, D), dtype=dtype)
-        L = _C.lib()
-        nb = L.yanerf_embedding_bwd_workspace_bytes(N, V, D)
-        ws = g.new_empty(nb, dtype=torch.uint8) if nb else None
-        _launch(g.get_device(), L.yanerf_embedding_backward, g.data_ptr(), _TYPES[g.dtype], ids.data_ptr(),
-                ids.element_size(), N, V, D, pad, scale, *ctx.mask, grad.data_ptr(), _TYPES[dtype],
-                ws.data_ptr() if nb else None)
-        return grad, None, None, None, None, None
-
-
 def embedding(table: torch.Tensor, ids: torch.Tensor, *, scale: float = 1.0, padding_idx: Optional[int] = None,
               dropout: float = 0.0, out_dtype: Optional[torch.dtype] = None, rng: Optional[Tuple[int, int]] = None,
               rng_base: Optional[torch.Tensor] = None, check: bool = True) -> torch.Tensor:
@@ -661,41 +544,18 @@ def embedding(table: torch.Tensor, ids: torch.Tensor, *, scale: float = 1.0, pad
 
     The gradient of the table sums the rows' gradients in fp32 in an order fixed by the ids (sorted, no float atomics:
     the same bits on every run) and is dense: zeros for rows that no id names and for row `padding_idx` (which may count
-    from the end, as in torch.nn.Embedding; its lookup is that of any row).
+    from the end, as in torch.nn.Embedding; its lookup is that of any row). Differentiable once.
 
     An id outside [0, V) gives a zero row and sets a flag that `check_embedding_ids` reads back and raises on: here when
     `check` (a host synchronisation; a loop over ids that it made itself passes check=False), never inside a graph
     capture."""
     _dev(table, ids)
-    if table.dim() != 2:
-        raise ValueError(f"embedding: the table must be [V, D], got {tuple(table.shape)}")
-    _code_type("embedding", table.dtype)
-    if out_dtype is None:
-        out_dtype = table.dtype
-    else:
-        _code_type("embedding", out_dtype)
-    if ids.dtype is not torch.int64 and ids.dtype is not torch.int32:
-        raise TypeError(f"embedding: ids must be int32 or int64, got {ids.dtype}")
+    kind = -1 if out_dtype is None else _TYPES.get(out_dtype)
+    if kind is None:
+        raise TypeError(f"embedding: element type {out_dtype} is not supported (float32, bfloat16, float16)")
     dev = table.get_device()
-    if ids.get_device() != dev:
-        raise RuntimeError(f"embedding: ids on {ids.device}, table on {table.device}")
-    V, D = table.shape
-    if V == 0 and ids.numel():
-        raise IndexError("embedding: ids into an empty table")
-    pad = -1
-    if padding_idx is not None:
-        if not -V <= padding_idx < V:
-            raise ValueError(f"embedding: padding_idx {padding_idx} is outside a table of {V} rows")
-        pad = int(padding_idx) % V
-    scale = float(scale)
-    if not math.isfinite(scale):
-        raise ValueError("embedding: scale is not finite")
-    mask = _mask("embedding", dropout, rng, rng_base, dev, ids.numel() * D)
-    ids = ids.contiguous()
-    if table.requires_grad and torch.is_grad_enabled():
-        out = _EmbeddingFn.apply(table, ids, scale, pad, mask, out_dtype)
-    else:
-        out = _embedding_forward(None, table, ids, scale, mask, out_dtype)
+    seed, off = (0, 0) if dropout == 0.0 else _mask_rng(dropout, rng, ids.numel() * table.shape[-1])
+    out = _C.torch_ops().embedding(table, ids, scale, padding_idx, dropout, seed, off, rng_base, kind, _id_flag(dev))
     if check:
         check_embedding_ids(dev)
     return out
