@@ -617,12 +617,13 @@ __global__ __launch_bounds__(kRankThreads) void rank_sort_kernel(KeyFromIds<IT> 
   constexpr int R = (int)(kRankMax / kRankThreads);
   for (int k = tid; k < kRankBins * COPIES; k += kRankThreads) next[k] = 0;
   __syncthreads();
-  uint32_t key[R];
+  uint32_t key[R], place[R];  // place: among the pairs of this part of the bin, in whatever order they come
 #pragma unroll
   for (int j = 0; j < R; ++j) key[j] = tid + j * kRankThreads < N ? src.at(tid + j * kRankThreads).key : 0u;
 #pragma unroll
   for (int j = 0; j < R; ++j)
-    if (tid + j * kRankThreads < N) atomicAdd(&next[bins(key[j], tid + j * kRankThreads) * COPIES + copy], 1u);
+    if (tid + j * kRankThreads < N)
+      place[j] = atomicAdd(&next[bins(key[j], tid + j * kRankThreads) * COPIES + copy], 1u);
   __syncthreads();
   uint32_t c[PER], sum = 0, all;
 #pragma unroll
@@ -642,7 +643,7 @@ __global__ __launch_bounds__(kRankThreads) void rank_sort_kernel(KeyFromIds<IT> 
 #pragma unroll
   for (int j = 0; j < R; ++j) {
     const int i = tid + j * kRankThreads;
-    if (i < N) binned[atomicAdd(&next[bins(key[j], i) * COPIES + copy], 1u)] = ((P)key[j] << kIndexBits) | (P)i;
+    if (i < N) binned[next[bins(key[j], i) * COPIES + copy] + place[j]] = ((P)key[j] << kIndexBits) | (P)i;
   }
   __syncthreads();
   const int first = blockIdx.x * kRankTile + (tid >> 6) * kRankItems;
@@ -801,7 +802,7 @@ __device__ __forceinline__ void sum_runs(RunEnds<THREADS, VEC>& ends, const Src&
 // ids, keeps the positions of its own rows in order, sorts them by row, adds their runs and writes zeros to its other
 // rows. The rows come in groups of 2^lgroup neighbours dealt out to the workgroups in turn, so that the low ids, which
 // word frequencies favour, spread over the chip. What it costs is that each workgroup reads every id (from L2). Bound by
-// latency: 1 id of 100 x 32 fp32 4.6 us, 4096 ids of 100 x 48 fp32 11.5 us (a sort, sums and a join: 18 us in three launches).
+// latency: 1 id of 100 x 32 fp32 4.3 us, 4096 ids of 100 x 48 fp32 9.0 us (a sort, sums and a join: 18 us in three launches).
 constexpr int kOwnThreads = 512, kOwnWaves = kOwnThreads / 64;
 constexpr int64_t kOwnMax = 4096;  // ids
 constexpr int64_t kOwnTable = 32ll << 20;  // bytes of the gradient
@@ -885,23 +886,25 @@ __global__ __launch_bounds__(kOwnThreads) void own_rows_kernel(const GT* g, cons
   for (int k = tid; k < (o.slots + 31) / 32; k += kOwnThreads) present[k] = 0;
   if (tid == 0) unsorted = 0;
 
-  // 1. the positions of this owner's rows, in order: count, then place
-  const int span = ((N + kOwnWaves - 1) / kOwnWaves + 63) / 64 * 64;  // a wave's consecutive ids
+  // 1. the positions of this owner's rows, in order: count, then place. A wave holds its consecutive ids in registers.
+  constexpr int B = (int)(kOwnMax / kOwnThreads);
+  const int span = ((N + kOwnWaves - 1) / kOwnWaves + 63) / 64 * 64;
   const int first = wave * span, end = first + span < N ? first + span : N;
-  auto slot_of = [&](int i) -> int64_t {  // -1: not this owner's
-    const int64_t id = id_bytes == 8 ? ((const int64_t*)ids)[i] : (int64_t)((const int32_t*)ids)[i];
-    const int64_t grp = id >> o.lgroup;
-    const bool mine = id >= 0 && id < V && id != pad && ((uint32_t)grp & ((1u << o.lown) - 1)) == owner;
-    return mine ? ((grp >> o.lown) << o.lgroup) + (id & in_group) : -1;
-  };
-  constexpr int B = 8;  // ids in flight a lane
+  int64_t id[B];
+#pragma unroll
+  for (int u = 0; u < B; ++u) {
+    const int i = first + u * 64 + lane;
+    id[u] = i < end ? (id_bytes == 8 ? ((const int64_t*)ids)[i] : (int64_t)((const int32_t*)ids)[i]) : -1;
+  }
+  int64_t slot[B];  // -1: not this owner's
   int count = 0;
-  for (int i0 = first; i0 < end; i0 += 64 * B) {
-    int64_t slot[B];
 #pragma unroll
-    for (int u = 0; u < B; ++u) slot[u] = i0 + u * 64 + lane < end ? slot_of(i0 + u * 64 + lane) : -1;
-#pragma unroll
-    for (int u = 0; u < B; ++u) count += __popcll(__ballot(slot[u] >= 0));
+  for (int u = 0; u < B; ++u) {
+    const int64_t grp = id[u] >> o.lgroup;
+    const bool mine =
+        id[u] >= 0 && id[u] < V && id[u] != pad && ((uint32_t)grp & ((1u << o.lown) - 1)) == owner;
+    slot[u] = mine ? ((grp >> o.lown) << o.lgroup) + (id[u] & in_group) : -1;
+    count += __popcll(__ballot(mine));
   }
   if (lane == 0) wave_count[wave] = count;
   __syncthreads();
@@ -911,22 +914,15 @@ __global__ __launch_bounds__(kOwnThreads) void own_rows_kernel(const GT* g, cons
     at += w < wave ? wave_count[w] : 0;
     M += wave_count[w];
   }
-  if (count) {
-    for (int i0 = first; i0 < end; i0 += 64 * B) {
-      int64_t slot[B];
 #pragma unroll
-      for (int u = 0; u < B; ++u) slot[u] = i0 + u * 64 + lane < end ? slot_of(i0 + u * 64 + lane) : -1;
-#pragma unroll
-      for (int u = 0; u < B; ++u) {
-        const uint64_t mine = __ballot(slot[u] >= 0);
-        if (slot[u] >= 0) {
-          list[at + __popcll(mine & ((1ull << lane) - 1))] =
-              ((uint32_t)slot[u] << kIndexBits) | (uint32_t)(i0 + u * 64 + lane);
-          atomicOr(&present[slot[u] >> 5], 1u << (slot[u] & 31));
-        }
-        at += __popcll(mine);
-      }
+  for (int u = 0; u < B; ++u) {
+    const uint64_t mine = __ballot(slot[u] >= 0);
+    if (slot[u] >= 0) {
+      list[at + __popcll(mine & ((1ull << lane) - 1))] =
+          ((uint32_t)slot[u] << kIndexBits) | (uint32_t)(first + u * 64 + lane);
+      atomicOr(&present[slot[u] >> 5], 1u << (slot[u] & 31));
     }
+    at += __popcll(mine);
   }
   __syncthreads();
 
