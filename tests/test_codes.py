@@ -56,6 +56,17 @@ def test_torch_binding_refusals():
         m.dropout(t, 0.5, 0, 0, torch.zeros(1, dtype=torch.int64))
 
 
+def test_forward_mode_is_refused():
+    import torch.autograd.forward_ad as fwd
+    m = _C.torch_ops()
+    with fwd.dual_level():
+        t = fwd.make_dual(torch.zeros(6, 4), torch.ones(6, 4))
+        with pytest.raises(RuntimeError, match="forward-mode"):
+            m.embedding(t, torch.zeros(3, dtype=torch.int64), 1.0, None, 0.0, 0, 0, None, -1, 0)
+        with pytest.raises(RuntimeError, match="forward-mode"):
+            m.dropout(t, 0.5, 0, 0, None)
+
+
 D16 = ctypes.c_void_p(16)
 
 

@@ -87,7 +87,12 @@ struct Mask {
   uint64_t again_offset() const { return used.defined() ? 0 : offset; }
 };
 
+void refuse_tangent(const char* what, const Tensor& t) {
+  if (t._fw_grad(/*level=*/0).defined())
+    throw std::runtime_error(std::string(what) + ": forward-mode differentiation is not supported");
+}
 void refuse_graph(const char* what, const Tensor& g) {
+  refuse_tangent(what, g);
   if (at::GradMode::is_enabled() && g.requires_grad())
     throw std::runtime_error(std::string(what) + ": a gradient of its gradient (create_graph=True) is not supported");
 }
@@ -119,6 +124,7 @@ Tensor dropout(const Tensor& x, double p, uint64_t seed, uint64_t offset, const 
                          " is not supported (float32, bfloat16, float16)");
   Mask m{p, seed, offset, rng_base, Tensor()};
   m.check("dropout", x);
+  refuse_tangent("dropout", x);
   const bool graph = at::GradMode::is_enabled() && x.requires_grad();
   if (graph) m.keep();
   Tensor y;
@@ -189,6 +195,7 @@ Tensor embedding(const Tensor& table, const Tensor& ids_in, double scale, std::o
   if (!std::isfinite(scale)) throw py::value_error("embedding: scale is not finite");
   Mask m{p, seed, offset, rng_base, Tensor()};
   m.check("embedding", table);
+  refuse_tangent("embedding", table);
   const bool graph = at::GradMode::is_enabled() && table.requires_grad();
   if (graph) m.keep();
   Tensor out, ids;
@@ -225,6 +232,6 @@ Tensor embedding(const Tensor& table, const Tensor& ids_in, double scale, std::o
 PYBIND11_MODULE(_codes_torch, m) {
   m.def("build_id", [] { return YANERF_SRC_SHA; });
   m.def("bind", &bind);
-  m.def("dropout", &dropout);
-  m.def("embedding", &embedding);
+  m.def("dropout", &dropout, py::call_guard<py::gil_scoped_release>());
+  m.def("embedding", &embedding, py::call_guard<py::gil_scoped_release>());
 }

@@ -554,7 +554,7 @@ def embedding(table: torch.Tensor, ids: torch.Tensor, *, scale: float = 1.0, pad
     if kind is None:
         raise TypeError(f"embedding: element type {out_dtype} is not supported (float32, bfloat16, float16)")
     dev = table.get_device()
-    seed, off = (0, 0) if dropout == 0.0 else _mask_rng(dropout, rng, ids.numel() * table.shape[-1])
+    seed, off = (0, 0) if dropout == 0.0 else _mask_rng(dropout, rng, ids.numel() * table.shape[-1] if table.dim() else 1)
     out = _C.torch_ops().embedding(table, ids, scale, padding_idx, dropout, seed, off, rng_base, kind, _id_flag(dev))
     if check:
         check_embedding_ids(dev)
