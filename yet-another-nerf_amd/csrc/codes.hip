@@ -7,7 +7,8 @@
 //
 // keep(e) is 1 where word e % 4 of Philox4x32-10(key = seed, counter = (e / 4, offset)) is at least
 // T = round(p 2^32): forward and backward evaluate it anew, so no mask is stored or read. A dropped element is 0
-// whatever its input holds. Products and sums are fp32; each output is rounded once.
+// whatever its input holds. Sums are fp32, products with f too but the gradient's, which is taken in 64 bits; each output
+// is rounded once more, to its type.
 //
 // The gradient groups the positions of each row with stable sorts, so the terms of a row are added in an order that the ids
 // alone fix: no float atomics, the same bits on every run. Which way depends on the sizes:
@@ -67,8 +68,8 @@ inline Mask make_mask(double p, uint64_t seed, uint64_t offset, const uint64_t* 
   return m;
 }
 
-// 1 / (1 - p), 0 where everything is dropped
-inline double mask_scale(double p, const Mask& m) { return m.mode == 2 ? 0.0 : 1.0 / (1.0 - p); }
+// scale / (1 - p), 0 where everything is dropped
+inline double mask_scale(double scale, double p, const Mask& m) { return m.mode == 2 ? 0.0 : scale / (1.0 - p); }
 
 __device__ __forceinline__ uint64_t mask_offset(const Mask& m) { return m.offset + (m.base ? *m.base : 0ull); }
 
@@ -683,11 +684,16 @@ __device__ __forceinline__ void masked_term(const GT* g, int64_t D, uint32_t pos
   if (m.mode != 0) apply_keep<VEC>(m, off, e, v);
 }
 
+// f * sum. In 64 bits: f is often a simple fraction (32 / 0.9 = 320 / 9), so that sums of few terms give products that lie
+// half a step of bf16 or fp16 from both neighbours, and a factor rounded to fp32 would move them off the half. One product
+// an output element: the kernels' times do not show it.
+__device__ __forceinline__ float scaled(float sum, double f) { return (float)((double)sum * f); }
+
 template <typename TT, int VEC>
-__device__ __forceinline__ void write_row(TT* grad, int64_t D, int64_t row, int64_t d, float f, const float (&acc)[VEC]) {
+__device__ __forceinline__ void write_row(TT* grad, int64_t D, int64_t row, int64_t d, double f, const float (&acc)[VEC]) {
   float v[VEC];
 #pragma unroll
-  for (int k = 0; k < VEC; ++k) v[k] = acc[k] * f;
+  for (int k = 0; k < VEC; ++k) v[k] = scaled(acc[k], f);
   store_vec<TT, VEC, (VEC > 1), false>(grad + row * D + d, v);
 }
 
@@ -706,7 +712,7 @@ struct RunEnds {
 // with the whole of [0, N) never writes.
 template <int THREADS, typename GT, typename TT, int VEC, typename Src>
 __device__ __forceinline__ void sum_runs(RunEnds<THREADS, VEC>& ends, const Src& src, int64_t N, int64_t base, int piece,
-                                         int lg, const GT* g, int64_t D, int64_t d, const Mask& m, uint64_t off, float f,
+                                         int lg, const GT* g, int64_t D, int64_t d, const Mask& m, uint64_t off, double f,
                                          TT* grad, float* heads, float* tails) {
   constexpr int U = 8;
   const int groups = THREADS >> lg, group = threadIdx.x >> lg, sub = threadIdx.x & ((1 << lg) - 1);
@@ -871,7 +877,7 @@ struct OwnList {
 
 template <typename GT, typename TT, int VEC>
 __global__ __launch_bounds__(kOwnThreads) void own_rows_kernel(const GT* g, const void* ids, int id_bytes, int N, int64_t V,
-                                                               int64_t D, int64_t pad, OwnPlan o, Mask m, float f,
+                                                               int64_t D, int64_t pad, OwnPlan o, Mask m, double f,
                                                                TT* grad) {
   extern __shared__ uint32_t shared[];
   __shared__ RunEnds<kOwnThreads, VEC> ends;
@@ -1061,7 +1067,7 @@ __global__ __launch_bounds__(kDenseThreads) void dense_sum_kernel(const GT* g, c
 constexpr int kDenseJoinThreads = 1024;
 template <typename TT>
 __global__ __launch_bounds__(kDenseJoinThreads) void dense_join_kernel(const float* partial, int64_t blocks, int64_t n, int lo,
-                                                                       float f, TT* grad) {
+                                                                       double f, TT* grad) {
   __shared__ float sums[kDenseJoinThreads];
   const int out = threadIdx.x & ((1 << lo) - 1), part = threadIdx.x >> lo, parts = kDenseJoinThreads >> lo;
   const int64_t k = ((int64_t)blockIdx.x << lo) + out;
@@ -1075,7 +1081,7 @@ __global__ __launch_bounds__(kDenseJoinThreads) void dense_join_kernel(const flo
   __syncthreads();
   if (part != 0 || k >= n) return;
   for (int q = 1; q < parts; ++q) s += sums[(q << lo) + out];
-  grad[k] = (TT)(s * f);
+  grad[k] = (TT)scaled(s, f);
 }
 
 // ---- long id lists: the sorted pairs in memory, a workgroup's runs cut by its neighbours' joined in a second launch.
@@ -1142,7 +1148,7 @@ constexpr int kAbsentRows = 1024;
 
 template <typename GT, typename TT, int VEC>
 __global__ __launch_bounds__(kRunThreads) void run_sum_kernel(const GT* g, const Pair* pairs, uint32_t V, int64_t N,
-                                                              int64_t D, RunPlan r, Mask m, float f, TT* grad,
+                                                              int64_t D, RunPlan r, Mask m, double f, TT* grad,
                                                               float* heads, float* tails, int rows, Div dv) {
   __shared__ RunEnds<kRunThreads, VEC> ends;
   __shared__ uint64_t staged[(kRunSpan + 16) / 8 * 9];
@@ -1178,7 +1184,7 @@ __global__ __launch_bounds__(kRunThreads) void run_sum_kernel(const GT* g, const
 // the run that workgroup b of run_sum_kernel started and did not end: its tail and the heads of the workgroups after it
 template <typename TT, int VEC>
 __global__ __launch_bounds__(kRunThreads) void run_join_kernel(const Pair* pairs, int64_t N, uint32_t V, int64_t D,
-                                                               RunPlan r, float f, TT* grad, const float* heads,
+                                                               RunPlan r, double f, TT* grad, const float* heads,
                                                                const float* tails) {
   const int64_t b = blockIdx.x % (uint32_t)r.blocks, next = (b + 1) * r.span;
   if (next >= N) return;
@@ -1290,7 +1296,7 @@ struct BucketTile {
 template <typename GT, typename TT, int DM>
 __global__ __launch_bounds__(kBucketThreads) void bucket_sum_kernel(const uint32_t* keys, const Row<GT, DM>* rows,
                                                                     const uint32_t* totals, BucketPlan b, int64_t V, int D,
-                                                                    float f, TT* grad, float* partial,
+                                                                    double f, TT* grad, float* partial,
                                                                     BucketTile* multi) {
   extern __shared__ float table[];  // [wave][row of the bucket][DM]
   __shared__ uint32_t part[kBucketWaves];
@@ -1362,7 +1368,7 @@ __global__ __launch_bounds__(kBucketThreads) void bucket_sum_kernel(const uint32
     } else {
       const int64_t row = row0 + k / DM;
       const int d = k % DM;
-      if (row < V && d < D) grad[row * D + d] = (TT)(s * f);
+      if (row < V && d < D) grad[row * D + d] = (TT)scaled(s, f);
     }
   }
 }
@@ -1370,7 +1376,7 @@ __global__ __launch_bounds__(kBucketThreads) void bucket_sum_kernel(const uint32
 // buckets of more than one tile: their tiles' tables, added in order; `split` workgroups a bucket
 template <typename TT, int DM>
 __global__ __launch_bounds__(256) void bucket_join_kernel(const float* partial, const BucketTile* multi, BucketPlan b,
-                                                          int split, int64_t V, int D, float f, TT* grad) {
+                                                          int split, int64_t V, int D, double f, TT* grad) {
   __shared__ float sums[256];
   const uint32_t bucket = blockIdx.x / split;
   const BucketTile t = multi[bucket];
@@ -1393,7 +1399,7 @@ __global__ __launch_bounds__(256) void bucket_join_kernel(const float* partial, 
     const int64_t row = ((int64_t)t.bucket << b.lrows) + k / DM;
     const int d = k % DM;
     if (part == 0 && k < floats && row < V && d < D)
-      grad[row * D + d] = (TT)((((sums[out] + sums[64 + out]) + sums[128 + out]) + sums[192 + out]) * f);
+      grad[row * D + d] = (TT)scaled(((sums[out] + sums[64 + out]) + sums[128 + out]) + sums[192 + out], f);
   }
 }
 
@@ -1497,7 +1503,7 @@ inline int sort_ids(const IT* ids, int64_t N, int64_t V, int64_t pad, char* ws, 
 
 template <typename GT, typename TT, int DM, typename IT>
 inline void bucket_gradient(const GT* g, const IT* ids, int64_t N, int64_t V, int64_t D, int64_t pad, const BucketPlan& b,
-                            const Mask& m, float f, TT* grad, char* ws, hipStream_t st) {
+                            const Mask& m, double f, TT* grad, char* ws, hipStream_t st) {
   typedef typename std::conditional<sizeof(GT) == 4, uint32_t, uint16_t>::type E;
   const BucketWs w = bucket_ws(N, b, sizeof(GT));
   uint32_t *counts = (uint32_t*)(ws + w.counts), *totals = (uint32_t*)(ws + w.totals), *keys = (uint32_t*)(ws + w.keys);
@@ -1556,7 +1562,7 @@ int yanerf_dropout(const void* x, int type, int64_t n, double p, uint64_t seed, 
   if (n == 0) return 0;
   YN_CHECK(x && y, "dropout: null pointer");
   const Mask m = make_mask(p, seed, offset, rng_base);
-  const float f = (float)mask_scale(p, m);
+  const float f = (float)mask_scale(1.0, p, m);
   const bool al = aligned(x, 16) && aligned(y, 16), nt = streams_past_cache(n * type_bytes(type));
   with_type(type, [&](auto t) {
     using T = decltype(t);
@@ -1585,7 +1591,7 @@ int yanerf_embedding_forward(const void* table, int table_type, int64_t table_st
   YN_CHECK(table && ids && out, "embedding: null pointer");
   YN_CHECK(table_stride >= 0, "embedding: negative table stride");
   const Mask m = make_mask(p, seed, offset, rng_base);
-  const float f = (float)(scale * mask_scale(p, m));
+  const float f = (float)mask_scale(scale, p, m);
   const int64_t wide = 16 / (type_bytes(table_type) > type_bytes(out_type) ? type_bytes(table_type) : type_bytes(out_type));
   auto fits = [&](int64_t vec) {
     return D % vec == 0 && table_stride % vec == 0 && aligned(table, vec * type_bytes(table_type)) &&
@@ -1658,7 +1664,7 @@ int yanerf_embedding_backward(const void* g, int g_type, const void* ids, int id
   YN_CHECK(N == 0 || (g && ids && (workspace || own_always(N, V, D))), "embedding_backward: null pointer");
   YN_CHECK(aligned(workspace, 16), "embedding_backward: the workspace is not aligned to 16 bytes");
   const Mask m = make_mask(p, seed, offset, rng_base);
-  const float f = (float)(scale * mask_scale(p, m));
+  const double f = mask_scale(scale, p, m);
   hipStream_t st = as_stream(stream);
   char* ws = (char*)workspace;
   if (N == 0) {
