@@ -9,10 +9,13 @@
 #include <torch/csrc/autograd/functions/utils.h>
 #include <torch/csrc/autograd/saved_variable.h>
 #include <torch/csrc/autograd/variable.h>
+#include <torch/csrc/jit/frontend/tracer.h>
 #include <torch/csrc/utils/pybind.h>
 
 #include <ATen/Functions.h>
 #include <c10/core/DeviceGuard.h>
+#include <c10/core/impl/LocalDispatchKeySet.h>
+#include <c10/core/impl/TorchDispatchModeTLS.h>
 #include <c10/hip/HIPStream.h>
 
 #include <cmath>
@@ -87,6 +90,22 @@ struct Mask {
   uint64_t again_offset() const { return used.defined() ? 0 : offset; }
 };
 
+// These calls are no operators of torch's dispatcher: one that records operators sees nothing of them but the allocation of
+// their outputs, and a replay would return memory that nobody wrote. Modes that only watch stay allowed.
+void refuse_recording(const char* what) {
+  using c10::impl::TorchDispatchModeKey;
+  using c10::impl::TorchDispatchModeTLS;
+  const char* by = nullptr;
+  if (torch::jit::tracer::isTracing()) by = "torch.jit.trace";
+  else if (c10::impl::tls_is_dispatch_key_included(c10::DispatchKey::PreDispatch)) by = "a pre-dispatch trace";
+  else if (TorchDispatchModeTLS::any_modes_set()) {
+    if (TorchDispatchModeTLS::get_mode(TorchDispatchModeKey::PROXY)) by = "make_fx";
+    else if (TorchDispatchModeTLS::get_mode(TorchDispatchModeKey::FAKE)) by = "a fake tensor mode";
+    else if (TorchDispatchModeTLS::get_mode(TorchDispatchModeKey::FUNCTIONAL)) by = "a functionalization mode";
+  }
+  if (by) throw std::runtime_error(std::string(what) + ": cannot be recorded by " + by);
+}
+
 void refuse_tangent(const char* what, const Tensor& t) {
   if (t._fw_grad(/*level=*/0).defined())
     throw std::runtime_error(std::string(what) + ": forward-mode differentiation is not supported");
@@ -112,6 +131,7 @@ struct DropoutBackward : Node {
   std::string name() const override { return "YanerfDropoutBackward"; }
   variable_list apply(variable_list&& grads) override {
     if (!grads[0].defined() || !task_should_compute_output(0)) return {Tensor()};
+    refuse_recording("dropout");
     refuse_graph("dropout", grads[0]);
     at::NoGradGuard no_grad;
     return {run_dropout(grads[0].contiguous(), mask, mask.again_offset(), mask.used_ptr(), nullptr)};
@@ -119,6 +139,7 @@ struct DropoutBackward : Node {
 };
 
 Tensor dropout(const Tensor& x, double p, uint64_t seed, uint64_t offset, const std::optional<Tensor>& rng_base) {
+  refuse_recording("dropout");
   if (type_of(x.scalar_type()) < 0)
     throw py::type_error(std::string("dropout: element type ") + c10::toString(x.scalar_type()) +
                          " is not supported (float32, bfloat16, float16)");
@@ -152,6 +173,7 @@ struct EmbeddingBackward : Node {
   void release_variables() override { ids.reset_data(); }
   variable_list apply(variable_list&& grads) override {
     if (!grads[0].defined() || !task_should_compute_output(0)) return {Tensor()};
+    refuse_recording("embedding");
     refuse_graph("embedding", grads[0]);
     at::NoGradGuard no_grad;
     const Tensor i = ids.unpack(), g = grads[0].contiguous();
@@ -172,6 +194,7 @@ struct EmbeddingBackward : Node {
 // out_type: -1 for the table's; flag: address of the device's flag of ids outside their table, or 0
 Tensor embedding(const Tensor& table, const Tensor& ids_in, double scale, std::optional<int64_t> padding_idx, double p,
                  uint64_t seed, uint64_t offset, const std::optional<Tensor>& rng_base, int out_type, uintptr_t flag) {
+  refuse_recording("embedding");
   if (table.dim() != 2)
     throw py::value_error("embedding: the table must be [V, D], got " + std::to_string(table.dim()) + " dimensions");
   const int type = type_of(table.scalar_type());

@@ -479,7 +479,8 @@ def adam_step(params: torch.Tensor, grads: torch.Tensor, exp_avg: torch.Tensor, 
 
 # ----------------------------------------------------------------------------------------- learned codes
 # Their autograd nodes and checks of arguments are native (csrc/codes_torch.cpp): these calls are short next to what a node
-# in Python costs.
+# in Python costs. They are no operators of torch's dispatcher, so recorders (torch.jit.trace, make_fx, fake tensors) are
+# refused: they would see the outputs' allocation only.
 _TYPES = {torch.float32: _C.TYPE_F32, torch.bfloat16: _C.TYPE_BF16, torch.float16: _C.TYPE_F16}
 _U64 = 0xFFFFFFFFFFFFFFFF
 
