@@ -286,6 +286,11 @@ int yanerf_embedding_forward(const void* table, int table_type, int64_t table_st
                              int64_t N, int64_t V, int64_t D, double scale, double p, uint64_t seed, uint64_t offset,
                              const uint64_t* rng_base, uint64_t* rng_used, void* out, int out_type, int* oob,
                              void* stream);
+/* An `oob` that is always there: the address of the library's own flag on the current device, 0 until a lookup sets it. It
+ * lives as long as the library. */
+int yanerf_id_flag(int** flag);
+/* *taken = *flag and *flag = 0 in one exchange on the device, so that no lookup's report between the two is lost. */
+int yanerf_flag_take(int* flag, int* taken, void* stream);
 /* Bytes of yanerf_embedding_backward's workspace (16-byte aligned, its contents need not be set; it may be NULL where
  * they are 0), -1 for sizes out of range. */
 int64_t yanerf_embedding_bwd_workspace_bytes(int64_t N, int64_t V, int64_t D);

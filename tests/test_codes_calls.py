@@ -1,5 +1,8 @@
 """Learned codes on the CPU: calls of the Python entry points that have to be refused, or have to be safe, whatever the
 tensors hold (nothing launches)."""
+import ctypes
+import weakref
+
 import pytest
 import torch
 
@@ -28,3 +31,47 @@ def test_recording_is_refused(how):
     for f in (lambda t: m.dropout(t, 0.5, 0, 0, None), lambda t: m.embedding(t, i, 1.0, None, 0.0, 0, 0, None, -1, 0)):
         with pytest.raises(RuntimeError, match="cannot be recorded"):
             recorders()[how](f)(torch.zeros(6, 4))
+
+
+def test_first_use_of_an_id_flag_by_two_threads(monkeypatch):
+    """Two threads that make their first lookup at once: each address that a lookup gets belongs to memory that stays (here to a
+    tensor that its thread still holds while another thread makes its own)."""
+    import threading
+    from types import SimpleNamespace
+    from yanerf_amd import ops
+    made, meet = [], threading.Barrier(2)
+
+    def zeros(*shape, **kw):
+        t = torch.full(shape, 0, dtype=kw["dtype"])
+        made.append(weakref.ref(t))
+        meet.wait(10)  # both threads have found none
+        return t
+
+    fake = SimpleNamespace(**{k: getattr(torch, k) for k in ("int32", "empty")}, zeros=zeros,
+                           cuda=SimpleNamespace(current_stream=lambda dev: SimpleNamespace(synchronize=lambda: None)))
+    monkeypatch.setattr(ops, "torch", fake)
+    held, done, got = [], threading.Barrier(3), []
+
+    def work():
+        got.append(ops._id_flag(0, own=True))
+        got.append(ops._id_flag(0, own=True))
+        done.wait(10)
+        done.wait(10)
+
+    threads = [threading.Thread(target=work) for _ in range(2)]
+    for t in threads:
+        t.start()
+    done.wait(10)
+    held = [r().data_ptr() for r in made if r() is not None]
+    done.wait(10)
+    for t in threads:
+        t.join()
+    assert len(got) == 4 and len(set(got)) == 2 and set(got) == set(held)
+
+
+def test_flag_c_refusals():
+    L = _C.lib()
+    assert L.yanerf_id_flag(None) == 1 and b"null" in L.yanerf_last_error()
+    p, q = ctypes.c_void_p(16), ctypes.c_void_p(32)
+    for a in ((None, p), (p, None), (p, p)):
+        assert L.yanerf_flag_take(*a, None) == 1 and b"pointers" in L.yanerf_last_error()

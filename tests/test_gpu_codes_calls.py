@@ -24,6 +24,89 @@ def captured(f, before=None):
     return g, out
 
 
+# ------------------------------------------------------------------------------------------- ids outside their table
+def test_flag_of_a_first_lookup_in_a_capture(ops):
+    """Ids outside the table are reported after replays, also if no lookup ran on the device before the capture (the first
+    test of this file)."""
+    table, ids = rand(10, 16), some_ids(50, 10)
+    g, y = captured(lambda: ops.embedding(table, ids, check=False))
+    g.replay()
+    torch.cuda.synchronize()
+    ops.check_embedding_ids(DEV)
+    assert torch.equal(y, table[ids])
+    for bad in (10, -1):
+        ids[7] = bad
+        g.replay()
+        with pytest.raises(IndexError):
+            ops.check_embedding_ids(DEV)
+        ops.check_embedding_ids(DEV)
+        assert not y[7].any()
+
+
+def test_a_checked_lookup_answers_for_its_own_ids(ops):
+    table, good, bad = rand(10, 16), some_ids(5, 10), torch.tensor([3, 10], device=DEV)
+    ops.embedding(table, bad, check=False)
+    ops.embedding(table, good)  # another caller's ids are no error of this call
+    with pytest.raises(IndexError):
+        ops.embedding(table, bad)
+    with pytest.raises(IndexError):  # and its report does not take theirs away
+        ops.check_embedding_ids(DEV)
+    ops.check_embedding_ids(DEV)
+    ops.embedding(table, good)
+    s = torch.cuda.Stream()
+    for _ in range(3):  # on several streams in turn
+        with torch.cuda.stream(s):
+            with pytest.raises(IndexError):
+                ops.embedding(table, bad)
+            ops.embedding(table, good)
+        ops.embedding(table, good)
+        with pytest.raises(IndexError):
+            ops.embedding(table, bad)
+    ops.check_embedding_ids(DEV)
+
+
+def test_id_flag_under_inference_mode(ops):
+    table, bad = rand(10, 16), torch.tensor([3, 10], device=DEV)
+    for check in (True, False):
+        with torch.inference_mode():
+            with pytest.raises(IndexError):
+                ops.embedding(table, bad, check=check)
+                ops.check_embedding_ids(DEV)
+        with pytest.raises(IndexError):
+            ops.embedding(table, bad, check=check)
+            ops.check_embedding_ids(DEV)
+        ops.check_embedding_ids(DEV)
+        ops.embedding(table, some_ids(5, 10))
+
+
+def test_id_flags_of_threads(ops):
+    """Checked lookups of several threads at once, half of them with a bad id: each raises for its own and for no other."""
+    import threading
+    table, good, bad = rand(100, 16), some_ids(6000, 100), some_ids(6000, 100)
+    bad[-1] = 100
+    torch.cuda.synchronize()
+    wrong = []
+
+    def work(k):
+        with torch.cuda.stream(torch.cuda.Stream()):
+            for _ in range(50):
+                try:
+                    ops.embedding(table, bad if k % 2 else good)
+                    raised = False
+                except IndexError:
+                    raised = True
+                if raised != bool(k % 2):
+                    wrong.append(k)
+
+    threads = [threading.Thread(target=work, args=(k,)) for k in range(4)]
+    for x in threads:
+        x.start()
+    for x in threads:
+        x.join()
+    assert not wrong
+    ops.check_embedding_ids(DEV)
+
+
 # ------------------------------------------------------------------------------------------- recorders
 def test_recording_is_refused(ops):
     """A recorder sees the allocation of the output and not the kernel, so its replay would return unwritten memory."""

@@ -47,7 +47,7 @@ EXPORTS = (
     "yanerf_composite_train", "yanerf_sample_pdf",
     "yanerf_refine", "yanerf_rgb_loss", "yanerf_adam", "yanerf_adam_scalars", "yanerf_adam_table", "yanerf_step_advance",
     "yanerf_scatter_rays", "yanerf_dropout", "yanerf_embedding_forward", "yanerf_embedding_bwd_workspace_bytes",
-    "yanerf_embedding_backward",
+    "yanerf_embedding_backward", "yanerf_id_flag", "yanerf_flag_take",
 )
 
 
@@ -121,6 +121,8 @@ def lib():
         "yanerf_dropout": (c_int, [P, c_int, i64, c_double, c_uint64, c_uint64, P, P, P, P]),
         "yanerf_embedding_forward": (c_int, [P, c_int, i64, P, c_int, i64, i64, i64, c_double, c_double, c_uint64,
                                              c_uint64, P, P, P, c_int, P, P]),
+        "yanerf_id_flag": (c_int, [POINTER(P)]),
+        "yanerf_flag_take": (c_int, [P, P, P]),
         "yanerf_embedding_bwd_workspace_bytes": (i64, [i64, i64, i64]),
         "yanerf_embedding_backward": (c_int, [P, c_int, P, c_int, i64, i64, i64, i64, c_double, c_double, c_uint64,
                                               c_uint64, P, P, c_int, P, P]),

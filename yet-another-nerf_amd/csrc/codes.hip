@@ -215,6 +215,20 @@ __global__ __launch_bounds__(256) void dropout_kernel(const T* x, T* y, int64_t 
   }
 }
 
+// ------------------------------------------------------------------------------------------ flags
+// The flag of ids outside their table that lookups without one of their own set: a variable of the library and not an
+// allocation, so that it is there, cleared, before the first lookup (also where that one is captured into a graph) and never
+// moves.
+__device__ int id_flag = 0;
+
+// lookups on other streams may set a flag while it is taken
+__device__ __forceinline__ void set_flag(int* flag) {
+  __hip_atomic_store(flag, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+}
+__global__ void take_flag_kernel(int* flag, int* taken) {
+  *taken = __hip_atomic_exchange(flag, 0, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+}
+
 // ------------------------------------------------------------------------------------------ lookup
 // A workgroup takes `rows` consecutive ids. Rows of whole vectors: lane t of the tile's rows * D / VEC vectors copies one,
 // kUnroll of them in flight (1, 2 and 8 measured the same or up to 10 % slower). The ids and hot rows come from L1 / L2, so
@@ -251,7 +265,7 @@ __global__ __launch_bounds__(256) void embedding_rows_of_vectors_kernel(const TT
 #pragma unroll
             for (int k = 0; k < VEC; ++k) v[u][k] *= f;
           } else {
-            if (oob) *oob = 1;
+            if (oob) set_flag(oob);
 #pragma unroll
             for (int k = 0; k < VEC; ++k) v[u][k] = 0.0f;
           }
@@ -289,7 +303,7 @@ __global__ __launch_bounds__(256) void embedding_any_rows_kernel(const TT* table
         if (t + k < total) {
           const int64_t id = (int64_t)ids[n0 + r];
           if (id >= 0 && id < V) v[k] = (float)table[id * stride + c] * f;
-          else if (oob) *oob = 1;
+          else if (oob) set_flag(oob);
         }
         if (++c == dd.d) {
           c = 0;
@@ -1627,6 +1641,22 @@ int yanerf_embedding_forward(const void* table, int table_type, int64_t table_st
     });
   });
   YN_LAUNCH_CHECK("embedding");
+  return 0;
+}
+
+int yanerf_id_flag(int** flag) {
+  YN_CHECK(flag, "id_flag: null pointer");
+  void* p = nullptr;
+  const hipError_t e = hipGetSymbolAddress(&p, HIP_SYMBOL(id_flag));
+  YN_CHECK(e == hipSuccess, "id_flag: %s", hipGetErrorString(e));
+  *flag = (int*)p;
+  return 0;
+}
+
+int yanerf_flag_take(int* flag, int* taken, void* stream) {
+  YN_CHECK(flag && taken && flag != taken, "flag_take: null or equal pointers");
+  hipLaunchKernelGGL(take_flag_kernel, dim3(1), dim3(1), 0, as_stream(stream), flag, taken);
+  YN_LAUNCH_CHECK("flag_take");
   return 0;
 }
 

@@ -6,6 +6,7 @@ ROCm device tensors and raises otherwise: there is no CPU/torch fallback for the
 from __future__ import annotations
 
 import ctypes
+import threading
 from contextlib import contextmanager
 from dataclasses import dataclass
 from typing import List, Optional, Sequence, Tuple
@@ -508,31 +509,50 @@ def dropout(x: torch.Tensor, p: float, *, rng: Optional[Tuple[int, int]] = None,
     return _C.torch_ops().dropout(x, p, *_mask_rng(p, rng, x.numel()), rng_base)
 
 
-_ID_FLAGS: dict = {}  # device index -> sticky int32 flag of ids outside their table (set by the lookup's kernel, cleared
-# where it is reported)
+_ID_FLAGS: dict = {}  # device index -> address of the library's flag there, for lookups that are not checked at once
+_OWN_FLAGS = threading.local()  # a thread's flags (device index -> int32 tensor) for those that are: they answer for their own
+# ids, whatever other threads look up meanwhile
 
 
-def _id_flag(dev: int) -> int:
-    """The address of the flag; 0, none, before there is one inside a capture, whose memory is the graph's own."""
-    f = _ID_FLAGS.get(dev)
-    if f is None:
-        if torch.cuda.is_current_stream_capturing():
-            return 0
-        f = torch.zeros(1, dtype=torch.int32, device=f"cuda:{dev}")
-        torch.cuda.current_stream(dev).synchronize()  # cleared before any stream's lookup can set it
-        _ID_FLAGS[dev] = f
-    return f.data_ptr()
+def _id_flag(dev: int, own: bool) -> int:
+    """The address of the flag that a lookup on device `dev` sets."""
+    if own:
+        f = _OWN_FLAGS.__dict__.get(dev)
+        if f is None:
+            f = torch.zeros(1, dtype=torch.int32, device=f"cuda:{dev}")
+            torch.cuda.current_stream(dev).synchronize()  # cleared before a lookup on any stream can set it
+            _OWN_FLAGS.__dict__[dev] = f
+        return f.data_ptr()
+    address = _ID_FLAGS.get(dev)
+    if address is None:
+        p = ctypes.c_void_p()
+        with torch.cuda.device(dev):
+            _C.check(_C.lib().yanerf_id_flag(ctypes.byref(p)), "yanerf_id_flag")
+        address = _ID_FLAGS[dev] = p.value
+    return address
+
+
+def _take_flag(dev: int, address: int) -> int:
+    """The flag's value, read and cleared at once (synchronises the current stream)."""
+    taken = torch.empty(1, dtype=torch.int32, device=f"cuda:{dev}")
+    with torch.cuda.device(dev):
+        _C.check(_C.lib().yanerf_flag_take(ctypes.c_void_p(address), _p(taken), _stream()), "yanerf_flag_take")
+    return int(taken.item())
+
+
+def _capturing(dev: int) -> bool:
+    with torch.cuda.device(dev):
+        return torch.cuda.is_current_stream_capturing()
 
 
 def check_embedding_ids(dev) -> None:
-    """Raise if any lookup on `dev` since the last check met an id outside its table (one host read-back for any number
-    of lookups; skipped while a stream is being captured into a graph)."""
+    """Raise if a lookup on `dev` with check=False, or a replayed one, has met an id outside its table since the last check
+    (one host read-back for any number of lookups; skipped while the stream is being captured into a graph). It sees the
+    lookups that `dev`'s current stream is ordered behind; a report of one that still runs on another stream is left for the
+    next check."""
     index = dev if isinstance(dev, int) else torch.device(dev).index
-    f = _ID_FLAGS.get(torch.cuda.current_device() if index is None else index)
-    if f is None or torch.cuda.is_current_stream_capturing():
-        return
-    if int(f.item()):
-        f.zero_()
+    index = torch.cuda.current_device() if index is None else index
+    if not _capturing(index) and _take_flag(index, _id_flag(index, False)):
         raise IndexError("embedding: an id lies outside its table")
 
 
@@ -547,16 +567,19 @@ def embedding(table: torch.Tensor, ids: torch.Tensor, *, scale: float = 1.0, pad
     the same bits on every run) and is dense: zeros for rows that no id names and for row `padding_idx` (which may count
     from the end, as in torch.nn.Embedding; its lookup is that of any row). Differentiable once.
 
-    An id outside [0, V) gives a zero row and sets a flag that `check_embedding_ids` reads back and raises on: here when
-    `check` (a host synchronisation; a loop over ids that it made itself passes check=False), never inside a graph
-    capture."""
+    An id outside [0, V) gives a zero row. With `check` the call raises then (a host synchronisation; a loop over ids that
+    it made itself passes check=False). Without it, and inside a graph capture, it sets a flag of the device that
+    `check_embedding_ids` reads back and raises on."""
     _dev(table, ids)
     kind = -1 if out_dtype is None else _TYPES.get(out_dtype)
     if kind is None:
         raise TypeError(f"embedding: element type {out_dtype} is not supported (float32, bfloat16, float16)")
     dev = table.get_device()
     seed, off = (0, 0) if dropout == 0.0 else _mask_rng(dropout, rng, ids.numel() * table.shape[-1] if table.dim() else 1)
-    out = _C.torch_ops().embedding(table, ids, scale, padding_idx, dropout, seed, off, rng_base, kind, _id_flag(dev))
-    if check:
-        check_embedding_ids(dev)
+    check = check and not _capturing(dev)
+    flag = _id_flag(dev, own=check)
+    out = _C.torch_ops().embedding(table, ids, scale, padding_idx, dropout, seed, off, rng_base, kind, flag)
+    if check and int(_OWN_FLAGS.__dict__[dev].item()):
+        _take_flag(dev, flag)
+        raise IndexError("embedding: an id lies outside its table")
     return out
