@@ -139,3 +139,31 @@ def test_watching_is_allowed(ops):
         y = f()
         (gt,) = torch.autograd.grad(y.sum(), t)
     assert torch.equal(y, want) and torch.equal(gt, gw)
+
+
+# ------------------------------------------------------------------------------------------- views
+def test_negative_views(ops):
+    """Views whose values are the negated memory (the imaginary part of a conjugate), as inputs and as gradients: contiguous
+    ones too, which contiguous() hands back as they are."""
+    for n in (1, 64):
+        x = torch.randn(n, dtype=torch.complex64, device=DEV).conj().imag
+        if n == 1:
+            assert x.is_neg() and x.is_contiguous()
+        want = R.dropout(x, 0.25, (1, 2))
+        R.assert_within(ops.dropout(x, 0.25, rng=(1, 2)), *want)
+    v = torch._neg_view(rand(40, 24))
+    assert v.is_neg() and v.is_contiguous()
+    R.assert_within(ops.dropout(v, 0.25, rng=(1, 2)), *R.dropout(v, 0.25, (1, 2)))
+    ids = some_ids(300, 40)
+    R.assert_within(ops.embedding(v, ids), *R.lookup(v, ids, F32))
+    R.assert_within(ops.embedding(v[:, ::2], ids), *R.lookup(v[:, ::2], ids, F32))
+    nid = torch._neg_view(-ids)
+    assert nid.is_neg()
+    leaf, x = rand(40, 24).requires_grad_(), rand(300, 24).requires_grad_()
+    assert torch.equal(ops.embedding(leaf, nid), leaf[ids])
+    g = torch._neg_view(rand(300, 24, seed=5))
+    for i in (ids, nid):
+        (gt,) = torch.autograd.grad(ops.embedding(leaf, i), leaf, g)
+        R.assert_within(gt, *R.table_gradient(g, ids, 40, F32))
+    (gx,) = torch.autograd.grad(ops.dropout(x, 0.25, rng=(1, 2)), x, g)
+    R.assert_within(gx, *R.dropout(g, 0.25, (1, 2)))

@@ -76,7 +76,7 @@ struct Mask {
     if (!(p >= 0.0 && p <= 1.0))
       throw py::value_error(std::string(what) + ": dropout probability " + std::to_string(p) + " is not in [0, 1]");
     if (!base) return;
-    if (!base->is_cuda() || base->device() != like.device() || base->numel() != 1 ||
+    if (!base->is_cuda() || base->device() != like.device() || base->numel() != 1 || base->is_neg() ||
         (base->scalar_type() != at::kLong && base->scalar_type() != at::kUInt64))
       throw py::value_error(std::string(what) + ": rng_base must be one int64 / uint64 element on " +
                             like.device().str());
@@ -116,6 +116,9 @@ void refuse_graph(const char* what, const Tensor& g) {
     throw std::runtime_error(std::string(what) + ": a gradient of its gradient (create_graph=True) is not supported");
 }
 
+// Its values in memory: contiguous() hands a contiguous view whose values are the negated memory back as it is
+Tensor resolved(const Tensor& t) { return t.resolve_neg().contiguous(); }
+
 // ------------------------------------------------------------------------------------------ dropout
 Tensor run_dropout(const Tensor& x, const Mask& m, uint64_t offset, const uint64_t* base, uint64_t* used) {
   Tensor y = at::empty(x.sizes(), x.options());
@@ -134,7 +137,7 @@ struct DropoutBackward : Node {
     refuse_recording("dropout");
     refuse_graph("dropout", grads[0]);
     at::NoGradGuard no_grad;
-    return {run_dropout(grads[0].contiguous(), mask, mask.again_offset(), mask.used_ptr(), nullptr)};
+    return {run_dropout(resolved(grads[0]), mask, mask.again_offset(), mask.used_ptr(), nullptr)};
   }
 };
 
@@ -151,7 +154,7 @@ Tensor dropout(const Tensor& x, double p, uint64_t seed, uint64_t offset, const 
   Tensor y;
   {
     at::NoGradGuard no_grad;
-    y = run_dropout(x.contiguous(), m, m.offset, m.base_ptr(), m.used_ptr());
+    y = run_dropout(resolved(x), m, m.offset, m.base_ptr(), m.used_ptr());
   }
   if (graph) {
     auto node = std::shared_ptr<DropoutBackward>(new DropoutBackward(), torch::autograd::deleteNode);
@@ -176,7 +179,7 @@ struct EmbeddingBackward : Node {
     refuse_recording("embedding");
     refuse_graph("embedding", grads[0]);
     at::NoGradGuard no_grad;
-    const Tensor i = ids.unpack(), g = grads[0].contiguous();
+    const Tensor i = ids.unpack(), g = resolved(grads[0]);
     const int64_t N = i.numel(), bytes = api.workspace(N, V, D);
     if (bytes < 0) done(1, "yanerf_embedding_bwd_workspace_bytes");
     Tensor grad = at::empty({V, D}, g.options().dtype(type));
@@ -224,8 +227,8 @@ Tensor embedding(const Tensor& table, const Tensor& ids_in, double scale, std::o
   Tensor out, ids;
   {
     at::NoGradGuard no_grad;
-    const Tensor t = D > 1 && table.stride(1) != 1 ? table.contiguous() : table;
-    ids = ids_in.contiguous();
+    const Tensor t = D > 1 && table.stride(1) != 1 ? resolved(table) : table.resolve_neg();
+    ids = resolved(ids_in);
     c10::SmallVector<int64_t, 6> shape(ids.sizes().begin(), ids.sizes().end());
     shape.push_back(D);
     out = at::empty(shape, t.options().dtype(out_type < 0 ? table.scalar_type() : scalar_of(out_type)));
