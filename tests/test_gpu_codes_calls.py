@@ -167,3 +167,58 @@ def test_negative_views(ops):
         R.assert_within(gt, *R.table_gradient(g, ids, 40, F32))
     (gx,) = torch.autograd.grad(ops.dropout(x, 0.25, rng=(1, 2)), x, g)
     R.assert_within(gx, *R.dropout(g, 0.25, (1, 2)))
+
+
+# ------------------------------------------------------------------------------------------- masks in captures
+def test_default_masks_are_refused_in_a_capture(ops):
+    """The module stream's draw is the host's: captured, every replay would drop the same elements."""
+    x, t, i = rand(500), rand(50, 8), some_ids(300, 50)
+    ops.dropout(x, 0.5), ops.embedding(t, i, dropout=0.5)
+    base = torch.zeros(1, dtype=torch.int64, device=DEV)
+    for f in (lambda **kw: ops.dropout(x, 0.5, **kw), lambda **kw: ops.embedding(t, i, dropout=0.5, check=False, **kw)):
+        before = ops.RNG.get_state()
+        with pytest.raises(RuntimeError, match="rng_base"):
+            captured(f)
+        assert ops.RNG.get_state() == before  # and drew nothing
+        g, y = captured(lambda: f(rng_base=base))
+        seen = []
+        for k in range(3):
+            base.fill_(k << 32)
+            g.replay()
+            torch.cuda.synchronize()
+            seen.append(y.clone())
+        assert not torch.equal(seen[0], seen[1]) and not torch.equal(seen[1], seen[2])
+        g, y = captured(lambda: f(rng=(1, 2)))  # one mask for all replays, by the caller's word
+        g.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(y, f(rng=(1, 2)))
+    captured(lambda: (ops.dropout(x, 0.0), ops.embedding(t, i, check=False)))
+
+
+def test_code_table_in_a_capture(ops):
+    """A CodeTable with dropout in training mode wants an rng_base in a capture, and each replay then draws another mask; the
+    gradient is that of the mask drawn."""
+    from yanerf_amd.pipelines.feature_extractors import FEATURE_EXTRACTORS
+    m = FEATURE_EXTRACTORS.build(dict(type="CodeTable", num_codes=50, latent_dim=8, dropout=0.5, init_std=1.0)).to(DEV)
+    ids, base = some_ids(300, 50), torch.zeros(1, dtype=torch.int64, device=DEV)
+    m(image_ids=ids)
+    with pytest.raises(RuntimeError, match="rng_base"):
+        captured(lambda: m(image_ids=ids))
+    seed, off = ops.RNG.get_state()
+
+    def step():
+        y = m(image_ids=ids, rng_base=base)["global_codes"]
+        return y.detach(), torch.autograd.grad(y, m.table, torch.ones_like(y))[0]
+
+    g, (y, gt) = captured(step)
+    masks = []
+    for k in range(3):
+        base.fill_(k << 32)
+        g.replay()
+        torch.cuda.synchronize()
+        R.assert_within(y, *R.lookup(m.table, ids, F32, 1.0, 0.5, (seed, off + (k << 32))))
+        R.assert_within(gt, *R.table_gradient(torch.ones_like(y), ids, 50, F32, 1.0, 0.5, (seed, off + (k << 32))))
+        masks.append(y != 0)
+    assert not torch.equal(masks[0], masks[1]) and not torch.equal(masks[1], masks[2])
+    m.eval()
+    captured(lambda: m(image_ids=ids))

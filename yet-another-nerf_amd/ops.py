@@ -486,14 +486,24 @@ _TYPES = {torch.float32: _C.TYPE_F32, torch.bfloat16: _C.TYPE_BF16, torch.float1
 _U64 = 0xFFFFFFFFFFFFFFFF
 
 
-def _mask_rng(p, rng: Optional[Tuple[int, int]], n: int) -> Tuple[int, int]:
+def _mask_rng(what: str, p, rng: Optional[Tuple[int, int]], rng_base: Optional[torch.Tensor], n: int,
+              dev: int) -> Tuple[int, int]:
     """(seed, offset) of a dropout mask over n elements; none is drawn where p is 0."""
     if p == 0.0:
         return 0, 0
     if rng is None:
+        if rng_base is None and p < 1.0 and _capturing(dev):
+            raise RuntimeError(f"{what}: captured into a graph, the module stream's draw would be the same mask in every "
+                               "replay; pass an rng_base that the program advances between replays (or an rng, where one "
+                               "mask is meant)")
         return RNG.next(n)
     seed, off = rng
     return int(seed) & _U64, int(off) & _U64
+
+
+def _capturing(dev: int) -> bool:
+    with torch.cuda.device(dev):
+        return torch.cuda.is_current_stream_capturing()
 
 
 def dropout(x: torch.Tensor, p: float, *, rng: Optional[Tuple[int, int]] = None,
@@ -504,9 +514,10 @@ def dropout(x: torch.Tensor, p: float, *, rng: Optional[Tuple[int, int]] = None,
 
     rng: the (seed, offset) of the mask; the default takes the next of the module stream, which follows
     torch.manual_seed. rng_base: one int64 element on x's device that is added to offset when the kernel runs (a captured
-    step advances it, so each replay draws another mask; the backward uses the forward's, also if the base has moved)."""
+    step advances it, so each replay draws another mask; the backward uses the forward's, also if the base has moved). A
+    graph capture wants one of the two: the module stream's draw, made once on the host, would be every replay's."""
     _dev(x)
-    return _C.torch_ops().dropout(x, p, *_mask_rng(p, rng, x.numel()), rng_base)
+    return _C.torch_ops().dropout(x, p, *_mask_rng("dropout", p, rng, rng_base, x.numel(), x.get_device()), rng_base)
 
 
 _ID_FLAGS: dict = {}  # device index -> address of the library's flag there, for lookups that are not checked at once
@@ -540,11 +551,6 @@ def _take_flag(dev: int, address: int) -> int:
     return int(taken.item())
 
 
-def _capturing(dev: int) -> bool:
-    with torch.cuda.device(dev):
-        return torch.cuda.is_current_stream_capturing()
-
-
 def check_embedding_ids(dev) -> None:
     """Raise if a lookup on `dev` with check=False, or a replayed one, has met an id outside its table since the last check
     (one host read-back for any number of lookups; skipped while the stream is being captured into a graph). It sees the
@@ -575,7 +581,8 @@ def embedding(table: torch.Tensor, ids: torch.Tensor, *, scale: float = 1.0, pad
     if kind is None:
         raise TypeError(f"embedding: element type {out_dtype} is not supported (float32, bfloat16, float16)")
     dev = table.get_device()
-    seed, off = (0, 0) if dropout == 0.0 else _mask_rng(dropout, rng, ids.numel() * table.shape[-1] if table.dim() else 1)
+    seed, off = (0, 0) if dropout == 0.0 else _mask_rng("embedding", dropout, rng, rng_base,
+                                                        ids.numel() * table.shape[-1] if table.dim() else 1, dev)
     check = check and not _capturing(dev)
     flag = _id_flag(dev, own=check)
     out = _C.torch_ops().embedding(table, ids, scale, padding_idx, dropout, seed, off, rng_base, kind, flag)

@@ -19,7 +19,8 @@ class CodeTable(torch.nn.Module):
 
     num_codes, latent_dim: the table. scale: multiplies the codes (and their gradient). dropout: probability of dropping
     an entry of a code in training mode (module.train()); evaluation looks the codes up as they are. padding_idx: a row
-    that stays as it is (it starts at zero). Rows start as N(0, init_std)."""
+    that stays as it is (it starts at zero). Rows start as N(0, init_std). A step that is captured into a graph with dropout
+    passes `rng_base` (ops.dropout) beside the ids."""
 
     def __init__(self, num_codes: int, latent_dim: int, scale: float = 1.0, dropout: float = 0.0,
                  padding_idx: Optional[int] = None, init_std: float = 0.01, ids_key: str = "image_ids"):
@@ -50,5 +51,6 @@ class CodeTable(torch.nn.Module):
             raise IndexError(f"CodeTable: an id lies outside {self.num_codes} codes")
         ids = ids.to(self.table.device, torch.int64)
         codes = ops.embedding(self.table, ids, scale=self.scale, padding_idx=self.padding_idx,
-                              dropout=self.dropout if self.training else 0.0, check=not on_host)
+                              dropout=self.dropout if self.training else 0.0, rng_base=kwargs.get("rng_base"),
+                              check=not on_host)
         return {"global_codes": codes}
