@@ -75,3 +75,20 @@ def test_flag_c_refusals():
     p, q = ctypes.c_void_p(16), ctypes.c_void_p(32)
     for a in ((None, p), (p, None), (p, p)):
         assert L.yanerf_flag_take(*a, None) == 1 and b"pointers" in L.yanerf_last_error()
+
+
+def test_binding_of_another_torch_is_refused(monkeypatch, tmp_path):
+    """The binding uses torch's C++ ABI: one built against another version does not run, whatever its sources were."""
+    assert _C.torch_ops().torch_version() == torch.__version__
+    monkeypatch.setattr(_C, "_torch_ops", None)
+    with monkeypatch.context() as m:
+        m.setattr(torch, "__version__", "1.0.0")
+        with pytest.raises(_C.HipError, match="built against torch"):
+            _C.torch_ops()
+    with monkeypatch.context() as m:
+        other = tmp_path / "_codes_torch.so"
+        other.write_bytes(b"not a library of this torch")
+        m.setattr(_C, "TORCH_LIB_PATH", other)
+        with pytest.raises(_C.HipError, match="does not load"):
+            _C.torch_ops()
+    assert _C.torch_ops().torch_version() == torch.__version__

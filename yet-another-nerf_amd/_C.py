@@ -145,22 +145,28 @@ _torch_ops = None
 
 def torch_ops():
     """Load (once) and return the torch binding of the learned codes, on the entry points of lib(); raise HipError if it is
-    absent or was built from other sources."""
+    absent, was built from other sources or against another version of torch."""
     global _torch_ops
     if _torch_ops is not None:
         return _torch_ops
-    import torch  # noqa: F401  (its libraries have to be loaded first)
+    import torch  # (its libraries have to be loaded first)
     L = lib()
     rebuild = "`python -c \"import __graft_entry__ as g; g.build()\"` or `make -C yet-another-nerf_amd/csrc`"
     if not TORCH_LIB_PATH.exists():
         raise HipError(f"_codes_torch.so not found at {TORCH_LIB_PATH}; build it with {rebuild}")
     spec = importlib.util.spec_from_file_location(__package__ + "._codes_torch", TORCH_LIB_PATH)
-    m = importlib.util.module_from_spec(spec)
-    spec.loader.exec_module(m)
+    try:
+        m = importlib.util.module_from_spec(spec)
+        spec.loader.exec_module(m)
+    except ImportError as e:
+        raise HipError(f"{TORCH_LIB_PATH} does not load into torch {torch.__version__}: rebuild it with {rebuild}") from e
     built, src = m.build_id(), source_id(TORCH_SOURCES)
     if built != src:
         raise HipError(f"{TORCH_LIB_PATH} was built from other sources (build id {built}, sources {src}): rebuild it with "
                        f"{rebuild}")
+    if m.torch_version() != str(torch.__version__):
+        raise HipError(f"{TORCH_LIB_PATH} was built against torch {m.torch_version()}, this is {torch.__version__}: rebuild it "
+                       f"with {rebuild}")
     address = lambda fn: ctypes.cast(fn, c_void_p).value
     m.bind(*(address(fn) for fn in (L.yanerf_last_error, L.yanerf_dropout, L.yanerf_embedding_forward,
                                     L.yanerf_embedding_bwd_workspace_bytes, L.yanerf_embedding_backward)))
