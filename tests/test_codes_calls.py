@@ -1,6 +1,7 @@
 """Learned codes on the CPU: calls of the Python entry points that have to be refused, or have to be safe, whatever the
 tensors hold (nothing launches)."""
 import ctypes
+import subprocess
 import weakref
 
 import pytest
@@ -92,3 +93,12 @@ def test_binding_of_another_torch_is_refused(monkeypatch, tmp_path):
         with pytest.raises(_C.HipError, match="does not load"):
             _C.torch_ops()
     assert _C.torch_ops().torch_version() == torch.__version__
+
+
+def test_the_library_builds_without_torch():
+    """make's default is the C ABI's library: no step of it runs Python, g++ or names torch; `all` builds the binding too."""
+    csrc = _C.PKG / "csrc"
+    plan = lambda *goal: subprocess.run(["make", "-n", "-B", "-C", str(csrc), "PYTHON=false", *goal], check=True,
+                                        capture_output=True, text=True).stdout
+    assert "libyanerf_hip.so" in plan() and "torch" not in plan() and "g++" not in plan()
+    assert "libyanerf_hip.so" in plan("all") and "_codes_torch.so" in plan("all")

@@ -83,7 +83,7 @@ def lib():
     if not LIB_PATH.exists():
         raise HipError(
             f"libyanerf_hip.so not found at {LIB_PATH}; build it with `python -c \"import __graft_entry__ as g; "
-            f"g.build()\"` or `make -C yet-another-nerf_amd/csrc`. There is no CPU fallback."
+            f"g.build()\"` or `make -C yet-another-nerf_amd/csrc all`. There is no CPU fallback."
         )
     L = ctypes.CDLL(str(LIB_PATH))
     P = c_void_p
@@ -151,7 +151,7 @@ def torch_ops():
         return _torch_ops
     import torch  # (its libraries have to be loaded first)
     L = lib()
-    rebuild = "`python -c \"import __graft_entry__ as g; g.build()\"` or `make -C yet-another-nerf_amd/csrc`"
+    rebuild = "`python -c \"import __graft_entry__ as g; g.build()\"` or `make -C yet-another-nerf_amd/csrc all`"
     if not TORCH_LIB_PATH.exists():
         raise HipError(f"_codes_torch.so not found at {TORCH_LIB_PATH}; build it with {rebuild}")
     spec = importlib.util.spec_from_file_location(__package__ + "._codes_torch", TORCH_LIB_PATH)
