@@ -102,3 +102,16 @@ def test_the_library_builds_without_torch():
                                         capture_output=True, text=True).stdout
     assert "libyanerf_hip.so" in plan() and "torch" not in plan() and "g++" not in plan()
     assert "libyanerf_hip.so" in plan("all") and "_codes_torch.so" in plan("all")
+
+
+@pytest.mark.parametrize("scale,p", [(3.5e38, 0.0), (-1e39, 0.0), (1e300, 0.0), (3e38, 0.5), (1e308, 0.99), (1e-38, 0.0),
+                                     (-1e-45, 0.0), (1e-320, 0.5)])
+def test_factors_outside_fp32_are_refused(scale, p):
+    """A factor that fp32 holds as infinity makes a row of zeros NaN, one below its normal numbers loses its digits."""
+    L, D16, m = _C.lib(), ctypes.c_void_p(16), _C.torch_ops()
+    assert L.yanerf_embedding_forward(D16, 0, 4, D16, 8, 3, 5, 4, scale, p, 1, 2, None, None, D16, 0, None, None) == 1
+    assert b"factor" in L.yanerf_last_error()
+    assert L.yanerf_embedding_backward(D16, 0, D16, 8, 3, 5, 4, -1, scale, p, 1, 2, None, D16, 0, D16, None) == 1
+    assert b"factor" in L.yanerf_last_error()
+    with pytest.raises(ValueError, match="factor"):
+        m.embedding(torch.zeros(5, 4), torch.zeros(3, dtype=torch.int64), scale, None, p, 0, 0, None, -1, 0)

@@ -222,3 +222,17 @@ def test_code_table_in_a_capture(ops):
     assert not torch.equal(masks[0], masks[1]) and not torch.equal(masks[1], masks[2])
     m.eval()
     captured(lambda: m(image_ids=ids))
+
+
+# ------------------------------------------------------------------------------------------- factors
+@pytest.mark.parametrize("scale,p", [(0.0, 0.0), (0.0, 0.5), (3.4e38, 0.0), (1.2e-38, 0.0), (-1.2e-38, 0.5), (1e300, 1.0),
+                                     (-3e37, 0.9), (1.0, 1.0 - 2.0 ** -31)])
+def test_factors_at_the_ends_of_fp32(ops, scale, p):
+    """The largest and smallest factors that are taken, and 0; a row of zeros stays one."""
+    table, ids, g = 1e-3 * rand(30, 8), some_ids(200, 30), 1e-3 * rand(200, 8, seed=3)
+    table[4] = 0.0
+    table.requires_grad_()
+    y = ops.embedding(table, ids, scale=scale, dropout=p, rng=(1, 2))
+    R.assert_within(y, *R.lookup(table, ids, F32, scale, p, (1, 2)))
+    (gt,) = torch.autograd.grad(y, table, g)
+    R.assert_within(gt, *R.table_gradient(g, ids, 30, F32, scale, p, (1, 2)))

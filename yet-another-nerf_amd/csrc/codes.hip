@@ -18,6 +18,7 @@
 //   N > 16384, rows of g of <= 16 bytes     one partition that carries the rows along (bucket_sum_kernel)
 //   the rest                                a sort of (id, position) pairs, then sums over pieces of the sorted list
 //                                           (rank_sort_kernel to N = 16384, sort_scatter_kernel beyond; run_sum_kernel)
+#include <cfloat>
 #include <cmath>
 #include <type_traits>
 
@@ -1557,6 +1558,13 @@ inline int tile_rows(int64_t N, int64_t per_row, int64_t work, int64_t multiple)
 }
 // outputs that leave no cache lines worth keeping (the Infinity Cache holds 256 MB) are stored non-temporally
 inline bool streams_past_cache(int64_t bytes) { return bytes >= (64ll << 20); }
+// The factor, 0 or a normal number of fp32, in which the lookup multiplies: beyond them 0 would become NaN, and below them the
+// factor's own digits go
+inline int factor_ok(const char* what, double f) {
+  YN_CHECK(f == 0.0 || (std::fabs(f) >= FLT_MIN && std::fabs(f) <= FLT_MAX),
+           "%s: the factor scale / (1 - p) = %g is outside the range of fp32", what, f);
+  return 0;
+}
 inline int mask_args_ok(const char* what, double p) {
   YN_CHECK(p >= 0.0 && p <= 1.0, "%s: p=%g is not a probability", what, p);
   return 0;
@@ -1605,6 +1613,7 @@ int yanerf_embedding_forward(const void* table, int table_type, int64_t table_st
   YN_CHECK(table && ids && out, "embedding: null pointer");
   YN_CHECK(table_stride >= 0, "embedding: negative table stride");
   const Mask m = make_mask(p, seed, offset, rng_base);
+  if (factor_ok("embedding", mask_scale(scale, p, m))) return 1;
   const float f = (float)mask_scale(scale, p, m);
   const int64_t wide = 16 / (type_bytes(table_type) > type_bytes(out_type) ? type_bytes(table_type) : type_bytes(out_type));
   auto fits = [&](int64_t vec) {
@@ -1695,6 +1704,7 @@ int yanerf_embedding_backward(const void* g, int g_type, const void* ids, int id
   YN_CHECK(aligned(workspace, 16), "embedding_backward: the workspace is not aligned to 16 bytes");
   const Mask m = make_mask(p, seed, offset, rng_base);
   const double f = mask_scale(scale, p, m);
+  if (factor_ok("embedding_backward", f)) return 1;
   hipStream_t st = as_stream(stream);
   char* ws = (char*)workspace;
   if (N == 0) {

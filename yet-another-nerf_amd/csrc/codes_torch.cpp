@@ -221,6 +221,9 @@ Tensor embedding(const Tensor& table, const Tensor& ids_in, double scale, std::o
   if (!std::isfinite(scale)) throw py::value_error("embedding: scale is not finite");
   Mask m{p, seed, offset, rng_base, Tensor()};
   m.check("embedding", table);
+  const double f = p < 1.0 ? scale / (1.0 - p) : 0.0;
+  if (f != 0.0 && !(std::fabs(f) >= std::numeric_limits<float>::min() && std::fabs(f) <= std::numeric_limits<float>::max()))
+    throw py::value_error("embedding: the factor scale / (1 - dropout) is outside the range of fp32");
   refuse_tangent("embedding", table);
   const bool graph = at::GradMode::is_enabled() && table.requires_grad();
   if (graph) m.keep();

@@ -566,7 +566,8 @@ def embedding(table: torch.Tensor, ids: torch.Tensor, *, scale: float = 1.0, pad
               dropout: float = 0.0, out_dtype: Optional[torch.dtype] = None, rng: Optional[Tuple[int, int]] = None,
               rng_base: Optional[torch.Tensor] = None, check: bool = True) -> torch.Tensor:
     """scale * table[ids], rows of `table` [V, D] (float32, bfloat16 or float16; rows may be strided) by integer `ids`
-    (int32 or int64, any shape), as [*ids.shape, D] of `out_dtype` (default: the table's). With dropout > 0 the result is
+    (int32 or int64, any shape), as [*ids.shape, D] of `out_dtype` (default: the table's). scale is 0 or, over 1 - dropout,
+    of the size of a normal fp32 number. With dropout > 0 the result is
     dropped out in the same kernel: the mask of `dropout()` over the result, with the same `rng` / `rng_base`.
 
     The gradient of the table sums the rows' gradients in fp32 in an order fixed by the ids (sorted, no float atomics:
