@@ -236,3 +236,38 @@ def test_factors_at_the_ends_of_fp32(ops, scale, p):
     R.assert_within(y, *R.lookup(table, ids, F32, scale, p, (1, 2)))
     (gt,) = torch.autograd.grad(y, table, g)
     R.assert_within(gt, *R.table_gradient(g, ids, 30, F32, scale, p, (1, 2)))
+
+
+# ------------------------------------------------------------------------------------------- what a backward is given
+def test_saved_tensor_hooks(ops):
+    """Ids that hooks move away and back give the same gradient; ids that come back elsewhere, in another type or in another
+    number are refused before a kernel reads them."""
+    t, i, g = rand(20, 8).requires_grad_(), some_ids(300, 20), rand(300, 8, seed=2)
+    (want,) = torch.autograd.grad(ops.embedding(t, i), t, g)
+    with torch.autograd.graph.save_on_cpu():
+        y = ops.embedding(t, i)
+    assert torch.equal(torch.autograd.grad(y, t, g)[0], want)
+    for back in (lambda x: x.int(), lambda x: x.repeat_interleave(2)[::2]):
+        with torch.autograd.graph.saved_tensors_hooks(lambda x: x, back):
+            y = ops.embedding(t, i)
+        assert torch.equal(torch.autograd.grad(y, t, g)[0], want)
+    for back in (lambda x: x.cpu(), lambda x: x.float(), lambda x: x[:-1], lambda x: x.repeat(2), lambda x: x.short()):
+        with torch.autograd.graph.saved_tensors_hooks(lambda x: x, back):
+            y = ops.embedding(t, i)
+        with pytest.raises(RuntimeError, match="saved ids"):
+            torch.autograd.grad(y, t, g)
+
+
+def test_direct_calls_of_the_nodes(ops):
+    """A node called as a function gets what its caller passes, which the engine has not compared with the output."""
+    t, x, i = rand(20, 8).requires_grad_(), rand(300, 8).requires_grad_(), some_ids(300, 20)
+    g = rand(300, 8, seed=2)
+    for y, leaf in ((ops.embedding(t, i, dropout=0.5, rng=(1, 2)), t), (ops.dropout(x, 0.5, rng=(1, 2)), x)):
+        (want,) = torch.autograd.grad(y, leaf, g, retain_graph=True)
+        assert torch.equal(y.grad_fn(g), want)
+        for bad in (g.cpu(), g[:-1], g.half(), g.double(), g.long(), torch.cat([g, g])):
+            with pytest.raises(RuntimeError, match="the gradient differs"):
+                y.grad_fn(bad)
+        with pytest.raises(TypeError):  # torch's own check
+            y.grad_fn()
+        assert y.grad_fn(None) is None

@@ -119,6 +119,20 @@ void refuse_graph(const char* what, const Tensor& g) {
 // Its values in memory: contiguous() hands a contiguous view whose values are the negated memory back as it is
 Tensor resolved(const Tensor& t) { return t.resolve_neg().contiguous(); }
 
+// What a backward may read of the gradient it is given: the engine has compared it with the output, a direct call of the node
+// has not
+struct Output {
+  int64_t numel = 0;
+  at::ScalarType type = at::kFloat;
+  c10::Device device = c10::Device(c10::kCUDA);
+  explicit Output(const Tensor& y) : numel(y.numel()), type(y.scalar_type()), device(y.device()) {}
+  Output() = default;
+  void check(const char* what, const Tensor& g) const {
+    if (g.device() != device || g.scalar_type() != type || g.numel() != numel)
+      throw std::runtime_error(std::string(what) + ": the gradient differs from the output in device, type or size");
+  }
+};
+
 // ------------------------------------------------------------------------------------------ dropout
 Tensor run_dropout(const Tensor& x, const Mask& m, uint64_t offset, const uint64_t* base, uint64_t* used) {
   Tensor y = at::empty(x.sizes(), x.options());
@@ -131,11 +145,13 @@ Tensor run_dropout(const Tensor& x, const Mask& m, uint64_t offset, const uint64
 
 struct DropoutBackward : Node {
   Mask mask;
+  Output output;
   std::string name() const override { return "YanerfDropoutBackward"; }
   variable_list apply(variable_list&& grads) override {
     if (!grads[0].defined() || !task_should_compute_output(0)) return {Tensor()};
     refuse_recording("dropout");
     refuse_graph("dropout", grads[0]);
+    output.check("dropout", grads[0]);
     at::NoGradGuard no_grad;
     return {run_dropout(resolved(grads[0]), mask, mask.again_offset(), mask.used_ptr(), nullptr)};
   }
@@ -159,6 +175,7 @@ Tensor dropout(const Tensor& x, double p, uint64_t seed, uint64_t offset, const 
   if (graph) {
     auto node = std::shared_ptr<DropoutBackward>(new DropoutBackward(), torch::autograd::deleteNode);
     node->mask = m;
+    node->output = Output(y);
     node->set_next_edges(torch::autograd::collect_next_edges(x));
     torch::autograd::set_history(y, node);
   }
@@ -169,6 +186,7 @@ Tensor dropout(const Tensor& x, double p, uint64_t seed, uint64_t offset, const 
 struct EmbeddingBackward : Node {
   torch::autograd::SavedVariable ids;
   Mask mask;
+  Output output;
   int64_t V = 0, D = 0, pad = -1;
   double scale = 1.0;
   at::ScalarType type = at::kFloat;
@@ -178,8 +196,13 @@ struct EmbeddingBackward : Node {
     if (!grads[0].defined() || !task_should_compute_output(0)) return {Tensor()};
     refuse_recording("embedding");
     refuse_graph("embedding", grads[0]);
+    output.check("embedding", grads[0]);
     at::NoGradGuard no_grad;
-    const Tensor i = ids.unpack(), g = resolved(grads[0]);
+    const Tensor i = resolved(ids.unpack()), g = resolved(grads[0]);
+    // hooks of saved tensors may hand back another tensor than was saved
+    if (i.device() != output.device || (i.scalar_type() != at::kLong && i.scalar_type() != at::kInt) ||
+        i.numel() * D != output.numel)
+      throw std::runtime_error("embedding: the saved ids came back with another device, type or size");
     const int64_t N = i.numel(), bytes = api.workspace(N, V, D);
     if (bytes < 0) done(1, "yanerf_embedding_bwd_workspace_bytes");
     Tensor grad = at::empty({V, D}, g.options().dtype(type));
@@ -245,6 +268,7 @@ Tensor embedding(const Tensor& table, const Tensor& ids_in, double scale, std::o
     auto node = std::shared_ptr<EmbeddingBackward>(new EmbeddingBackward(), torch::autograd::deleteNode);
     node->ids = torch::autograd::SavedVariable(ids, /*is_output=*/false);
     node->mask = m;
+    node->output = Output(out);
     node->V = V;
     node->D = D;
     node->pad = pad;
