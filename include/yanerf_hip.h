@@ -267,7 +267,8 @@ int yanerf_step_advance(uint64_t* state, uint64_t rng_delta, void* stream);
  *   backward evaluates it anew from the same (seed, offset).
  *   rng_base: NULL, or 1 device u64 added to `offset` (a graph-captured step advances it on the device).
  *   rng_used: NULL, or 1 device u64 that receives offset + *rng_base, for a backward that runs after the base moved on
- *     (pass it as that call's rng_base with offset 0). Not written where a call has no elements.
+ *     (pass it as that call's rng_base with offset 0). Not rng_base itself, which the kernel's other workgroups still read.
+ *     Not written where a call has no elements.
  *   Sums are fp32. The lookup's and dropout's products are fp32 too; the gradient multiplies each sum by the factor in 64
  *   bits. Each output is rounded once more, to its type. scale / (1 - p) is 0 or has the size of a normal
  *   fp32 number. N, V < 2^31; D <= 2^24; N * D, V * D and dropout's n <= 2^36.

@@ -115,3 +115,12 @@ def test_factors_outside_fp32_are_refused(scale, p):
     assert b"factor" in L.yanerf_last_error()
     with pytest.raises(ValueError, match="factor"):
         m.embedding(torch.zeros(5, 4), torch.zeros(3, dtype=torch.int64), scale, None, p, 0, 0, None, -1, 0)
+
+
+def test_rng_used_is_not_rng_base():
+    """One workgroup would write the offset while the others still read the base."""
+    L, D16, b, u = _C.lib(), ctypes.c_void_p(16), ctypes.c_void_p(64), ctypes.c_void_p(128)
+    assert L.yanerf_dropout(D16, 0, 8, 0.5, 1, 2, b, b, D16, None) == 1 and b"rng_used" in L.yanerf_last_error()
+    assert L.yanerf_embedding_forward(D16, 0, 4, D16, 8, 3, 5, 4, 1.0, 0.5, 1, 2, b, b, D16, 0, None, None) == 1
+    assert b"rng_used" in L.yanerf_last_error()
+    assert L.yanerf_dropout(D16, 0, 0, 0.5, 1, 2, b, u, D16, None) == 0 and L.yanerf_dropout(D16, 0, 0, 0.5, 1, 2, None, None, D16, None) == 0

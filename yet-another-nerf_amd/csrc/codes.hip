@@ -1581,6 +1581,7 @@ int yanerf_dropout(const void* x, int type, int64_t n, double p, uint64_t seed, 
   YN_CHECK(type_ok(type), "dropout: unknown element type %d", type);
   YN_CHECK(n >= 0 && n <= (1ll << 36), "dropout: n=%lld out of range", (long long)n);
   if (mask_args_ok("dropout", p)) return 1;
+  YN_CHECK(!rng_used || rng_used != rng_base, "dropout: rng_used is rng_base");
   if (n == 0) return 0;
   YN_CHECK(x && y, "dropout: null pointer");
   const Mask m = make_mask(p, seed, offset, rng_base);
@@ -1608,6 +1609,7 @@ int yanerf_embedding_forward(const void* table, int table_type, int64_t table_st
   YN_CHECK(id_bytes == 4 || id_bytes == 8, "embedding: ids of %d bytes", id_bytes);
   if (embedding_sizes_ok("embedding", N, V, D) || mask_args_ok("embedding", p)) return 1;
   YN_CHECK(std::isfinite(scale), "embedding: scale is not finite");
+  YN_CHECK(!rng_used || rng_used != rng_base, "embedding: rng_used is rng_base");
   if (N == 0 || D == 0) return 0;
   YN_CHECK(V >= 1, "embedding: an empty table");
   YN_CHECK(table && ids && out, "embedding: null pointer");
