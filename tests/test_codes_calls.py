@@ -124,3 +124,28 @@ def test_rng_used_is_not_rng_base():
     assert L.yanerf_embedding_forward(D16, 0, 4, D16, 8, 3, 5, 4, 1.0, 0.5, 1, 2, b, b, D16, 0, None, None) == 1
     assert b"rng_used" in L.yanerf_last_error()
     assert L.yanerf_dropout(D16, 0, 0, 0.5, 1, 2, b, u, D16, None) == 0 and L.yanerf_dropout(D16, 0, 0, 0.5, 1, 2, None, None, D16, None) == 0
+
+
+def test_module_stream_and_seeds(monkeypatch):
+    """The default masks' stream as ops.dropout describes it: another seed starts it anew, the same seed goes on, set_state
+    starts it anew at the same seed."""
+    from yanerf_amd import ops
+    monkeypatch.setattr(ops, "_capturing", lambda dev: False)
+    before, seed = ops.RNG.get_state(), torch.initial_seed()
+    try:
+        torch.manual_seed(123)
+        ops.RNG.set_state((None, 0))
+        assert [ops._mask_rng("dropout", 0.5, None, None, 100, 0) for _ in range(2)] == [(123, 0), (123, 100)]
+        torch.manual_seed(123)
+        assert ops._mask_rng("dropout", 0.5, None, None, 100, 0) == (123, 200)
+        torch.manual_seed(124)
+        assert ops._mask_rng("dropout", 0.5, None, None, 100, 0) == (124, 0)
+        torch.manual_seed(123)
+        assert ops._mask_rng("dropout", 0.5, None, None, 100, 0) == (123, 0)
+        ops.RNG.set_state((None, 0))
+        assert ops._mask_rng("dropout", 0.5, None, None, 100, 0) == (123, 0)
+        assert ops._mask_rng("dropout", 0.5, (-1, 2 ** 64 + 7), None, 100, 0) == (2 ** 64 - 1, 7)
+        assert ops.RNG.get_state() == (123, 100)
+    finally:
+        torch.manual_seed(seed)
+        ops.RNG.set_state(before)

@@ -512,8 +512,10 @@ def dropout(x: torch.Tensor, p: float, *, rng: Optional[Tuple[int, int]] = None,
     1 / (1 - p). The mask is a function of a Philox counter (include/yanerf_hip.h): it is never stored, and the backward
     draws it again. A dropped element is 0 even where x is infinite or NaN. Differentiable once.
 
-    rng: the (seed, offset) of the mask; the default takes the next of the module stream, which follows
-    torch.manual_seed. rng_base: one int64 element on x's device that is added to offset when the kernel runs (a captured
+    rng: the (seed, offset) of the mask; the default takes the next of the module stream RNG. That starts anew when
+    torch.manual_seed sets another seed than it had, and goes on where it is when the seed is set again:
+    RNG.set_state((None, 0)) starts it anew there. It does not follow torch's generator states, so a forward that is run
+    twice (activation checkpointing) has to pass its rng. rng_base: one int64 element on x's device that is added to offset when the kernel runs (a captured
     step advances it, so each replay draws another mask; the backward uses the forward's, also if the base has moved). A
     graph capture wants one of the two: the module stream's draw, made once on the host, would be every replay's."""
     _dev(x)
