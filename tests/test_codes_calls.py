@@ -149,3 +149,20 @@ def test_module_stream_and_seeds(monkeypatch):
     finally:
         torch.manual_seed(seed)
         ops.RNG.set_state(before)
+
+
+def test_identity_mapper_passes_on():
+    """Without dropout, and with it in evaluation mode, the mapper is the reference's: what it is given comes back."""
+    from yanerf_amd.pipelines.feature_extractors import FEATURE_EXTRACTORS
+    codes = torch.ones(2, 4)
+    m = FEATURE_EXTRACTORS.build(dict(type="IdentityMapper"))
+    out = m(global_codes=codes, other=3)
+    assert out["global_codes"] is codes and out["other"] == 3 and m() == {} and not m.state_dict()
+    m = FEATURE_EXTRACTORS.build(dict(type="IdentityMapper", dropout=0.5))
+    assert m(other=3, global_codes=None) == {"other": 3, "global_codes": None}
+    with pytest.raises(RuntimeError, match="HIP kernels"):
+        m(global_codes=codes)
+    assert m.eval()(global_codes=codes)["global_codes"] is codes
+    for p in (-0.1, 1.5, float("nan")):
+        with pytest.raises(ValueError):
+            FEATURE_EXTRACTORS.build(dict(type="IdentityMapper", dropout=p))

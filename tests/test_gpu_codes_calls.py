@@ -271,3 +271,50 @@ def test_direct_calls_of_the_nodes(ops):
         with pytest.raises(TypeError):  # torch's own check
             y.grad_fn()
         assert y.grad_fn(None) is None
+
+
+# ------------------------------------------------------------------------------------------- in the pipeline
+def test_caller_codes_with_dropout_in_the_pipeline(ops):
+    """The conditional pipeline drops entries of the codes that its caller computes, in training: the loss and the gradient of
+    the codes are those of the same codes dropped by the stated mask and passed through a plain IdentityMapper; evaluation
+    passes them on as they are."""
+    from test_gpu_codes import conditional_pipeline
+    from yanerf_amd.pipelines.utils import EvaluationMode as EM
+    torch.manual_seed(0)
+    drops = conditional_pipeline(dict(type="IdentityMapper", dropout=0.25))
+    plain = conditional_pipeline(dict(type="IdentityMapper"))
+    plain.load_state_dict(drops.state_dict())
+    B = 3
+    poses, focal = torch.randn(B, 3, 4, device=DEV), torch.ones(B, device=DEV) * 500
+    image, codes = torch.rand(B, 6, 10, 3, device=DEV), rand(B, 1, 4, seed=4).requires_grad_()
+    run = lambda pipe, c, mode: pipe(poses=poses, focal_lengths=focal, image_rgb=image, evaluation_mode=mode, global_codes=c)
+    with torch.no_grad():
+        a, b = (run(pipe.eval(), codes.squeeze(1), EM.EVALUATION)["rendered_images"] for pipe in (drops, plain))
+    assert torch.equal(a, b)
+    drops.train(), plain.train()
+    seed = torch.initial_seed()
+    ops.RNG.set_state((seed, 1 << 20))
+    p1 = run(drops, codes.squeeze(1), EM.TRAINING)["objective"].mean()
+    (g1,) = torch.autograd.grad(p1, codes)
+    # raygen takes the first draws, the mapper the next
+    keep = torch.from_numpy(R.keep_mask(B * 4, 0.25, seed, (1 << 20) + B * 4 * 5).reshape(B, 4)).to(DEV)
+    ops.RNG.set_state((seed, 1 << 20))
+    draw, calls = ops.RNG.next, []
+
+    def next_(n=1):
+        calls.append(n)
+        r = draw(n)
+        if len(calls) == 1:
+            draw(B * 4)  # the mapper's draw
+        return r
+
+    ops.RNG.next = next_
+    try:
+        dropped = codes.squeeze(1) * keep / 0.75
+        p2 = run(plain, dropped, EM.TRAINING)["objective"].mean()
+    finally:
+        del ops.RNG.next
+    (g2,) = torch.autograd.grad(p2, codes)
+    assert keep.any() and not keep.all()
+    assert abs(p1.item() - p2.item()) <= 1e-5 * abs(p2.item())
+    assert (g1[~keep[:, None]] == 0).all() and (g1 - g2).abs().max() <= 1e-4 * g2.abs().max()
