@@ -297,8 +297,9 @@ int yanerf_flag_take(int* flag, int* taken, void* stream);
  * they are 0), -1 for sizes out of range. */
 int64_t yanerf_embedding_bwd_workspace_bytes(int64_t N, int64_t V, int64_t D);
 /* grad_table[v][d] = scale / (1 - p) * sum over n with ids[n] = v of keep(n D + d) g[n][d]: every row is written, rows
- * that no id names and row padding_idx (-1: none; its lookup is that of any row) with zeros. Ids outside [0, V) take no part. The order of each sum
- * depends on the ids alone (no float atomics). */
+ * that no id names and row padding_idx (-1: none; its lookup is that of any row) with zeros. Ids outside [0, V) take no
+ * part. The order of each sum follows from the ids, the sizes, the types and the pointers' alignment (no float atomics):
+ * equal calls give equal bits. */
 int yanerf_embedding_backward(const void* g, int g_type, const void* ids, int id_bytes, int64_t N, int64_t V,
                               int64_t D, int64_t padding_idx, double scale, double p, uint64_t seed, uint64_t offset,
                               const uint64_t* rng_base, void* grad_table, int table_type, void* workspace,

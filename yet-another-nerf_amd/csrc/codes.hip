@@ -10,8 +10,8 @@
 // whatever its input holds. Sums are fp32, products with f too but the gradient's, which is taken in 64 bits; each output
 // is rounded once more, to its type.
 //
-// The gradient groups the positions of each row with stable sorts, so the terms of a row are added in an order that the ids
-// alone fix: no float atomics, the same bits on every run. Which way depends on the sizes:
+// The gradient groups the positions of each row with stable sorts, so the terms of a row are added in an order that the call
+// fixes (its ids, sizes, types and alignment): no float atomics, the same bits on every run. Which way depends on the sizes:
 //
 //   N <= 4096, gradient <= 32 MB            one launch, each workgroup picks the ids of its own rows (own_rows_kernel)
 //   V <= 32                                 one pass over g with a table a lane (dense_sum_kernel)
@@ -690,7 +690,8 @@ __global__ __launch_bounds__(kRankThreads) void rank_sort_kernel(KeyFromIds<IT> 
 // A run is the sorted positions of one row. Sorted positions are cut into equal pieces whatever the runs' lengths are, so
 // that a row named by most ids costs no more than many rows named once: a group of lanes (one vector of columns a lane)
 // adds a piece, writes the rows whose runs lie inside it, and leaves the sums of the runs that its ends cut, which are then
-// joined in the order of the pieces. Pieces depend on the ids alone, so the order of every sum does.
+// joined in the order of the pieces. Pieces depend on the sizes and the vector's width, runs on the ids: nothing else changes
+// the order of a sum.
 template <typename GT, int VEC>
 __device__ __forceinline__ void masked_term(const GT* g, int64_t D, uint32_t pos, int64_t d, const Mask& m, uint64_t off,
                                             float (&v)[VEC]) {
@@ -849,7 +850,8 @@ inline OwnPlan own_plan(int64_t N, int64_t V, int64_t D, int vec, int64_t g_byte
   while (o.lg > 2 && ((dv + (1 << o.lg) - 1) >> o.lg) * groups < 64) --o.lg;
   while (o.lg < 6 && ((dv + (1 << o.lg) - 1) >> o.lg) > 256) ++o.lg;
   o.chunks = (dv + (1 << o.lg) - 1) >> o.lg;
-  // owners: one for every 32 KB of zeros or 8 KB of gradient rows, up to 1024 workgroups
+  // owners: one for every 32 KB of zeros or 8 KB of gradient rows, up to 1024 workgroups, then up to the next power of two
+  // (fewer than 2048 workgroups where the columns make no more than 1024 chunks)
   const int64_t most = 1024 / o.chunks > 1 ? 1024 / o.chunks : 1;
   int64_t want = V * D * t_bytes / 32768;
   want = want > N * D * g_bytes / 8192 ? want : N * D * g_bytes / 8192;
@@ -866,6 +868,11 @@ inline OwnPlan own_plan(int64_t N, int64_t V, int64_t D, int vec, int64_t g_byte
 // the list packs (slot, index) into 32 bits, and list and presence bits share the LDS with RunEnds; large tables are left
 // to the sorted path, whose zeros stream faster (100 ids of 500000 x 100 bf16: 29 us against 32; 4000 of 50000 x 1000: 37
 // against 60)
+// The other end, us for one launch against the other paths: with rows named evenly it wins up to 4096 ids (4096 of
+// 5000 x 64 bf16 11.2 / 17.7, 50000 x 32 fp32 9.2 / 16.4) and, with the registers and LDS for more, beyond (8192: 15.3 / 19.5,
+// 13.8 / 18.9); with word frequencies, where one owner has most positions, it is level at 2048 (17.7 / 17.8, 16.8 / 17.1), behind
+// at 4096 (21.9 / 20.1, 21.8 / 19.6; 500 x 4 fp32 41.1 / 23.2) and further behind beyond (8192: 32.6 / 25.1, 30.1 / 23.3). Tables
+// of up to 32 rows would be faster with a table a lane from about 1000 ids on (4096 of 17 x 64 bf16 21.6 / 9.5).
 inline bool own_fits(int64_t N, int64_t table_bytes, const OwnPlan& o) {
   return N <= kOwnMax && table_bytes <= kOwnTable && o.slots < (1ll << (32 - kIndexBits)) && o.lds <= 100 * 1024;
 }
@@ -1241,7 +1248,7 @@ __global__ __launch_bounds__(kRunThreads) void run_join_kernel(const Pair* pairs
 // ---- long id lists of short rows (up to 16 bytes of g): gathering such rows one by one would fetch a cache line for each.
 // One partition by ranges of table rows carries the rows of g along, dropout applied; then a workgroup streams a tile of a
 // bucket, each wave into its own LDS table of the bucket's rows. Lanes of a wave that hold the same row add one after the
-// other in the order of the lanes, so that the ids alone fix the sums' order. A bucket of more than one tile leaves its
+// other in the order of the lanes, so that the ids fix the sums' order. A bucket of more than one tile leaves its
 // tiles' tables to a second launch. Every row of a bucket is written, so the gradient needs no zeros beforehand. 6.3 M ids of
 // 512000 x 2 fp32: count 10, scan 11, partition 43, sums 46, join 7 us (sorting pairs and gathering: 270 us); the partition
 // is bound like the sort's scatter, the sums by the turns of the lanes that share a row.
@@ -1260,7 +1267,8 @@ inline BucketPlan bucket_plan(int64_t N, int64_t V, int64_t D, int64_t g_bytes) 
   BucketPlan b{0, 0, 0, 1};
   if (D * g_bytes > 16) return b;
   while (b.dm < D) b.dm *= 2;
-  // up to 1023 buckets (and one for the ids that take no part), none expected to hold less than half a tile
+  // up to 1023 buckets (and one for the ids that take no part), as many as would hold half a tile each; more, of fewer ids,
+  // where a bucket has all the rows that its table holds (16385 ids of 2000000 x 1: 977 buckets of 17 ids)
   int64_t most = N / (kBucketTile / 2);
   most = most < 1 ? 1 : most > 1023 ? 1023 : most;
   while (((V + (1ll << b.lrows) - 1) >> b.lrows) > most && ((2ll << b.lrows) * b.dm <= kBucketFloats)) ++b.lrows;

@@ -572,7 +572,7 @@ def embedding(table: torch.Tensor, ids: torch.Tensor, *, scale: float = 1.0, pad
     of the size of a normal fp32 number. With dropout > 0 the result is
     dropped out in the same kernel: the mask of `dropout()` over the result, with the same `rng` / `rng_base`.
 
-    The gradient of the table sums the rows' gradients in fp32 in an order fixed by the ids (sorted, no float atomics:
+    The gradient of the table sums the rows' gradients in fp32 in an order fixed by the call (sorted, no float atomics:
     the same bits on every run) and is dense: zeros for rows that no id names and for row `padding_idx` (which may count
     from the end, as in torch.nn.Embedding; its lookup is that of any row). Differentiable once.
 
