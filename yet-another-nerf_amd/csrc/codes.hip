@@ -187,7 +187,8 @@ inline bool aligned(const void* p, int64_t bytes) { return ((uintptr_t)p & (uint
 // ------------------------------------------------------------------------------------------ dropout
 // Bound by the bytes of x and y: 16 bytes a lane each way, loaded before anything else is looked at, and one Philox call
 // for every 4 elements hides behind them. A lane takes one vector: loops over more of them measured 10 % slower. 201 M bf16
-// values: 133 us, 6.1 TB/s (a copy of them by torch 152 us); 33.5 M fp32 values: 42 us, 6.3 TB/s.
+// values: 142 to 145 us for a launch by itself, 5.6 TB/s, and 134 us for each of a row of launches (a copy of them by torch
+// 151 us); 33.5 M fp32 values: 42 us, 6.4 TB/s.
 template <typename T, bool ALIGNED, bool NT>
 __global__ __launch_bounds__(256) void dropout_kernel(const T* x, T* y, int64_t n, int64_t first, Mask m, float f,
                                                       uint64_t* used) {
@@ -233,8 +234,8 @@ __global__ void take_flag_kernel(int* flag, int* taken) {
 // ------------------------------------------------------------------------------------------ lookup
 // A workgroup takes `rows` consecutive ids. Rows of whole vectors: lane t of the tile's rows * D / VEC vectors copies one,
 // kUnroll of them in flight (1, 2 and 8 measured the same or up to 10 % slower). The ids and hot rows come from L1 / L2, so
-// the output's bytes bound it: 640000 x 16 bf16 7.7 us (20 MB out), 6.3 M x 2 fp32 21 us (50 MB out, 8 bytes a lane);
-// with dropout Philox does, 16384 x 1024 bf16 16.6 us.
+// the output's bytes bound it: 640000 x 16 bf16 7.4 us (20 MB out), 6.3 M x 2 fp32 21 us (50 MB out, 8 bytes a lane);
+// with dropout Philox does, 16384 x 1024 bf16 16.0 us.
 constexpr int kUnroll = 4;
 
 template <typename TT, typename OT, typename IT, int VEC, bool NT>
@@ -286,7 +287,7 @@ __global__ __launch_bounds__(256) void embedding_rows_of_vectors_kernel(const TT
 }
 
 // Any other row length, stride or alignment: a lane takes 4 consecutive elements of the output, wherever rows begin, so
-// that one Philox call still serves 4 of them and stores stay wide. `rows` is a multiple of 4. 10007 x 37 fp16: 4.1 us.
+// that one Philox call still serves 4 of them and stores stay wide. `rows` is a multiple of 4. 10007 x 37 fp16: 4.2 us.
 template <typename TT, typename OT, typename IT, bool ALIGNED>
 __global__ __launch_bounds__(256) void embedding_any_rows_kernel(const TT* table, int64_t stride, const IT* ids,
                                                                  int64_t N, int64_t V, Div dd, int rows, OT* out, Mask m,
@@ -824,7 +825,7 @@ __device__ __forceinline__ void sum_runs(RunEnds<THREADS, VEC>& ends, const Src&
 // ids, keeps the positions of its own rows in order, sorts them by row, adds their runs and writes zeros to its other
 // rows. The rows come in groups of 2^lgroup neighbours dealt out to the workgroups in turn, so that the low ids, which
 // word frequencies favour, spread over the chip. What it costs is that each workgroup reads every id (from L2). Bound by
-// latency: 1 id of 100 x 32 fp32 4.3 us, 4096 ids of 100 x 48 fp32 9.0 us (a sort, sums and a join: 18 us in three launches).
+// latency: 1 id of 100 x 32 fp32 4.6 us, 4096 ids of 100 x 48 fp32 8.9 us (a sort, sums and a join: 18 us in three launches).
 constexpr int kOwnThreads = 512, kOwnWaves = kOwnThreads / 64;
 constexpr int64_t kOwnMax = 4096;  // ids
 constexpr int64_t kOwnTable = 32ll << 20;  // bytes of the gradient
@@ -1250,7 +1251,7 @@ __global__ __launch_bounds__(kRunThreads) void run_join_kernel(const Pair* pairs
 // bucket, each wave into its own LDS table of the bucket's rows. Lanes of a wave that hold the same row add one after the
 // other in the order of the lanes, so that the ids fix the sums' order. A bucket of more than one tile leaves its
 // tiles' tables to a second launch. Every row of a bucket is written, so the gradient needs no zeros beforehand. 6.3 M ids of
-// 512000 x 2 fp32: count 10, scan 11, partition 43, sums 46, join 7 us (sorting pairs and gathering: 270 us); the partition
+// 512000 x 2 fp32: count 10, scan 11, partition 42, sums 46, join 7 us (sorting pairs and gathering: 270 us); the partition
 // is bound like the sort's scatter, the sums by the turns of the lanes that share a row.
 constexpr int kBucketThreads = 512, kBucketWaves = kBucketThreads / 64;
 constexpr int64_t kBucketTile = 8192;    // positions a workgroup
