@@ -166,3 +166,24 @@ def test_identity_mapper_passes_on():
     for p in (-0.1, 1.5, float("nan")):
         with pytest.raises(ValueError):
             FEATURE_EXTRACTORS.build(dict(type="IdentityMapper", dropout=p))
+
+
+def test_recorders_leave_no_id_flag():
+    """A thread's first checked lookup under a recorder is refused before the recorder's tensor becomes the thread's flag."""
+    import threading
+    from torch._subclasses.fake_tensor import FakeTensorMode
+    from yanerf_amd import ops
+    seen = []
+
+    def work():
+        with FakeTensorMode(allow_non_fake_inputs=True):
+            try:
+                ops._id_flag(0, own=True)
+            except RuntimeError as e:
+                seen.append(str(e))
+        seen.append(dict(ops._OWN_FLAGS.__dict__))
+
+    t = threading.Thread(target=work)
+    t.start()
+    t.join()
+    assert "cannot be recorded" in seen[0] and seen[1:] == [{}]

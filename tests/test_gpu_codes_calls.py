@@ -123,6 +123,30 @@ def test_recording_is_refused(ops):
             make_fx(lambda g: torch.autograd.grad(y, leaf, g, retain_graph=True)[0])(torch.ones_like(y))
 
 
+def test_checked_lookups_after_a_recorder(ops):
+    """A thread whose first checked lookup runs under fake tensors, and is refused, looks up as ever afterwards."""
+    import threading
+    from torch.fx.experimental.proxy_tensor import make_fx
+    t, i, seen = rand(64, 16), some_ids(50, 64), []
+
+    def work():
+        for mode in ("fake", "real"):
+            try:
+                make_fx(lambda t: ops.embedding(t, i), tracing_mode=mode)(t)
+            except RuntimeError as e:
+                seen.append("cannot be recorded" in str(e))
+        seen.append(torch.equal(ops.embedding(t, i), t[i]))
+        try:
+            ops.embedding(t, i + 64)
+        except IndexError:
+            seen.append(True)
+
+    x = threading.Thread(target=work)
+    x.start()
+    x.join()
+    assert seen == [True] * 4
+
+
 def test_watching_is_allowed(ops):
     """A dispatch mode that only watches gets the eager results."""
     from torch.utils._python_dispatch import TorchDispatchMode

@@ -286,6 +286,7 @@ PYBIND11_MODULE(_codes_torch, m) {
   m.def("build_id", [] { return YANERF_SRC_SHA; });
   m.def("torch_version", [] { return YANERF_TORCH_VERSION; });
   m.def("bind", &bind);
+  m.def("refuse_recording", &refuse_recording);
   m.def("dropout", &dropout, py::call_guard<py::gil_scoped_release>());
   m.def("embedding", &embedding, py::call_guard<py::gil_scoped_release>());
 }

@@ -515,9 +515,10 @@ def dropout(x: torch.Tensor, p: float, *, rng: Optional[Tuple[int, int]] = None,
     rng: the (seed, offset) of the mask; the default takes the next of the module stream RNG. That starts anew when
     torch.manual_seed sets another seed than it had, and goes on where it is when the seed is set again:
     RNG.set_state((None, 0)) starts it anew there. It does not follow torch's generator states, so a forward that is run
-    twice (activation checkpointing) has to pass its rng. rng_base: one int64 element on x's device that is added to offset when the kernel runs (a captured
-    step advances it, so each replay draws another mask; the backward uses the forward's, also if the base has moved). A
-    graph capture wants one of the two: the module stream's draw, made once on the host, would be every replay's."""
+    twice (activation checkpointing) has to pass its rng. rng_base: one int64 element on x's device that is added to
+    offset when the kernel runs (a captured step advances it, so each replay draws another mask; the backward uses the
+    forward's, also if the base has moved). A graph capture wants one of the two: the module stream's draw, made once on
+    the host, would be every replay's."""
     _dev(x)
     return _C.torch_ops().dropout(x, p, *_mask_rng("dropout", p, rng, rng_base, x.numel(), x.get_device()), rng_base)
 
@@ -532,6 +533,7 @@ def _id_flag(dev: int, own: bool) -> int:
     if own:
         f = _OWN_FLAGS.__dict__.get(dev)
         if f is None:
+            _C.torch_ops().refuse_recording("embedding")  # before a recorder's tensor becomes the thread's flag
             f = torch.zeros(1, dtype=torch.int32, device=f"cuda:{dev}")
             torch.cuda.current_stream(dev).synchronize()  # cleared before a lookup on any stream can set it
             _OWN_FLAGS.__dict__[dev] = f
@@ -569,8 +571,8 @@ def embedding(table: torch.Tensor, ids: torch.Tensor, *, scale: float = 1.0, pad
               rng_base: Optional[torch.Tensor] = None, check: bool = True) -> torch.Tensor:
     """scale * table[ids], rows of `table` [V, D] (float32, bfloat16 or float16; rows may be strided) by integer `ids`
     (int32 or int64, any shape), as [*ids.shape, D] of `out_dtype` (default: the table's). scale is 0 or, over 1 - dropout,
-    of the size of a normal fp32 number. With dropout > 0 the result is
-    dropped out in the same kernel: the mask of `dropout()` over the result, with the same `rng` / `rng_base`.
+    of the size of a normal fp32 number. With dropout > 0 the result is dropped out in the same kernel: the mask of
+    `dropout()` over the result, with the same `rng` / `rng_base`.
 
     The gradient of the table sums the rows' gradients in fp32 in an order fixed by the call (sorted, no float atomics:
     the same bits on every run) and is dense: zeros for rows that no id names and for row `padding_idx` (which may count
